@@ -68,6 +68,11 @@ enum class WeightType { f32 = 0, f16 = 1, q4_0 = 2, rowwise_i8 = 3, q6_k = 4 };
 enum class ElementwiseOp { add = 0, multiply = 1, silu = 2, rms_norm = 3, scale = 4 };
 
 struct SwiGLULayout;
+struct KVCacheLayout;
+struct KVPagesLayout;
+struct KVAppendLayout;
+struct PagedAttentionLayout;
+struct LogitsLayout;
 
 // Per-call state owner: binds to the first device it is used on and owns
 // lazily grown device workspaces (reference k200.h:62-88).
@@ -88,6 +93,23 @@ private:
                               WeightType);
     friend void elementwise(Kernel &, int, void *, const void *, const void *, int, int, int, ElementwiseOp,
                             float);
+    friend bool paged_attention(Kernel &, int, void *, const void *, const void *, const void *, const int *,
+                                const int *, const KVCacheLayout &, const PagedAttentionLayout &);
+    friend bool kv_append(Kernel &, int, void *, void *, void *, const void *, const void *, const void *,
+                          const int *, const int *, const int *, const int *, const float *, const float *,
+                          const KVCacheLayout &, const KVAppendLayout &);
+    friend bool kv_reserve(Kernel &, int, int *, int *, int *, const int *, const int *, int,
+                           const KVCacheLayout &, const KVPagesLayout &);
+    friend bool kv_fork(Kernel &, int, void *, void *, int *, int *, int *, const int *, const int *, int,
+                        const KVCacheLayout &, const KVPagesLayout &);
+    friend bool kv_free(Kernel &, int, int *, int *, int *, const int *, int, const KVCacheLayout &,
+                        const KVPagesLayout &);
+    friend bool kv_compact(Kernel &, int, void *, void *, int *, int *, int *, const int *, const int *,
+                           const int *, const KVCacheLayout &, const KVPagesLayout &);
+    friend bool kv_copy_pages(Kernel &, int, void *, void *, const int *, const int *, int, const KVCacheLayout &,
+                              const KVPagesLayout &);
+    friend bool process_logits(Kernel &, int, void *, const void *, const float *, const int *, const int *,
+                               const int *, const float *, const int *, const uint32_t *, const LogitsLayout &);
 };
 
 // Packed rowwise INT8 weight layout (reference k200.h:90-96):
@@ -347,6 +369,132 @@ bool common_q4_matmul_pair(CommonQ4Workspace &, int device, void * y0, void * y1
                            const CommonQ4Weight & w1, const CommonQ4ActivationLease &, uint64_t generation);
 CommonQ4PairStatistics common_q4_pair_statistics(const CommonQ4Workspace &);
 CommonQ4PairStatus common_q4_pair_last_status(const CommonQ4Workspace &);
+
+// ---------------------------------------------------------------------------
+// Paged key-value cache and the operators on it and on logits (declared by this
+// library; the reference's own cache entry points are not). All of them submit
+// like matmul: select(device) + check(wait()) completes them. They return false,
+// with no work submitted, for arguments that break the rules stated here or
+// (the layouts' own rules) named by the *_reason functions, for a bad device, a
+// Kernel bound to another one, overlapping ranges where none are allowed, and
+// when a workspace cannot be allocated. Pointers are device memory.
+//
+// A pool holds F16 values of `pages` pages: value i of token t of head h of
+// page p is element p * page_stride + h * head_stride + t * token_stride + i.
+// Keys and values have a pool each, of the same layout. Either order within a
+// page (a head's tokens together, or a token's heads together) and any padding
+// may be given by the strides (in elements, multiples of 8); pools are 16-byte
+// aligned. Sequence s of a table holds its tokens in the pages
+// table[s * row_pages + token / page_tokens].
+struct KVCacheLayout {
+    int pages, page_tokens, heads, width;       // width: values of a head, a multiple of 8 up to 256
+    int64_t page_stride, head_stride, token_stride;
+};
+// "" or the first rule broken: "shape", "stride", "byte extent".
+const char * kv_cache_reason(const KVCacheLayout &);
+
+// What the kernels met on `device` since the last call, completing its work
+// first: 0, or a sum of 1 (a page id outside the pool; its tokens were left out),
+// 2 (a sequence, position or length out of range; left out or cut) and 4 (no
+// free page: the sequence kept its length, a fork's child is empty). -1: no such device.
+int kv_cache_status(int device);
+
+// One new token per sequence: y[s][h] = sum over tokens t of
+// softmax_t(scale * q[s][h] . k[s][t]) v[s][t], query heads sharing key-value
+// heads in equal groups (query head h uses head h / (query_heads / heads)).
+// t runs over the sequence's lengths[s] tokens, or the last `window` of them
+// (window 0: all); a sequence of length 0, and a row of which every weight is 0, give zeros. Pages before
+// the window and past the length are not read. `longest` bounds the lengths
+// (up to row_pages * page_tokens). q and y have rows of [query_heads][width] values of
+// `type`, q_stride and y_stride elements apart. F32 q and y get F32 arithmetic
+// (products of keys and weights split in two F16 parts, F32 sums and statistics).
+struct PagedAttentionLayout {
+    int sequences, query_heads, longest, window, row_pages;
+    int64_t q_stride, y_stride;
+    float scale;
+    InputType type;
+};
+// "" or the first rule broken of the two layouts: those of kv_cache_reason,
+// "type", "shape", "heads", "length", "scale", "stride".
+const char * paged_attention_reason(const KVCacheLayout &, const PagedAttentionLayout &);
+bool paged_attention(Kernel &, int device, void * y, const void * q, const void * k, const void * v,
+                     const int * table, const int * lengths, const KVCacheLayout &, const PagedAttentionLayout &);
+
+// Stores `tokens` new tokens: token i becomes token position[i] of sequence
+// sequence[i], whose table row already holds the page. With rotary > 0 the first `rotary`
+// values of each head of q and k are turned by the angle whose cosine and sine
+// stand in row position[i] of two [positions][rotary / 2] F32 tables: pair j is
+// values (2j, 2j + 1) (adjacent) or (j, j + rotary / 2) (halves). k, v rows of
+// [heads][width] and q rows of [query_heads][width] values of `type` are
+// *_stride elements apart, so that they may lie in one product's rows. Turned q
+// goes to q_out (q may be null, then query_heads is ignored; q_out may be q with
+// equal strides). k and v are rounded to F16 once. position null: token i is the
+// newest, lengths[i] - 1, of sequence i (sequence null too, tokens <= sequences). A
+// negative position or sequence marks a token that is left out; one out of range is left out and reported. Two tokens of one
+// call must not name one place.
+enum class RotaryPairs { adjacent, halves };
+struct KVAppendLayout {
+    int tokens, sequences, row_pages, query_heads;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    int rotary, positions;
+    RotaryPairs pairs;
+    InputType type;
+};
+const char * kv_append_reason(const KVCacheLayout &, const KVAppendLayout &);
+bool kv_append(Kernel &, int device, void * k_pool, void * v_pool, void * q_out, const void * q, const void * k,
+               const void * v, const int * sequence, const int * position, const int * lengths, const int * table,
+               const float * cosine, const float * sine, const KVCacheLayout &, const KVAppendLayout &);
+
+// The pages of `sequences` sequences: table [sequences][row_pages] (-1 past a
+// sequence's last page), lengths [sequences] in tokens, references [pages]
+// (how many rows hold a page; 0: free). `layers` pools stand layer_stride
+// elements apart and share the table. Lists are distinct sequences; entries out
+// of range are left out and reported. New pages are the lowest free ones, in list order.
+struct KVPagesLayout {
+    int sequences, row_pages, layers;
+    int64_t layer_stride;
+};
+const char * kv_pages_reason(const KVCacheLayout &, const KVPagesLayout &);
+// Makes room for added[i] more tokens of sequence rows[i] and adds them to its length.
+bool kv_reserve(Kernel &, int device, int * table, int * lengths, int * references, const int * rows,
+                const int * added, int count, const KVCacheLayout &, const KVPagesLayout &);
+// children[i] continues parents[i] as it stood before the call: full pages are
+// shared, a last page that is not full is copied to a page that was free before
+// the call. What a child held is released. A sequence may be parent of several
+// children, and a parent may itself be a child.
+bool kv_fork(Kernel &, int device, void * k, void * v, int * table, int * lengths, int * references,
+             const int * parents, const int * children, int count, const KVCacheLayout &, const KVPagesLayout &);
+// Releases what the listed sequences hold: rows -1, lengths 0.
+bool kv_free(Kernel &, int device, int * table, int * lengths, int * references, const int * rows, int count,
+             const KVCacheLayout &, const KVPagesLayout &);
+// Moves pages so that the U used ones are pages 0..U-1: the i-th free page below
+// U takes the i-th used page from U up. Writes the rows and counts that result
+// (table_out and references_out may be table and references) and U to *used.
+bool kv_compact(Kernel &, int device, void * k, void * v, int * table_out, int * references_out, int * used,
+                const int * table, const int * lengths, const int * references, const KVCacheLayout &,
+                const KVPagesLayout &);
+// Copies page sources[i] to destinations[i] in all layers (pairs with a negative
+// entry are left out). No destination may be named twice or be a source.
+bool kv_copy_pages(Kernel &, int device, void * k, void * v, const int * sources, const int * destinations,
+                   int count, const KVCacheLayout &, const KVPagesLayout &);
+
+// Logits before a token is chosen, F32, row by row: with n the times that token t
+// stands among the row's first history_lengths[row] history entries and
+// (r, f, p) = penalties[row], z = logits[t]; n > 0: z = z > 0 ? z / r : z * r; z
+// -= n f + (n > 0) p; z += the value of the row's last bias entry for t; then
+// -inf where bit t % 32 of mask word t / 32 is 0. penalties, history, bias_ids
+// and mask may be null (nothing of the kind; the bias arrays go together, history
+// needs penalties). Entries outside the vocabulary are left out. y may be logits
+// (equal strides). Strides are elements between rows.
+struct LogitsLayout {
+    int rows, vocabulary;
+    int64_t logits_stride, y_stride, history_stride, bias_stride, mask_stride;
+};
+const char * logits_reason(const LogitsLayout &);
+bool process_logits(Kernel &, int device, void * y, const void * logits, const float * penalties,
+                    const int * history, const int * history_lengths, const int * bias_ids,
+                    const float * bias_values, const int * bias_lengths, const uint32_t * mask,
+                    const LogitsLayout &);
 
 // Same layout as the reference (reference k200.h:345-350): matmul submissions
 // on devices 0 and 1, peer copy count and bytes.

@@ -240,6 +240,73 @@ enum { KUNLUN_NOALLOC_INVALID = -1, KUNLUN_NOALLOC_TOO_LARGE = -2 };
 int kunlun_matmul_noalloc(int device, void *y, const void *w, const void *x, int k, int n, int batch, int type,
                           void *stream, const char **route);
 
+/* Paged key-value cache and logits (declared by this library; see the comments
+ * in k200.h, which hold for these functions too). The structs have the fields of
+ * kunlun::KVCacheLayout, PagedAttentionLayout, KVAppendLayout, KVPagesLayout and
+ * LogitsLayout; type is a KUNLUN_INPUT_* and pairs a KUNLUN_ROTARY_* value. The
+ * operators submit like kunlun_matmul and return 1, or 0 when the arguments break
+ * a rule (nothing submitted, nothing aborted). */
+typedef struct {
+    int pages, page_tokens, heads, width;
+    int64_t page_stride, head_stride, token_stride;
+} kunlun_kv_cache_layout;
+typedef struct {
+    int sequences, query_heads, longest, window, row_pages;
+    int64_t q_stride, y_stride;
+    float scale;
+    int type;
+} kunlun_paged_attention_layout;
+enum { KUNLUN_ROTARY_ADJACENT = 0, KUNLUN_ROTARY_HALVES = 1 };
+typedef struct {
+    int tokens, sequences, row_pages, query_heads;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    int rotary, positions;
+    int pairs, type;
+} kunlun_kv_append_layout;
+typedef struct {
+    int sequences, row_pages, layers;
+    int64_t layer_stride;
+} kunlun_kv_pages_layout;
+typedef struct {
+    int rows, vocabulary;
+    int64_t logits_stride, y_stride, history_stride, bias_stride, mask_stride;
+} kunlun_logits_layout;
+/* kv_cache_reason() and the others: "" or the first rule broken. */
+const char *kunlun_kv_cache_reason(const kunlun_kv_cache_layout *cache);
+const char *kunlun_paged_attention_reason(const kunlun_kv_cache_layout *cache,
+                                          const kunlun_paged_attention_layout *call);
+const char *kunlun_kv_append_reason(const kunlun_kv_cache_layout *cache, const kunlun_kv_append_layout *call);
+const char *kunlun_kv_pages_reason(const kunlun_kv_cache_layout *cache, const kunlun_kv_pages_layout *pages);
+const char *kunlun_logits_reason(const kunlun_logits_layout *call);
+/* kv_cache_status(): completes the device's work; what its kernels met since the last call (a sum of these), -1: no such device. */
+enum { KUNLUN_KV_BAD_PAGE = 1, KUNLUN_KV_BAD_INDEX = 2, KUNLUN_KV_NO_PAGE = 4 };
+int kunlun_kv_cache_status(int device);
+int kunlun_paged_attention(kunlun_kernel *kernel, int device, void *y, const void *q, const void *k, const void *v,
+                           const int *table, const int *lengths, const kunlun_kv_cache_layout *cache,
+                           const kunlun_paged_attention_layout *call);
+int kunlun_kv_append(kunlun_kernel *kernel, int device, void *k_pool, void *v_pool, void *q_out, const void *q,
+                     const void *k, const void *v, const int *sequence, const int *position, const int *lengths,
+                     const int *table, const float *cosine, const float *sine, const kunlun_kv_cache_layout *cache,
+                     const kunlun_kv_append_layout *call);
+int kunlun_kv_reserve(kunlun_kernel *kernel, int device, int *table, int *lengths, int *references, const int *rows,
+                      const int *added, int count, const kunlun_kv_cache_layout *cache,
+                      const kunlun_kv_pages_layout *pages);
+int kunlun_kv_fork(kunlun_kernel *kernel, int device, void *k, void *v, int *table, int *lengths, int *references,
+                   const int *parents, const int *children, int count, const kunlun_kv_cache_layout *cache,
+                   const kunlun_kv_pages_layout *pages);
+int kunlun_kv_free(kunlun_kernel *kernel, int device, int *table, int *lengths, int *references, const int *rows,
+                   int count, const kunlun_kv_cache_layout *cache, const kunlun_kv_pages_layout *pages);
+int kunlun_kv_compact(kunlun_kernel *kernel, int device, void *k, void *v, int *table_out, int *references_out,
+                      int *used, const int *table, const int *lengths, const int *references,
+                      const kunlun_kv_cache_layout *cache, const kunlun_kv_pages_layout *pages);
+int kunlun_kv_copy_pages(kunlun_kernel *kernel, int device, void *k, void *v, const int *sources,
+                         const int *destinations, int count, const kunlun_kv_cache_layout *cache,
+                         const kunlun_kv_pages_layout *pages);
+int kunlun_process_logits(kunlun_kernel *kernel, int device, void *y, const void *logits, const float *penalties,
+                          const int *history, const int *history_lengths, const int *bias_ids,
+                          const float *bias_values, const int *bias_lengths, const uint32_t *mask,
+                          const kunlun_logits_layout *call);
+
 #ifdef __cplusplus
 }
 #endif

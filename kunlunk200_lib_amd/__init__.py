@@ -114,6 +114,20 @@ C_FUNCTIONS = [
                                               _c_void_p, ctypes.c_uint64]),
     ("kunlun_common_q4_pair_statistics", None, [_c_void_p, ctypes.POINTER(_c_size)]),
     ("kunlun_common_q4_pair_last_status", _c_int, [_c_void_p]),
+    ("kunlun_kv_cache_reason", ctypes.c_char_p, [_c_void_p]),
+    ("kunlun_paged_attention_reason", ctypes.c_char_p, [_c_void_p, _c_void_p]),
+    ("kunlun_kv_append_reason", ctypes.c_char_p, [_c_void_p, _c_void_p]),
+    ("kunlun_kv_pages_reason", ctypes.c_char_p, [_c_void_p, _c_void_p]),
+    ("kunlun_logits_reason", ctypes.c_char_p, [_c_void_p]),
+    ("kunlun_kv_cache_status", _c_int, [_c_int]),
+    ("kunlun_paged_attention", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 8),
+    ("kunlun_kv_append", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 14),
+    ("kunlun_kv_reserve", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 5 + [_c_int] + [_c_void_p] * 2),
+    ("kunlun_kv_fork", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int] + [_c_void_p] * 2),
+    ("kunlun_kv_free", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] + [_c_void_p] * 2),
+    ("kunlun_kv_compact", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 10),
+    ("kunlun_kv_copy_pages", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] + [_c_void_p] * 2),
+    ("kunlun_process_logits", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 10),
 ]
 
 
@@ -618,6 +632,141 @@ def common_q4_pair_statistics(workspace: CommonQ4Workspace) -> dict:
 
 def common_q4_pair_last_status(workspace: CommonQ4Workspace) -> CommonQ4PairStatus:
     return CommonQ4PairStatus(load().kunlun_common_q4_pair_last_status(workspace.handle))
+
+
+def _fields(*names, **types):
+    return [(n, types.get(n, _c_int)) for n in names]
+
+
+class KVCacheLayout(ctypes.Structure):
+    """F16 pools of pages: value i of token t of head h of page p is element
+    p * page_stride + h * head_stride + t * token_stride + i (include/kunlun/k200.h)."""
+    _fields_ = _fields("pages", "page_tokens", "heads", "width", "page_stride", "head_stride", "token_stride",
+                       page_stride=ctypes.c_int64, head_stride=ctypes.c_int64, token_stride=ctypes.c_int64)
+
+
+class PagedAttentionLayout(ctypes.Structure):
+    """One paged_attention call; q_stride and y_stride are elements between sequences, type an InputType."""
+    _fields_ = _fields("sequences", "query_heads", "longest", "window", "row_pages", "q_stride", "y_stride", "scale",
+                       "type", q_stride=ctypes.c_int64, y_stride=ctypes.c_int64, scale=ctypes.c_float)
+
+
+class RotaryPairs(enum.IntEnum):
+    """Which values of a head turn together: (2j, 2j + 1) or (j, j + rotary / 2)."""
+    adjacent = 0
+    halves = 1
+
+
+class KVAppendLayout(ctypes.Structure):
+    """One kv_append call; strides are elements between tokens."""
+    _fields_ = _fields("tokens", "sequences", "row_pages", "query_heads", "q_stride", "k_stride", "v_stride",
+                       "q_out_stride", "rotary", "positions", "pairs", "type", q_stride=ctypes.c_int64,
+                       k_stride=ctypes.c_int64, v_stride=ctypes.c_int64, q_out_stride=ctypes.c_int64)
+
+
+class KVPagesLayout(ctypes.Structure):
+    """The sequences of a table and the layers (pools layer_stride elements apart) that share it."""
+    _fields_ = _fields("sequences", "row_pages", "layers", "layer_stride", layer_stride=ctypes.c_int64)
+
+
+class LogitsLayout(ctypes.Structure):
+    """One process_logits call; strides are elements between rows (mask_stride 0: one mask for all rows)."""
+    _fields_ = _fields("rows", "vocabulary", "logits_stride", "y_stride", "history_stride", "bias_stride",
+                       "mask_stride", logits_stride=ctypes.c_int64, y_stride=ctypes.c_int64,
+                       history_stride=ctypes.c_int64, bias_stride=ctypes.c_int64, mask_stride=ctypes.c_int64)
+
+
+KV_BAD_PAGE, KV_BAD_INDEX, KV_NO_PAGE = 1, 2, 4
+
+
+def kv_cache_reason(cache: KVCacheLayout) -> str:
+    """"" when supported, else the first rule broken."""
+    return load().kunlun_kv_cache_reason(ctypes.byref(cache)).decode()
+
+
+def paged_attention_reason(cache: KVCacheLayout, call: PagedAttentionLayout) -> str:
+    return load().kunlun_paged_attention_reason(ctypes.byref(cache), ctypes.byref(call)).decode()
+
+
+def kv_append_reason(cache: KVCacheLayout, call: KVAppendLayout) -> str:
+    return load().kunlun_kv_append_reason(ctypes.byref(cache), ctypes.byref(call)).decode()
+
+
+def kv_pages_reason(cache: KVCacheLayout, pages: KVPagesLayout) -> str:
+    return load().kunlun_kv_pages_reason(ctypes.byref(cache), ctypes.byref(pages)).decode()
+
+
+def logits_reason(call: LogitsLayout) -> str:
+    return load().kunlun_logits_reason(ctypes.byref(call)).decode()
+
+
+def kv_cache_status(device: int) -> int:
+    """What the cache's kernels met since the last call (a sum of KV_* values), after completing
+    the device's work; -1 for no such device."""
+    return load().kunlun_kv_cache_status(int(device))
+
+
+def paged_attention(kernel: Kernel, device: int, y, q, k, v, table, lengths, cache: KVCacheLayout,
+                    call: PagedAttentionLayout) -> bool:
+    """Submit the attention of one new token per sequence over its pages; False when the
+    arguments break a rule (paged_attention_reason names the layouts')."""
+    return bool(load().kunlun_paged_attention(kernel.handle, int(device), _ptr(y), _ptr(q), _ptr(k), _ptr(v),
+                                              _ptr(table), _ptr(lengths), ctypes.byref(cache), ctypes.byref(call)))
+
+
+def kv_append(kernel: Kernel, device: int, k_pool, v_pool, q_out, q, k, v, sequence, position, lengths, table,
+              cosine, sine, cache: KVCacheLayout, call: KVAppendLayout) -> bool:
+    """Submit new tokens: q and k turned by their positions' angles, k and v stored into their pages."""
+    return bool(load().kunlun_kv_append(kernel.handle, int(device), _ptr(k_pool), _ptr(v_pool), _ptr(q_out), _ptr(q),
+                                        _ptr(k), _ptr(v), _ptr(sequence), _ptr(position), _ptr(lengths), _ptr(table),
+                                        _ptr(cosine), _ptr(sine), ctypes.byref(cache), ctypes.byref(call)))
+
+
+def kv_reserve(kernel: Kernel, device: int, table, lengths, references, rows, added, count: int,
+               cache: KVCacheLayout, pages: KVPagesLayout) -> bool:
+    """Submit: room for added[i] more tokens of sequence rows[i], on the lowest free pages."""
+    return bool(load().kunlun_kv_reserve(kernel.handle, int(device), _ptr(table), _ptr(lengths), _ptr(references),
+                                         _ptr(rows), _ptr(added), int(count), ctypes.byref(cache),
+                                         ctypes.byref(pages)))
+
+
+def kv_fork(kernel: Kernel, device: int, k, v, table, lengths, references, parents, children, count: int,
+            cache: KVCacheLayout, pages: KVPagesLayout) -> bool:
+    """Submit: children[i] continues parents[i], full pages shared and the last one copied."""
+    return bool(load().kunlun_kv_fork(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(table), _ptr(lengths),
+                                      _ptr(references), _ptr(parents), _ptr(children), int(count),
+                                      ctypes.byref(cache), ctypes.byref(pages)))
+
+
+def kv_free(kernel: Kernel, device: int, table, lengths, references, rows, count: int, cache: KVCacheLayout,
+            pages: KVPagesLayout) -> bool:
+    """Submit: what the listed sequences hold is released."""
+    return bool(load().kunlun_kv_free(kernel.handle, int(device), _ptr(table), _ptr(lengths), _ptr(references),
+                                      _ptr(rows), int(count), ctypes.byref(cache), ctypes.byref(pages)))
+
+
+def kv_compact(kernel: Kernel, device: int, k, v, table_out, references_out, used, table, lengths, references,
+               cache: KVCacheLayout, pages: KVPagesLayout) -> bool:
+    """Submit: the used pages become the lowest ones; *used is how many there are."""
+    return bool(load().kunlun_kv_compact(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(table_out),
+                                         _ptr(references_out), _ptr(used), _ptr(table), _ptr(lengths),
+                                         _ptr(references), ctypes.byref(cache), ctypes.byref(pages)))
+
+
+def kv_copy_pages(kernel: Kernel, device: int, k, v, sources, destinations, count: int, cache: KVCacheLayout,
+                  pages: KVPagesLayout) -> bool:
+    """Submit: page sources[i] copied to destinations[i] in all layers."""
+    return bool(load().kunlun_kv_copy_pages(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(sources),
+                                            _ptr(destinations), int(count), ctypes.byref(cache),
+                                            ctypes.byref(pages)))
+
+
+def process_logits(kernel: Kernel, device: int, y, logits, penalties, history, history_lengths, bias_ids,
+                   bias_values, bias_lengths, mask, call: LogitsLayout) -> bool:
+    """Submit: penalties for repeated tokens, biases and a mask on rows of F32 logits."""
+    return bool(load().kunlun_process_logits(kernel.handle, int(device), _ptr(y), _ptr(logits), _ptr(penalties),
+                                             _ptr(history), _ptr(history_lengths), _ptr(bias_ids),
+                                             _ptr(bias_values), _ptr(bias_lengths), _ptr(mask), ctypes.byref(call)))
 
 
 def statistics() -> dict:

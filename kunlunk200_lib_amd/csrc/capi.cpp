@@ -30,6 +30,31 @@ kunlun::InputType input_type(int type) {
     kunlun::require(type == KUNLUN_INPUT_F32 || type == KUNLUN_INPUT_F16);
     return type == KUNLUN_INPUT_F16 ? kunlun::InputType::f16 : kunlun::InputType::f32;
 }
+
+// The C structs as the C++ ones; unknown enumeration values are kept for the rules to refuse.
+kunlun::KVCacheLayout layout(const kunlun_kv_cache_layout & c) {
+    return {c.pages, c.page_tokens, c.heads, c.width, c.page_stride, c.head_stride, c.token_stride};
+}
+kunlun::PagedAttentionLayout layout(const kunlun_paged_attention_layout & p) {
+    return {p.sequences, p.query_heads, p.longest, p.window, p.row_pages, p.q_stride, p.y_stride, p.scale,
+            static_cast<kunlun::InputType>(p.type)};
+}
+kunlun::KVAppendLayout layout(const kunlun_kv_append_layout & p) {
+    return {p.tokens, p.sequences, p.row_pages, p.query_heads, p.q_stride, p.k_stride, p.v_stride, p.q_out_stride,
+            p.rotary, p.positions, static_cast<kunlun::RotaryPairs>(p.pairs), static_cast<kunlun::InputType>(p.type)};
+}
+kunlun::KVPagesLayout layout(const kunlun_kv_pages_layout & p) {
+    return {p.sequences, p.row_pages, p.layers, p.layer_stride};
+}
+kunlun::LogitsLayout layout(const kunlun_logits_layout & p) {
+    return {p.rows, p.vocabulary, p.logits_stride, p.y_stride, p.history_stride, p.bias_stride, p.mask_stride};
+}
+
+// 1 and the route noted on the handle, or 0.
+int done(kunlun_kernel * kernel, bool submitted) {
+    if (submitted) kernel->route = kunlun::detail::route_of_last_matmul();
+    return submitted ? 1 : 0;
+}
 } // namespace
 
 extern "C" {
@@ -291,5 +316,81 @@ void kunlun_matmul_swiglu(kunlun_kernel * kernel, int device, void * y, const vo
 size_t kunlun_matmul_count(int device) { return kunlun::detail::matmul_count(device); }
 void * kunlun_stream(int device) { return static_cast<void *>(kunlun::detail::context(device).stream); }
 const char * kunlun_kernel_route(const kunlun_kernel * kernel) { return kernel ? kernel->route : nullptr; }
+
+const char * kunlun_kv_cache_reason(const kunlun_kv_cache_layout * cache) {
+    return cache ? kunlun::kv_cache_reason(layout(*cache)) : "shape";
+}
+const char * kunlun_paged_attention_reason(const kunlun_kv_cache_layout * cache,
+                                           const kunlun_paged_attention_layout * call) {
+    return cache && call ? kunlun::paged_attention_reason(layout(*cache), layout(*call)) : "shape";
+}
+const char * kunlun_kv_append_reason(const kunlun_kv_cache_layout * cache, const kunlun_kv_append_layout * call) {
+    return cache && call ? kunlun::kv_append_reason(layout(*cache), layout(*call)) : "shape";
+}
+const char * kunlun_kv_pages_reason(const kunlun_kv_cache_layout * cache, const kunlun_kv_pages_layout * pages) {
+    return cache && pages ? kunlun::kv_pages_reason(layout(*cache), layout(*pages)) : "shape";
+}
+const char * kunlun_logits_reason(const kunlun_logits_layout * call) {
+    return call ? kunlun::logits_reason(layout(*call)) : "shape";
+}
+int kunlun_kv_cache_status(int device) { return kunlun::kv_cache_status(device); }
+
+int kunlun_paged_attention(kunlun_kernel * kernel, int device, void * y, const void * q, const void * k,
+                           const void * v, const int * table, const int * lengths,
+                           const kunlun_kv_cache_layout * cache, const kunlun_paged_attention_layout * call) {
+    return kernel && cache && call &&
+           done(kernel, kunlun::paged_attention(kernel->kernel, device, y, q, k, v, table, lengths, layout(*cache),
+                                                layout(*call)));
+}
+int kunlun_kv_append(kunlun_kernel * kernel, int device, void * k_pool, void * v_pool, void * q_out, const void * q,
+                     const void * k, const void * v, const int * sequence, const int * position, const int * lengths,
+                     const int * table, const float * cosine, const float * sine,
+                     const kunlun_kv_cache_layout * cache, const kunlun_kv_append_layout * call) {
+    return kernel && cache && call &&
+           done(kernel, kunlun::kv_append(kernel->kernel, device, k_pool, v_pool, q_out, q, k, v, sequence, position,
+                                          lengths, table, cosine, sine, layout(*cache), layout(*call)));
+}
+int kunlun_kv_reserve(kunlun_kernel * kernel, int device, int * table, int * lengths, int * references,
+                      const int * rows, const int * added, int count, const kunlun_kv_cache_layout * cache,
+                      const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_reserve(kernel->kernel, device, table, lengths, references, rows, added, count,
+                                           layout(*cache), layout(*pages)));
+}
+int kunlun_kv_fork(kunlun_kernel * kernel, int device, void * k, void * v, int * table, int * lengths,
+                   int * references, const int * parents, const int * children, int count,
+                   const kunlun_kv_cache_layout * cache, const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_fork(kernel->kernel, device, k, v, table, lengths, references, parents, children,
+                                        count, layout(*cache), layout(*pages)));
+}
+int kunlun_kv_free(kunlun_kernel * kernel, int device, int * table, int * lengths, int * references, const int * rows,
+                   int count, const kunlun_kv_cache_layout * cache, const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_free(kernel->kernel, device, table, lengths, references, rows, count,
+                                        layout(*cache), layout(*pages)));
+}
+int kunlun_kv_compact(kunlun_kernel * kernel, int device, void * k, void * v, int * table_out, int * references_out,
+                      int * used, const int * table, const int * lengths, const int * references,
+                      const kunlun_kv_cache_layout * cache, const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_compact(kernel->kernel, device, k, v, table_out, references_out, used, table,
+                                           lengths, references, layout(*cache), layout(*pages)));
+}
+int kunlun_kv_copy_pages(kunlun_kernel * kernel, int device, void * k, void * v, const int * sources,
+                         const int * destinations, int count, const kunlun_kv_cache_layout * cache,
+                         const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_copy_pages(kernel->kernel, device, k, v, sources, destinations, count,
+                                              layout(*cache), layout(*pages)));
+}
+int kunlun_process_logits(kunlun_kernel * kernel, int device, void * y, const void * logits, const float * penalties,
+                          const int * history, const int * history_lengths, const int * bias_ids,
+                          const float * bias_values, const int * bias_lengths, const uint32_t * mask,
+                          const kunlun_logits_layout * call) {
+    return kernel && call &&
+           done(kernel, kunlun::process_logits(kernel->kernel, device, y, logits, penalties, history, history_lengths,
+                                               bias_ids, bias_values, bias_lengths, mask, layout(*call)));
+}
 
 }

@@ -1,0 +1,475 @@
+// Pages of a paged key-value cache: taken, shared, copied, moved and given back
+// by reference counts.
+//
+// What has to be decided in order (which free page goes to which sequence, which page
+// moves where) is decided by one workgroup with prefix sums over the reference
+// counts, in the order of page numbers and of the caller's list, so that the
+// same calls give the same tables every time; counts themselves change by
+// integer atomics. What moves data (rows, pages) follows in a second launch over the
+// whole card and is bound by the bytes it copies.
+#include "device_common.h"
+#include "launch.h"
+#include "paged.h"
+
+#include <algorithm>
+
+namespace {
+
+using kk::kWave;
+using kk::PoolView;
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr int kCopyThreads = 256;
+
+struct PagesArgs {
+    _Float16 *k, *v;
+    int *table, *lengths, *references;
+    int *status;
+    PoolView pool;
+    int64_t layer_stride;
+    int sequences, row_pages, layers;
+};
+
+// Sum of `v` over the threads before this one; `total` over all of them. Ends
+// with a barrier, so it may be called again at once.
+template <typename T>
+__device__ __forceinline__ T prefix(T v, T &total, T *scratch) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    T sum = v;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const T other = __shfl_up(sum, o, kWave);
+        if (lane >= o) sum += other;
+    }
+    if (lane == kWave - 1) scratch[wave] = sum;
+    __syncthreads();
+    T before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+        const T x = scratch[w];
+        before += w < wave ? x : 0;
+        total += x;
+    }
+    __syncthreads();
+    return before + sum - v;
+}
+
+// Writes the lowest `wanted` free pages to found[] in order; returns how many there are.
+__device__ __forceinline__ int free_pages(const int *references, int pages, int wanted, int *found, int *scratch) {
+    int have = 0;
+    for (int p0 = 0; p0 < pages && have < wanted; p0 += kPlanThreads) {
+        const int p = p0 + threadIdx.x;
+        const bool is_free = p < pages && references[p] == 0;
+        int total;
+        const int at = have + prefix<int>(is_free, total, scratch);
+        if (is_free && at < wanted) found[at] = p;
+        have += total;
+    }
+    __syncthreads();
+    return min(have, wanted);
+}
+
+__device__ __forceinline__ int pages_of(const PagesArgs &a, int tokens) {
+    return a.pool.per_page.div(tokens + a.pool.page_tokens - 1);
+}
+// A length as it can be: within the row.
+__device__ __forceinline__ int length_of(const PagesArgs &a, int s) {
+    const int len = a.lengths[s];
+    const int64_t most = (int64_t)a.row_pages * a.pool.page_tokens;
+    if (len < 0 || len > most) {
+        kk::report(a.status, kk::kBadIndex);
+        return len < 0 ? 0 : static_cast<int>(most);
+    }
+    return len;
+}
+__device__ __forceinline__ bool sequence_ok(const PagesArgs &a, int s) {
+    if (static_cast<unsigned>(s) < static_cast<unsigned>(a.sequences)) return true;
+    kk::report(a.status, kk::kBadIndex);
+    return false;
+}
+// Gives back the first n pages of a row.
+__device__ __forceinline__ void release_row(const PagesArgs &a, const int *row, int n) {
+    for (int j = threadIdx.x; j < n; j += blockDim.x) {
+        const int page = row[j];
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pool.pages)) atomicSub(&a.references[page], 1);
+        else kk::report(a.status, kk::kBadPage);
+    }
+}
+
+// ---- kv_reserve ----------------------------------------------------------------------------
+
+__global__ __launch_bounds__(kPlanThreads) void reserve(PagesArgs a, const int *rows, const int *added, int count,
+                                                        int *need_of, int *first_of, int *found) {
+    __shared__ int scratch[kPlanWaves];
+    __shared__ long long sums[kPlanWaves];
+    int64_t wanted = 0;
+    for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
+        const int i = i0 + threadIdx.x;
+        int need = -1;                           // -1: left out
+        if (i < count && sequence_ok(a, rows[i])) {
+            const int64_t len = length_of(a, rows[i]), more = added[i];
+            if (more >= 0 && len + more <= (int64_t)a.row_pages * a.pool.page_tokens)
+                need = pages_of(a, static_cast<int>(len + more)) - pages_of(a, static_cast<int>(len));
+            else
+                kk::report(a.status, kk::kBadIndex);
+        }
+        long long total;
+        const int64_t at = wanted + prefix<long long>(max(need, 0), total, sums);
+        if (i < count) {
+            need_of[i] = need;
+            // past the pool's size no page is left for it
+            first_of[i] = static_cast<int>(min<int64_t>(at, a.pool.pages));
+        }
+        wanted += total;
+    }
+    const int have = free_pages(a.references, a.pool.pages, static_cast<int>(min<int64_t>(wanted, a.pool.pages)),
+                                found, scratch);
+    // a wave for each listed sequence
+    for (int i = threadIdx.x / kWave; i < count; i += kPlanWaves) {
+        const int need = need_of[i], first = first_of[i];
+        if (need < 0) continue;
+        if (need > 0 && (int64_t)first + need > have) {
+            if (threadIdx.x % kWave == 0) kk::report(a.status, kk::kNoPage);
+            continue;
+        }
+        const int s = rows[i], len = length_of(a, s), held = pages_of(a, len);
+        for (int j = threadIdx.x % kWave; j < need; j += kWave) {
+            const int page = found[first + j];
+            a.table[(int64_t)s * a.row_pages + held + j] = page;
+            a.references[page] = 1;
+        }
+        if (threadIdx.x % kWave == 0) a.lengths[s] = len + added[i];
+    }
+}
+
+// ---- kv_fork -------------------------------------------------------------------------------
+
+// What the first launch finds out of fork i: the parent's length (-1: left out), and the page that
+// its last, not full page is copied to (-1: there is none, -2: no page was free).
+struct ForkNote {
+    int length, page;
+};
+
+// Workgroup 0 finds the pages; workgroup 1 + i copies the parent's row aside (a
+// parent may be a child whose row the second launch overwrites).
+__global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int *parents, const int *children,
+                                                          int count, ForkNote *notes, int *found, int *rows) {
+    if (blockIdx.x > 0) {
+        const int i = blockIdx.x - 1, s = parents[i];
+        if (static_cast<unsigned>(s) >= static_cast<unsigned>(a.sequences)) return;
+        const int n = pages_of(a, length_of(a, s));
+        for (int j = threadIdx.x; j < n; j += kPlanThreads)
+            rows[(int64_t)i * a.row_pages + j] = a.table[(int64_t)s * a.row_pages + j];
+        return;
+    }
+    __shared__ int scratch[kPlanWaves];
+    int wanted = 0;
+    for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
+        const int i = i0 + threadIdx.x;
+        int length = -1;
+        if (i < count && sequence_ok(a, parents[i]) && sequence_ok(a, children[i])) length = length_of(a, parents[i]);
+        const bool part = length > 0 && length % a.pool.page_tokens != 0;
+        int total;
+        const int at = wanted + prefix<int>(part, total, scratch);
+        if (i < count) notes[i] = ForkNote{length, part ? at : -1};
+        wanted += total;
+    }
+    const int have = free_pages(a.references, a.pool.pages, min(wanted, a.pool.pages), found, scratch);
+    for (int i = threadIdx.x; i < count; i += kPlanThreads) {
+        const int at = notes[i].page;
+        if (at >= 0) notes[i].page = at < have ? found[at] : -2;
+        if (at >= have && at >= 0) kk::report(a.status, kk::kNoPage);
+    }
+}
+
+// Fork i: its first workgroup releases the child's pages and writes the child's row,
+// the others copy the tokens of the parent's last page.
+__global__ __launch_bounds__(kCopyThreads) void fork_apply(PagesArgs a, const int *children, const ForkNote *notes,
+                                                           const int *rows) {
+    const int i = blockIdx.y;
+    const ForkNote note = notes[i];
+    if (note.length < 0) return;
+    const int full = a.pool.per_page.div(note.length), rest = note.length - full * a.pool.page_tokens;
+    const int *from = rows + (int64_t)i * a.row_pages;
+    if (blockIdx.x == 0) {
+        const int s = children[i];
+        int *row = a.table + (int64_t)s * a.row_pages;
+        const int old = pages_of(a, length_of(a, s));
+        release_row(a, row, old);
+        __syncthreads();
+        const int kept = note.page == -2 ? 0 : full;
+        for (int j = threadIdx.x; j < a.row_pages; j += kCopyThreads) {
+            int page = -1;
+            if (j < kept) {
+                page = from[j];
+                if (static_cast<unsigned>(page) < static_cast<unsigned>(a.pool.pages)) atomicAdd(&a.references[page], 1);
+                else kk::report(a.status, kk::kBadPage);
+            } else if (j == full && note.page >= 0) {
+                page = note.page;
+                atomicAdd(&a.references[page], 1);
+            }
+            row[j] = page;
+        }
+        if (threadIdx.x == 0) a.lengths[s] = note.page == -2 ? 0 : note.length;
+        return;
+    }
+    if (note.page < 0) return;
+    const int page = from[full];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.pages)) {
+        if (blockIdx.x == 1 && threadIdx.x == 0) kk::report(a.status, kk::kBadPage);
+        return;
+    }
+    // 16 bytes a thread: a (layer, pool, head) at a time, its rows of `rest` tokens
+    const int row_vectors = a.pool.width / 8, vectors = rest * row_vectors;
+    const int blocks = a.layers * 2 * a.pool.heads;
+    for (int b = blockIdx.x - 1; b < blocks; b += gridDim.x - 1) {
+        const int head = b % a.pool.heads, pool = b / a.pool.heads % 2, layer = b / a.pool.heads / 2;
+        _Float16 *base = (pool ? a.v : a.k) + layer * a.layer_stride + head * a.pool.head_stride;
+        const _Float16 *src = base + page * a.pool.page_stride;
+        _Float16 *dst = base + note.page * a.pool.page_stride;
+        for (int x = threadIdx.x; x < vectors; x += kCopyThreads) {
+            const int token = x / row_vectors, at = x - token * row_vectors;
+            const int64_t off = token * a.pool.token_stride + at * 8;
+            *reinterpret_cast<uint4 *>(dst + off) = *reinterpret_cast<const uint4 *>(src + off);
+        }
+    }
+}
+
+// ---- kv_free -------------------------------------------------------------------------------
+
+__global__ __launch_bounds__(kCopyThreads) void free_rows(PagesArgs a, const int *list) {
+    const int s = list[blockIdx.x];
+    if (static_cast<unsigned>(s) >= static_cast<unsigned>(a.sequences)) {
+        if (threadIdx.x == 0) kk::report(a.status, kk::kBadIndex);
+        return;
+    }
+    // of two entries that name one sequence only one finds its length
+    __shared__ int length;
+    if (threadIdx.x == 0) length = atomicExch(&a.lengths[s], 0);
+    __syncthreads();
+    const int64_t most = (int64_t)a.row_pages * a.pool.page_tokens;
+    if (length < 0 || length > most) {
+        if (threadIdx.x == 0) kk::report(a.status, kk::kBadIndex);
+    }
+    const int n = pages_of(a, length < 0 ? 0 : static_cast<int>(min<int64_t>(length, most)));
+    int *row = a.table + (int64_t)s * a.row_pages;
+    release_row(a, row, n);
+    for (int j = threadIdx.x; j < n; j += kCopyThreads) row[j] = -1;
+}
+
+// ---- kv_compact ----------------------------------------------------------------------------
+
+// One workgroup: U, then the lists of holes below U and of used pages from U up.
+__global__ __launch_bounds__(kPlanThreads) void compact_plan(const int *references, int *references_out, int pages,
+                                                             int *used_out, int *moves, int *holes, int *movers,
+                                                             int *place) {
+    __shared__ int scratch[kPlanWaves];
+    int used = 0;
+    for (int p0 = 0; p0 < pages; p0 += kPlanThreads) {
+        const int p = p0 + threadIdx.x;
+        int total;
+        prefix<int>(p < pages && references[p] > 0, total, scratch);
+        used += total;
+    }
+    int n_holes = 0, n_movers = 0;
+    for (int p0 = 0; p0 < pages; p0 += kPlanThreads) {
+        const int p = p0 + threadIdx.x;
+        const bool taken = p < pages && references[p] > 0;
+        int total;
+        const bool hole = p < used && !taken;
+        const int h = n_holes + prefix<int>(hole, total, scratch);
+        n_holes += total;
+        const bool mover = p >= used && taken;
+        const int m = n_movers + prefix<int>(mover, total, scratch);
+        n_movers += total;
+        if (hole) holes[h] = p;
+        if (mover) movers[m] = p;
+        else if (p >= used && p < pages) place[p] = p;   // named by no count: a row that names it keeps it
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_movers; i += kPlanThreads) place[movers[i]] = holes[i];
+    // counts: the used pages below U keep theirs, holes take their mover's; then 0 from U up
+    if (references_out != references)
+        for (int p = threadIdx.x; p < used; p += kPlanThreads) references_out[p] = references[p];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_movers; i += kPlanThreads) references_out[holes[i]] = references[movers[i]];
+    __syncthreads();
+    for (int p = used + threadIdx.x; p < pages; p += kPlanThreads) references_out[p] = 0;
+    if (threadIdx.x == 0) {
+        *used_out = used;
+        *moves = n_movers;
+    }
+}
+
+// Copies page src to dst in one layer's pool; the workgroup takes part `part` of
+// `parts`. DENSE: a page is one run of values.
+template <bool DENSE>
+__device__ __forceinline__ void copy_page(const PagesArgs &a, _Float16 *pool, int src, int dst, int part, int parts) {
+    const _Float16 *from = pool + src * a.pool.page_stride;
+    _Float16 *to = pool + dst * a.pool.page_stride;
+    const int row_vectors = a.pool.width / 8;
+    const int64_t vectors = (int64_t)a.pool.heads * a.pool.page_tokens * row_vectors;
+    for (int64_t x = (int64_t)part * kCopyThreads + threadIdx.x; x < vectors; x += (int64_t)parts * kCopyThreads) {
+        int64_t off = x * 8;
+        if constexpr (!DENSE) {
+            const int64_t row = x / row_vectors;
+            const int head = static_cast<int>(row / a.pool.page_tokens), token = static_cast<int>(row % a.pool.page_tokens);
+            off = head * a.pool.head_stride + token * a.pool.token_stride + (x - row * row_vectors) * 8;
+        }
+        *reinterpret_cast<uint4 *>(to + off) = *reinterpret_cast<const uint4 *>(from + off);
+    }
+}
+
+// Pages sources[i] -> destinations[i], i < *count: work items are (pair, layer, pool, part).
+template <bool DENSE>
+__device__ __forceinline__ void copy_pairs(const PagesArgs &a, const int *sources, const int *destinations, int count,
+                                           int parts, int item, int step) {
+    const int per_pair = a.layers * 2 * parts;
+    const int64_t items = (int64_t)count * per_pair;
+    for (int64_t x = item; x < items; x += step) {
+        const int i = static_cast<int>(x / per_pair), rest = static_cast<int>(x - (int64_t)i * per_pair);
+        const int part = rest % parts, pool = rest / parts % 2, layer = rest / parts / 2;
+        const int src = sources[i], dst = destinations[i];
+        if (src < 0 || dst < 0) continue;
+        if (src >= a.pool.pages || dst >= a.pool.pages) {
+            if (rest == 0 && threadIdx.x == 0) kk::report(a.status, kk::kBadPage);
+            continue;
+        }
+        copy_page<DENSE>(a, (pool ? a.v : a.k) + layer * a.layer_stride, src, dst, part, parts);
+    }
+}
+
+template <bool DENSE>
+__global__ __launch_bounds__(kCopyThreads) void copy_pages(PagesArgs a, const int *sources, const int *destinations,
+                                                           int count, int parts) {
+    copy_pairs<DENSE>(a, sources, destinations, count, parts, blockIdx.x, gridDim.x);
+}
+
+// The first row_groups workgroups rewrite the table, the others move the pages.
+template <bool DENSE>
+__global__ __launch_bounds__(kCopyThreads) void compact_apply(PagesArgs a, const int *table, const int *used,
+                                                              const int *moves, const int *holes, const int *movers,
+                                                              const int *place, int parts, int row_groups) {
+    if (static_cast<int>(blockIdx.x) >= row_groups) {
+        copy_pairs<DENSE>(a, movers, holes, *moves, parts, blockIdx.x - row_groups, gridDim.x - row_groups);
+        return;
+    }
+    const int u = *used;
+    for (int s = blockIdx.x; s < a.sequences; s += row_groups) {
+        const int n = pages_of(a, length_of(a, s));
+        for (int j = threadIdx.x; j < a.row_pages; j += kCopyThreads) {
+            const int64_t at = (int64_t)s * a.row_pages + j;
+            int page = table[at];
+            if (j < n) {
+                if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.pages)) kk::report(a.status, kk::kBadPage);
+                else if (page >= u) page = place[page];
+            }
+            a.table[at] = page;
+        }
+    }
+}
+
+PagesArgs args_of(void *k, void *v, int *table, int *lengths, int *references, const kunlun::KVCacheLayout &c,
+                  const kunlun::KVPagesLayout &p, int *status) {
+    PagesArgs a;
+    a.k = static_cast<_Float16 *>(k);
+    a.v = static_cast<_Float16 *>(v);
+    a.table = table;
+    a.lengths = lengths;
+    a.references = references;
+    a.status = status;
+    a.pool = PoolView(c);
+    a.layer_stride = p.layer_stride;
+    a.sequences = p.sequences;
+    a.row_pages = p.row_pages;
+    a.layers = p.layers;
+    return a;
+}
+
+// A page is one run of values, in either order.
+bool dense(const kunlun::KVCacheLayout &c) {
+    const int64_t w = c.width;
+    const bool heads = (c.page_tokens == 1 || c.token_stride == w) && (c.heads == 1 || c.head_stride == w * c.page_tokens);
+    const bool tokens = (c.heads == 1 || c.head_stride == w) && (c.page_tokens == 1 || c.token_stride == w * c.heads);
+    return heads || tokens;
+}
+
+// Workgroups that share a page's values in one pool: 16 KiB each.
+int parts_of(const kunlun::KVCacheLayout &c) {
+    const int64_t bytes = (int64_t)c.heads * c.page_tokens * c.width * 2;
+    return static_cast<int>(std::min<int64_t>(64, (bytes + 16383) / 16384));
+}
+
+} // namespace
+
+extern "C" size_t kk_kv_reserve_workspace_bytes(const kunlun::KVCacheLayout &c, int count) {
+    return ((size_t)2 * count + c.pages) * sizeof(int);
+}
+extern "C" int kk_kv_reserve(int *table, int *lengths, int *references, const int *rows, const int *added, int count,
+                  const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
+                  hipStream_t stream) {
+    int *need = static_cast<int *>(workspace);
+    hipLaunchKernelGGL(reserve, dim3(1), dim3(kPlanThreads), 0, stream,
+                       args_of(nullptr, nullptr, table, lengths, references, c, p, status), rows, added, count, need,
+                       need + count, need + 2 * (size_t)count);
+    return hipGetLastError();
+}
+
+extern "C" size_t kk_kv_fork_workspace_bytes(const kunlun::KVPagesLayout &p, int count) {
+    return (size_t)count * (sizeof(ForkNote) + sizeof(int) + (size_t)p.row_pages * sizeof(int));
+}
+extern "C" int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *references, const int *parents, const int *children,
+               int count, const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
+               hipStream_t stream) {
+    const PagesArgs a = args_of(k, v, table, lengths, references, c, p, status);
+    ForkNote *notes = static_cast<ForkNote *>(workspace);
+    int *found = reinterpret_cast<int *>(notes + count), *rows = found + count;
+    hipLaunchKernelGGL(fork_plan, dim3(1 + count), dim3(kPlanThreads), 0, stream, a, parents, children, count, notes,
+                       found, rows);
+    // at most eight (layer, pool, head) blocks of the last page per workgroup
+    const int blocks = p.layers * 2 * c.heads, copiers = std::max(1, std::min(blocks, 4096 / count));
+    hipLaunchKernelGGL(fork_apply, dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);
+    return hipGetLastError();
+}
+
+extern "C" int kk_kv_free(int *table, int *lengths, int *references, const int *rows, int count, const kunlun::KVCacheLayout &c,
+               const kunlun::KVPagesLayout &p, int *status, hipStream_t stream) {
+    hipLaunchKernelGGL(free_rows, dim3(count), dim3(kCopyThreads), 0, stream,
+                       args_of(nullptr, nullptr, table, lengths, references, c, p, status), rows);
+    return hipGetLastError();
+}
+
+extern "C" size_t kk_kv_compact_workspace_bytes(const kunlun::KVCacheLayout &c) { return ((size_t)3 * c.pages + 64) * sizeof(int); }
+extern "C" int kk_kv_compact(void *k, void *v, int *table_out, int *references_out, int *used, const int *table,
+                  const int *lengths, const int *references, const kunlun::KVCacheLayout &c,
+                  const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus, hipStream_t stream) {
+    int *moves = static_cast<int *>(workspace), *holes = moves + 64, *movers = holes + c.pages, *place = movers + c.pages;
+    hipLaunchKernelGGL(compact_plan, dim3(1), dim3(kPlanThreads), 0, stream, references, references_out, c.pages, used,
+                       moves, holes, movers, place);
+    const PagesArgs a = args_of(k, v, table_out, const_cast<int *>(lengths), nullptr, c, p, status);
+    const int groups = std::min(p.sequences, 256), parts = parts_of(c);
+    const dim3 grid(groups + 8 * cus);
+    if (dense(c))
+        hipLaunchKernelGGL(compact_apply<true>, grid, dim3(kCopyThreads), 0, stream, a, table, used, moves, holes,
+                           movers, place, parts, groups);
+    else
+        hipLaunchKernelGGL(compact_apply<false>, grid, dim3(kCopyThreads), 0, stream, a, table, used, moves, holes,
+                           movers, place, parts, groups);
+    return hipGetLastError();
+}
+
+extern "C" int kk_kv_copy_pages(void *k, void *v, const int *sources, const int *destinations, int count,
+                     const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, int *status, int cus,
+                     hipStream_t stream) {
+    const PagesArgs a = args_of(k, v, nullptr, nullptr, nullptr, c, p, status);
+    const int parts = parts_of(c);
+    const int64_t items = (int64_t)count * p.layers * 2 * parts;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(items, 8 * cus)));
+    if (dense(c))
+        hipLaunchKernelGGL(copy_pages<true>, grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
+    else
+        hipLaunchKernelGGL(copy_pages<false>, grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
+    return hipGetLastError();
+}

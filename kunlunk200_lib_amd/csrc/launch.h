@@ -5,6 +5,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <kunlun/k200.h>
 #include <cstddef>
 #include <cstdint>
 
@@ -143,5 +144,46 @@ int kk_i8_quantize(const float *x, int k, int batch, void *workspace, int *statu
 // the quantized activations in `workspace` with int8 weight rows W[n,k].
 int kk_i8_matmul(const void *workspace, const int8_t *w, const float *scales, const float *maxima,
                  float *y, int k, int n, int batch, hipStream_t stream, const char **route);
+
+// Attention of one new token per sequence over a paged cache (k200.h). The
+// workspace (kk_paged_attention_workspace_bytes, may be 0) holds the sums of
+// sequences split over several workgroups.
+size_t kk_paged_attention_workspace_bytes(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p,
+                                          int cus);
+int kk_paged_attention(void *y, const void *q, const void *k, const void *v, const int *table, const int *lengths,
+                       const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, void *workspace,
+                       int *status, int cus, hipStream_t stream);
+
+// New tokens into the cache (k200.h); q null: keys and values only.
+int kk_kv_append(void *k_pool, void *v_pool, void *q_out, const void *q, const void *k, const void *v,
+                 const int *sequence, const int *position, const int *lengths, const int *table, const float *cosine,
+                 const float *sine, const kunlun::KVCacheLayout &c, const kunlun::KVAppendLayout &p, int *status,
+                 hipStream_t stream);
+
+// Pages taken, shared, given back, moved and copied (k200.h), each with the
+// bytes of workspace it needs.
+size_t kk_kv_reserve_workspace_bytes(const kunlun::KVCacheLayout &c, int count);
+int kk_kv_reserve(int *table, int *lengths, int *references, const int *rows, const int *added, int count,
+                  const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
+                  hipStream_t stream);
+size_t kk_kv_fork_workspace_bytes(const kunlun::KVPagesLayout &p, int count);
+int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *references, const int *parents, const int *children,
+               int count, const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
+               hipStream_t stream);
+int kk_kv_free(int *table, int *lengths, int *references, const int *rows, int count, const kunlun::KVCacheLayout &c,
+               const kunlun::KVPagesLayout &p, int *status, hipStream_t stream);
+size_t kk_kv_compact_workspace_bytes(const kunlun::KVCacheLayout &c);
+int kk_kv_compact(void *k, void *v, int *table_out, int *references_out, int *used, const int *table,
+                  const int *lengths, const int *references, const kunlun::KVCacheLayout &c,
+                  const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus, hipStream_t stream);
+int kk_kv_copy_pages(void *k, void *v, const int *sources, const int *destinations, int count,
+                     const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, int *status, int cus,
+                     hipStream_t stream);
+
+// Penalties, biases and a mask on rows of logits (k200.h).
+int kk_process_logits(float *y, const float *logits, const float *penalties, const int *history,
+                      const int *history_lengths, const int *bias_ids, const float *bias_values,
+                      const int *bias_lengths, const uint32_t *mask, const kunlun::LogitsLayout &p,
+                      hipStream_t stream);
 
 }

@@ -171,6 +171,7 @@ Kernel::~Kernel() {
         release(impl_->id, impl_->i8_workspace, impl_->i8_workspace_size);
         release(impl_->id, impl_->gemm_workspace, impl_->gemm_workspace_size);
         release(impl_->id, impl_->pair_workspace, impl_->pair_workspace_size);
+        release(impl_->id, impl_->kv_workspace, impl_->kv_workspace_size);
     }
     delete impl_;
 }

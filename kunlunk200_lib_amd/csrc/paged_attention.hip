@@ -1,0 +1,472 @@
+// Attention of one new token per sequence over a paged F16 key-value cache.
+//
+// For query head h of sequence s, with key-value head h / group,
+//   y = sum_t w_t v_t / sum_t w_t,   w_t = exp(scale * q . k_t - m),
+// m the running maximum: one pass over keys and values, sums and statistics in
+// F32, exponents in base 2 (log2(e) goes into q).
+//
+// A workgroup takes one key-value head of one sequence (all of its query heads,
+// so that the cache is read once) over one chunk of tokens; its four waves
+// take steps of 32 tokens in turn. Both products run on
+// v_mfma_f32_16x16x32_f16 with the cache's rows as one operand:
+//   scores  [16 tokens x 16 columns] += K rows (as stored)  x  q columns
+//   outputs [16 values x 16 columns] += V transposed        x  weight columns
+// The score tiles leave lane (column c, group G) with tokens 4G..4G+3 of both
+// tiles of a step; V rows are loaded in that token order, so the weights go into the
+// second product where they are. A lane loads 8 consecutive values of 8 tokens
+// (16 lanes read whole rows) and picks value j of each by v_perm_b32: 32 per
+// step at width 128, against 1024 multiply-adds per lane and query head.
+//
+// Columns. The tile's 16 columns are 8 query heads twice: a factor x is split
+// into fp16 parts x = hi + lo (hi 11 bits, lo the next 11), hi in column c and lo in
+// column c + 8 of one tile; the two columns' sums are added at the end. So F32
+// queries and weights cost no instruction more than F16 ones with 8 query heads
+// or fewer, and errors stay at 2^-22. q is scaled by a power of two
+// (max |q| in [2^10, 2^11)) and the weights by 2^14, so that what the low
+// parts lose below 2^-24 stays far below that.
+//
+// What bounds it: reading the cache (4 * width bytes per token and head).
+//
+// Sequences of more than one chunk leave (sum w v, m, sum w) per chunk in the
+// workspace; a second launch joins them in order, so results do not
+// depend on the order in which chunks end.
+#include "device_common.h"
+#include "launch.h"
+#include "paged.h"
+
+#include <algorithm>
+
+namespace {
+
+using kk::half8;
+using kk::kWave;
+using kk::PoolView;
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kStep = 32;                // tokens of a wave's step
+constexpr int kMinChunk = kWaves * kStep;
+constexpr int kMaxChunk = 2048;
+constexpr float kWeightLog2 = 14.0f;     // weights are scaled by 2^14
+
+struct AttendArgs {
+    const _Float16 *k, *v;
+    const int *table, *lengths;
+    const void *q;
+    void *y;
+    float *part_o, *part_ml;             // [sequence][query head][chunk]: width sums; m and sum w
+    int *status;
+    PoolView pool;
+    int64_t q_stride, y_stride;
+    int query_heads, group, tiles, longest, window, row_pages, chunk, chunks, f16;
+    float scale_log2;
+};
+
+__device__ __forceinline__ int length_of(const AttendArgs &a, int s, bool tell) {
+    int len = a.lengths[s];
+    if (len < 0 || len > a.longest) {
+        if (tell) kk::report(a.status, kk::kBadIndex);
+        len = len < 0 ? 0 : a.longest;
+    }
+    return len;
+}
+
+__device__ __forceinline__ float load_query(const AttendArgs &a, int64_t at) {
+    return a.f16 ? static_cast<float>(static_cast<const _Float16 *>(a.q)[at]) : static_cast<const float *>(a.q)[at];
+}
+
+__device__ __forceinline__ void store_output(const AttendArgs &a, int64_t at, float v) {
+    if (a.f16) static_cast<_Float16 *>(a.y)[at] = static_cast<_Float16>(v);   // the one rounding of an F16 output
+    else static_cast<float *>(a.y)[at] = v;
+}
+
+// Lane moves across the four groups of 16 lanes (each pairs with both others' sums).
+__device__ __forceinline__ float across_groups_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// The value of the lane eight columns on (row_ror:8): a column's other part.
+__device__ __forceinline__ float other_part(float v) { return kk::dpp_move<0x128>(v); }
+
+// D32: 32-value pieces of a head (width <= 32 * D32). VW: values a lane loads of a V row
+// (16 lanes: width <= 16 * VW). NT: column tiles (8 query heads each). FAST: width == 32 *
+// D32 and page_tokens % 4 == 0 (a lane's four consecutive tokens share a page).
+template <int D32, int VW, int NT, bool FAST>
+__global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
+    static_assert(VW == 4 || VW == 8 || VW == 16, "4, 8 or 2 x 8 values of a V row per lane");
+    constexpr int VR = VW / 2;                       // dwords of a lane's part of a V row
+    constexpr int DPad = 16 * VW;
+    extern __shared__ float lds[];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int c = lane & 15, G = lane >> 4;
+    const int s = blockIdx.z, chunk = blockIdx.y, kvh = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
+    const int head0 = kvh * a.group + tile * 8 * NT;                        // first query head
+    const int heads = min(8 * NT, a.group - tile * 8 * NT);
+    const int width = a.pool.width;
+
+    const int len = length_of(a, s, tid == 0 && chunk == 0 && blockIdx.x == 0);
+    const int first = a.window > 0 ? max(0, len - a.window) : 0;
+    const int base = first & ~(kStep - 1);
+    const int begin = base + chunk * a.chunk;
+    const int end = min(len, begin + a.chunk);
+    const bool single = len - base <= a.chunk;
+    if (begin >= end) {
+        if (chunk == 0)                              // no tokens: zeros
+            for (int i = tid; i < heads * width; i += kThreads)
+                store_output(a, s * a.y_stride + (int64_t)(head0 + i / width) * width + i % width, 0.0f);
+        return;
+    }
+
+    // page ids of the chunk; a bad one is reported and its tokens left out
+    int *page_ids = reinterpret_cast<int *>(lds);
+    const int page0 = a.pool.per_page.div(max(begin, first));
+    const int last_page = a.pool.per_page.div(end - 1);
+    bool bad = false;
+    for (int i = tid; i <= last_page - page0; i += kThreads) {
+        int id = a.table[(int64_t)s * a.row_pages + page0 + i];
+        if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool.pages)) {
+            bad = true;
+            id = -1;
+        }
+        page_ids[i] = id;
+    }
+    if (bad) kk::report(a.status, kk::kBadPage);
+    const bool holes = __syncthreads_or(bad);
+
+    // q columns: column c is head c % 8 of each tile, its high (c < 8) or low part
+    half8 qf[NT][D32];
+    float undo[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int h = nt * 8 + (c & 7);
+        const int64_t row = s * a.q_stride + (int64_t)(head0 + (h < heads ? h : 0)) * width;
+        float v[D32][8], top = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D32; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = d * 32 + G * 8 + i;
+                v[d][i] = h < heads && (FAST || at < width) ? load_query(a, row + at) * a.scale_log2 : 0.0f;
+                top = fmaxf(top, fabsf(v[d][i]));
+            }
+        top = across_groups_max(top);
+        // 2^e with top * 2^e in [2^10, 2^11); Inf stays as it is
+        const int exponent = static_cast<int>((__float_as_uint(top) >> 23) & 0xff) - 127;
+        const int e = top == 0.0f || exponent == 128 ? 0 : min(10 - exponent, 100);
+        undo[nt] = ldexpf(1.0f, -e);
+#pragma unroll
+        for (int d = 0; d < D32; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = ldexpf(v[d][i], e);
+                const _Float16 hi = static_cast<_Float16>(x);
+                qf[nt][d][i] = c < 8 ? hi : static_cast<_Float16>(x - static_cast<float>(hi));
+            }
+    }
+
+    float4v acc[NT][VW];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m[nt] = -INFINITY;
+        l[nt] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VW; ++j) acc[nt][j] = float4v{0, 0, 0, 0};
+    }
+
+    const _Float16 *k_head = a.k + (int64_t)kvh * a.pool.head_stride;
+    const _Float16 *v_head = a.v + (int64_t)kvh * a.pool.head_stride;
+    // element offset of token t's row (t in the chunk); `ok` false where its page is missing
+    auto row_of = [&](int t, bool &ok) -> int64_t {
+        const int p = a.pool.per_page.div(t);
+        const int id = page_ids[p - page0];
+        ok = id >= 0;
+        return (int64_t)max(id, 0) * a.pool.page_stride + (int64_t)(t - p * a.pool.page_tokens) * a.pool.token_stride;
+    };
+
+    auto step = [&](int t0, auto masked_) {
+        constexpr bool masked = decltype(masked_)::value;
+        const int lo = max(first, begin), hi = end - 1;
+        half8 kf[2][D32];
+        uint32_t vr[8][VR];
+        bool ok[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            int t = t0 + half * 16 + c;
+            if (masked) t = min(max(t, lo), hi);
+            bool there;
+            const _Float16 *row = k_head + row_of(t, there);
+#pragma unroll
+            for (int d = 0; d < D32; ++d) {
+                const int at = d * 32 + G * 8;
+                if (FAST || at < width) kf[half][d] = *reinterpret_cast<const half8 *>(row + at);
+                else kf[half][d] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int want = t0 + (i < 4 ? 0 : 16) + G * 4 + (i & 3);
+            int t = want;
+            ok[i] = true;
+            bool there;
+            if (masked) {
+                t = min(max(t, lo), hi);
+                ok[i] = t == want;
+            }
+            const _Float16 *row = v_head + row_of(t, there);
+            ok[i] = ok[i] && there;
+#pragma unroll
+            for (int part = 0; part < (VW + 7) / 8; ++part) {
+                const int at = part * 128 + c * (VW < 8 ? VW : 8);
+                if (FAST || at < width) {
+                    if constexpr (VW == 4) {
+                        const uint2 x = *reinterpret_cast<const uint2 *>(row + at);
+                        vr[i][0] = x.x, vr[i][1] = x.y;
+                    } else {
+                        const uint4 x = *reinterpret_cast<const uint4 *>(row + at);
+                        vr[i][part * 4] = x.x, vr[i][part * 4 + 1] = x.y;
+                        vr[i][part * 4 + 2] = x.z, vr[i][part * 4 + 3] = x.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < (VW < 8 ? 2 : 4); ++u) vr[i][part * 4 + u] = 0;
+                }
+            }
+            if (masked && !ok[i]) {                  // 0 * NaN would reach the sums
+#pragma unroll
+                for (int u = 0; u < VR; ++u) vr[i][u] = 0;
+            }
+        }
+        half8 pf[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float4v tile_s[2] = {float4v{0, 0, 0, 0}, float4v{0, 0, 0, 0}};
+#pragma unroll
+            for (int d = 0; d < D32; ++d) {
+                tile_s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][d], qf[nt][d], tile_s[0], 0, 0, 0);
+                tile_s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][d], qf[nt][d], tile_s[1], 0, 0, 0);
+            }
+            float sc[8], sum = 0.0f, top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float part = tile_s[i / 4][i % 4];
+                sc[i] = (part + other_part(part)) * undo[nt];
+                sum += sc[i];
+            }
+            if (__any(!(fabsf(sum) < INFINITY))) {
+                // infinite keys or queries: the high part's infinity, as F32 products have it
+                // (its low part gives NaN or the other sign)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float part = tile_s[i / 4][i % 4], other = other_part(part);
+                    const float high = c < 8 ? part : other;
+                    if (fabsf(high) == INFINITY) sc[i] = high;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (masked && !ok[i]) sc[i] = -INFINITY;
+                top = fmaxf(top, sc[i]);
+            }
+            top = fmaxf(m[nt], across_groups_max(top));
+            if (__any(top > m[nt])) {
+                const float alpha = top > m[nt] ? exp2f(m[nt] - top) : 1.0f;   // 0 from no token yet
+                l[nt] *= alpha;
+#pragma unroll
+                for (int j = 0; j < VW; ++j) acc[nt][j] *= alpha;
+                m[nt] = top;
+            }
+            const float shift = kWeightLog2 - (top == -INFINITY ? 0.0f : top);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p = __builtin_amdgcn_exp2f(sc[i] + shift);
+                l[nt] += p;
+                const _Float16 high = static_cast<_Float16>(p);
+                pf[nt][i] = c < 8 ? high : static_cast<_Float16>(p - static_cast<float>(high));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+            union { uint32_t u[4]; half8 h; } vf;
+            const int word = (j / 8) * 4 + (j % 8) / 2;
+            const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                vf.u[u] = __builtin_amdgcn_perm(vr[2 * u + 1][word], vr[2 * u][word], pick);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                acc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, pf[nt], acc[nt][j], 0, 0, 0);
+        }
+    };
+
+    for (int t0 = begin + wave * kStep; t0 < end; t0 += kWaves * kStep) {
+        if (t0 >= first && t0 + kStep <= end && !holes) step(t0, std::false_type{});
+        else step(t0, std::true_type{});
+    }
+    __syncthreads();                                 // page_ids are read; the sums go over them
+
+    // the waves' sums side by side, then one sum per value
+    float *wave_ml = lds, *wave_o = lds + kWaves * NT * 8 * 2;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float total = across_groups_sum(l[nt]);
+        const int h = nt * 8 + c;
+        const bool mine = c < 8 && h < heads;
+        if (mine && G == 0) {
+            wave_ml[(wave * NT * 8 + h) * 2] = m[nt];
+            wave_ml[(wave * NT * 8 + h) * 2 + 1] = total;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+                const float v = acc[nt][j][r] + other_part(acc[nt][j][r]);
+                // row 4G + r of product j is value VW * (4G + r) + j (two halves of 128 at VW 16)
+                const int d = (j / 8) * 128 + (4 * G + r) * (VW < 8 ? VW : 8) + j % 8;
+                if (mine) wave_o[(wave * heads + h) * DPad + d] = v;
+            }
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * width; i += kThreads) {
+        const int h = i / width, d = i - h * width;
+        float top = -INFINITY, total = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_ml[(w * NT * 8 + h) * 2]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float mw = wave_ml[(w * NT * 8 + h) * 2];
+            const float scale = mw == -INFINITY ? 0.0f : exp2f(mw - top);
+            total += scale * wave_ml[(w * NT * 8 + h) * 2 + 1];
+            sum += scale * wave_o[(w * heads + h) * DPad + d];
+        }
+        if (single) {
+            store_output(a, s * a.y_stride + (int64_t)(head0 + h) * width + d, total == 0.0f ? 0.0f : sum / total);
+        } else {
+            const int64_t at = ((int64_t)s * a.query_heads + head0 + h) * a.chunks + chunk;
+            a.part_o[at * width + d] = sum;
+            if (d == 0) {
+                a.part_ml[at * 2] = top;
+                a.part_ml[at * 2 + 1] = total;
+            }
+        }
+    }
+}
+
+// Joins the chunks of one query head: y = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
+__global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
+    const int h = blockIdx.x, s = blockIdx.y, width = a.pool.width;
+    const int len = length_of(a, s, false);
+    const int base = (a.window > 0 ? max(0, len - a.window) : 0) & ~(kStep - 1);
+    if (len - base <= a.chunk) return;               // written by its one chunk
+    const int n = (len - base + a.chunk - 1) / a.chunk;
+    const int64_t at = ((int64_t)s * a.query_heads + h) * a.chunks;
+    for (int d = threadIdx.x; d < width; d += kThreads) {
+        float top = -INFINITY, total = 0.0f, sum = 0.0f;
+        for (int i = 0; i < n; ++i) top = fmaxf(top, a.part_ml[(at + i) * 2]);
+        for (int i = 0; i < n; ++i) {
+            const float mi = a.part_ml[(at + i) * 2];
+            const float scale = mi == -INFINITY ? 0.0f : exp2f(mi - top);
+            total += scale * a.part_ml[(at + i) * 2 + 1];
+            sum += scale * a.part_o[(at + i) * width + d];
+        }
+        store_output(a, s * a.y_stride + (int64_t)h * width + d, total == 0.0f ? 0.0f : sum / total);
+    }
+}
+
+struct Plan {
+    int group, nt, tiles, chunk, chunks;
+};
+
+Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus) {
+    Plan r;
+    r.group = p.query_heads / c.heads;
+    r.nt = r.group > 8 && c.width <= 128 ? 2 : 1;
+    r.tiles = (r.group + 8 * r.nt - 1) / (8 * r.nt);
+    const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
+    const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
+    const int64_t wanted = (longest * rows + 4 * cus - 1) / (4 * cus);   // tokens per workgroup, four to a CU
+    r.chunk = static_cast<int>(std::min<int64_t>(kMaxChunk, std::max<int64_t>(kMinChunk, (wanted + kMinChunk - 1) / kMinChunk * kMinChunk)));
+    r.chunks = (longest + r.chunk - 1) / r.chunk;
+    return r;
+}
+
+template <int D32, int VW, int NT, bool FAST>
+hipError_t launch(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
+    const size_t ids = (p.chunk / a.pool.page_tokens + 2) * sizeof(int);
+    const size_t sums = (size_t)kWaves * (NT * 8 * 2 + std::min(p.group, 8 * NT) * 16 * VW) * sizeof(float);
+    const size_t lds = std::max(ids, sums);          // at most 33 KiB
+    hipLaunchKernelGGL((attend<D32, VW, NT, FAST>), dim3(heads * p.tiles, p.chunks, sequences), dim3(kThreads), lds,
+                       stream, a);
+    return hipGetLastError();
+}
+
+template <int D32, int VW>
+hipError_t launch_width(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
+    const bool fast = a.pool.width == 32 * D32 && a.pool.page_tokens % 4 == 0;
+    if constexpr (VW <= 8) {
+        if (p.nt == 2)
+            return fast ? launch<D32, VW, 2, true>(a, p, sequences, heads, stream)
+                        : launch<D32, VW, 2, false>(a, p, sequences, heads, stream);
+    }
+    return fast ? launch<D32, VW, 1, true>(a, p, sequences, heads, stream)
+                : launch<D32, VW, 1, false>(a, p, sequences, heads, stream);
+}
+
+} // namespace
+
+extern "C" size_t kk_paged_attention_workspace_bytes(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p,
+                                          int cus) {
+    const Plan r = plan_of(c, p, cus);
+    return r.chunks == 1 ? 0 : (size_t)p.sequences * p.query_heads * r.chunks * (c.width + 2) * sizeof(float);
+}
+
+extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const void *v, const int *table, const int *lengths,
+                       const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, void *workspace,
+                       int *status, int cus, hipStream_t stream) {
+    const Plan r = plan_of(c, p, cus);
+    if (c.width <= 0 || c.width > 256 || c.width % 8 || p.sequences > 65535 || r.chunks > 65535 ||
+        (r.chunks > 1 && !workspace))
+        return hipErrorInvalidValue;
+    AttendArgs a;
+    a.k = static_cast<const _Float16 *>(k);
+    a.v = static_cast<const _Float16 *>(v);
+    a.table = table;
+    a.lengths = lengths;
+    a.q = q;
+    a.y = y;
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = a.part_o + (size_t)p.sequences * p.query_heads * r.chunks * c.width;
+    a.status = status;
+    a.pool = PoolView(c);
+    a.q_stride = p.q_stride;
+    a.y_stride = p.y_stride;
+    a.query_heads = p.query_heads;
+    a.group = r.group;
+    a.tiles = r.tiles;
+    a.longest = p.longest;
+    a.window = p.window;
+    a.row_pages = p.row_pages;
+    a.chunk = r.chunk;
+    a.chunks = r.chunks;
+    a.f16 = p.type == kunlun::InputType::f16;
+    a.scale_log2 = p.scale * 1.44269504088896340736f;
+    hipError_t rc;
+    if (c.width <= 64) rc = launch_width<2, 4>(a, r, p.sequences, c.heads, stream);
+    else if (c.width <= 96) rc = launch_width<3, 8>(a, r, p.sequences, c.heads, stream);
+    else if (c.width <= 128) rc = launch_width<4, 8>(a, r, p.sequences, c.heads, stream);
+    else if (c.width <= 192) rc = launch_width<6, 16>(a, r, p.sequences, c.heads, stream);
+    else rc = launch_width<8, 16>(a, r, p.sequences, c.heads, stream);
+    if (rc != hipSuccess || r.chunks == 1) return rc;
+    hipLaunchKernelGGL(join_chunks, dim3(p.query_heads, p.sequences), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}

@@ -84,8 +84,8 @@ DeviceContext & context(int device) {
         check_hip(hipStreamCreate(&ctx.stream), "hipStreamCreate");
         void * word = nullptr;
         check_hip(hipMalloc(&word, 256), "hipMalloc(status)");
-        const int zero = 0;
-        check_hip(hipMemcpy(word, &zero, sizeof(zero), hipMemcpyHostToDevice), "hipMemcpy(status)");
+        const int zeros[64] = {};
+        check_hip(hipMemcpy(word, zeros, sizeof(zeros), hipMemcpyHostToDevice), "hipMemcpy(status)");
         ctx.status = static_cast<int *>(word);
         check_hip(hipDeviceGetAttribute(&ctx.cus, hipDeviceAttributeMultiprocessorCount, device),
                   "hipDeviceGetAttribute(multiprocessors)");
@@ -93,6 +93,8 @@ DeviceContext & context(int device) {
     }
     return ctx;
 }
+
+bool device_visible(int device) { return device >= 0 && device < visible_devices(); }
 
 void count_matmul(int device) { ++matmuls[device]; }
 size_t matmul_count(int device) {

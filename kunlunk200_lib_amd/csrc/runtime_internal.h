@@ -15,7 +15,7 @@ namespace detail {
 struct DeviceContext {
     bool ready = false;
     hipStream_t stream = nullptr;
-    int *status = nullptr;          // device word written by kernels on bad input
+    int *status = nullptr;          // device words: [0] set on a non-finite rowwise_i8 activation, [1] kv_cache_status
     bool status_pending = false;    // a submitted kernel may have written it
     int cus = 0;                    // compute units of the device
 };
@@ -24,6 +24,8 @@ std::recursive_mutex & mutex();
 // Selects `device` and returns its context, creating stream and status word.
 DeviceContext & context(int device);
 int current_device();
+// Whether the id names a device that the library may use.
+bool device_visible(int device);
 void count_matmul(int device);
 size_t matmul_count(int device);
 // Abort with the diagnostic context and a message (the require() text).
@@ -65,6 +67,8 @@ struct Kernel::Impl {
     size_t gemm_workspace_size = 0;
     void * pair_workspace = nullptr;    // gate/up GEMV outputs of matmul_swiglu; elementwise copy of b
     size_t pair_workspace_size = 0;
+    void * kv_workspace = nullptr;      // chunks of paged_attention; lists of the page operations
+    size_t kv_workspace_size = 0;
     const char * route = nullptr;
 };
 
