@@ -48,7 +48,8 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kStep = 32;                // tokens of a wave's step
 constexpr int kMinChunk = kWaves * kStep;
-constexpr int kMaxChunk = 2048;
+constexpr int kMaxChunk = 512;
+constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr float kWeightLog2 = 14.0f;     // weights are scaled by 2^14
 
 struct AttendArgs {
@@ -60,21 +61,22 @@ struct AttendArgs {
     int *status;
     PoolView pool;
     int64_t q_stride, y_stride;
-    int query_heads, group, tiles, longest, window, row_pages, chunk, chunks, f16;
+    int query_heads, group, tiles, longest, window, row_pages, chunk, chunks, f16, q_wide;
     float scale_log2;
 };
 
+// A word that no lane writes during the launch, read through the scalar cache.
+__device__ __forceinline__ int scalar_load(const int *p) {
+    return *(const __attribute__((address_space(4))) int *)(p);
+}
+
 __device__ __forceinline__ int length_of(const AttendArgs &a, int s, bool tell) {
-    int len = a.lengths[s];
+    int len = scalar_load(a.lengths + s);
     if (len < 0 || len > a.longest) {
         if (tell) kk::report(a.status, kk::kBadIndex);
         len = len < 0 ? 0 : a.longest;
     }
     return len;
-}
-
-__device__ __forceinline__ float load_query(const AttendArgs &a, int64_t at) {
-    return a.f16 ? static_cast<float>(static_cast<const _Float16 *>(a.q)[at]) : static_cast<const float *>(a.q)[at];
 }
 
 __device__ __forceinline__ void store_output(const AttendArgs &a, int64_t at, float v) {
@@ -98,21 +100,48 @@ __device__ __forceinline__ float across_groups_sum(float v) {
 // The value of the lane eight columns on (row_ror:8): a column's other part.
 __device__ __forceinline__ float other_part(float v) { return kk::dpp_move<0x128>(v); }
 
-// D32: 32-value pieces of a head (width <= 32 * D32). VW: values a lane loads of a V row
-// (16 lanes: width <= 16 * VW). NT: column tiles (8 query heads each). FAST: width == 32 *
-// D32 and page_tokens % 4 == 0 (a lane's four consecutive tokens share a page).
-template <int D32, int VW, int NT, bool FAST>
+// Eight values of a row of q (16-byte loads where a.q_wide allows).
+__device__ __forceinline__ void load_query(const AttendArgs &a, int64_t at, float (&v)[8]) {
+    if (a.f16) {
+        const _Float16 *q = static_cast<const _Float16 *>(a.q) + at;
+        if (a.q_wide) {
+            const half8 x = *reinterpret_cast<const half8 *>(q);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(q[i]);
+        }
+    } else {
+        const float *q = static_cast<const float *>(a.q) + at;
+        if (a.q_wide) {
+            const float4v x = *reinterpret_cast<const float4v *>(q), y = *reinterpret_cast<const float4v *>(q + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = x[i], v[i + 4] = y[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = q[i];
+        }
+    }
+}
+
+// D32: 32-value pieces of a head (width <= 32 * D32; FULL: equal). VW: values a lane loads of a V
+// row (16 lanes: width <= 16 * VW). NT: column tiles (8 query heads each). UNI: page_tokens % 16
+// == 0, so that a half step of 16 tokens lies in one page: its address is scalar, its page id a
+// scalar load. Otherwise the chunk's page ids wait in LDS and each lane finds its rows there.
+template <int D32, int VW, int NT, bool UNI, bool FULL>
 __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     static_assert(VW == 4 || VW == 8 || VW == 16, "4, 8 or 2 x 8 values of a V row per lane");
+    constexpr int VP = VW < 8 ? VW : 8;              // values of one load
     constexpr int VR = VW / 2;                       // dwords of a lane's part of a V row
     constexpr int DPad = 16 * VW;
     extern __shared__ float lds[];
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, G = lane >> 4;
     const int s = blockIdx.z, chunk = blockIdx.y, kvh = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
     const int head0 = kvh * a.group + tile * 8 * NT;                        // first query head
     const int heads = min(8 * NT, a.group - tile * 8 * NT);
-    const int width = a.pool.width;
+    const int width = FULL ? 32 * D32 : a.pool.width;
 
     const int len = length_of(a, s, tid == 0 && chunk == 0 && blockIdx.x == 0);
     const int first = a.window > 0 ? max(0, len - a.window) : 0;
@@ -126,39 +155,133 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
                 store_output(a, s * a.y_stride + (int64_t)(head0 + i / width) * width + i % width, 0.0f);
         return;
     }
+    const int lo = max(first, begin), hi = end - 1;  // first and last token of the chunk
+    const int *row = a.table + (int64_t)s * a.row_pages;
 
-    // page ids of the chunk; a bad one is reported and its tokens left out
+    // !UNI: page ids of the chunk; a bad one is reported and its tokens left out
     int *page_ids = reinterpret_cast<int *>(lds);
-    const int page0 = a.pool.per_page.div(max(begin, first));
-    const int last_page = a.pool.per_page.div(end - 1);
-    bool bad = false;
-    for (int i = tid; i <= last_page - page0; i += kThreads) {
-        int id = a.table[(int64_t)s * a.row_pages + page0 + i];
-        if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool.pages)) {
-            bad = true;
-            id = -1;
+    const int page0 = a.pool.per_page.div(lo);
+    bool holes = false;
+    if constexpr (!UNI) {
+        const int last_page = a.pool.per_page.div(hi);
+        bool bad = false;
+        for (int i = tid; i <= last_page - page0; i += kThreads) {
+            int id = row[page0 + i];
+            if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool.pages)) {
+                bad = true;
+                id = -1;
+            }
+            page_ids[i] = id;
         }
-        page_ids[i] = id;
+        if (bad) kk::report(a.status, kk::kBadPage);
+        holes = __syncthreads_or(bad);
     }
-    if (bad) kk::report(a.status, kk::kBadPage);
-    const bool holes = __syncthreads_or(bad);
+
+    const _Float16 *k_head = a.k + (int64_t)kvh * a.pool.head_stride;
+    const _Float16 *v_head = a.v + (int64_t)kvh * a.pool.head_stride;
+
+    // the registers of a step: its K rows as A operands, its V rows as loaded
+    half8 kf[2][D32];
+    uint32_t vr[8][VR];
+    // UNI: where the step's two halves stand, and whether their pages exist
+    struct Halves {
+        int64_t at[2];
+        bool ok[2];
+    };
+    auto find = [&](int t0) {
+        Halves w;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int t = min(max(t0 + half * 16, lo & ~15), hi & ~15);
+            const int p = a.pool.per_page.div(t);
+            int id = scalar_load(row + p);
+            w.ok[half] = static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages);
+            if (!w.ok[half]) {
+                if (lane == 0) kk::report(a.status, kk::kBadPage);
+                id = 0;
+            }
+            w.at[half] = (int64_t)id * a.pool.page_stride + (int64_t)(t - p * a.pool.page_tokens) * a.pool.token_stride;
+        }
+        return w;
+    };
+    // !UNI: the row of token t, moved into the chunk
+    auto row_of = [&](int t) -> int64_t {
+        t = min(max(t, lo), hi);
+        const int p = a.pool.per_page.div(t);
+        return (int64_t)max(page_ids[p - page0], 0) * a.pool.page_stride +
+               (int64_t)(t - p * a.pool.page_tokens) * a.pool.token_stride;
+    };
+    // a lane's token of V register i, which is also the token of its score i
+    auto token_of = [&](int t0, int i) { return t0 + (i < 4 ? 0 : 16) + G * 4 + (i & 3); };
+    const uint32_t k_lane = static_cast<uint32_t>(c * a.pool.token_stride) + G * 8;
+    const uint32_t v_lane = static_cast<uint32_t>(G * 4 * a.pool.token_stride);
+    auto load_k = [&](int t0, const Halves &w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            int64_t at = 0;
+            if constexpr (!UNI) at = row_of(t0 + half * 16 + c);
+#pragma unroll
+            for (int d = 0; d < D32; ++d) {
+                const bool in = FULL || d * 32 + G * 8 < width;
+                const _Float16 *p = UNI ? k_head + w.at[half] + (k_lane + (in ? d * 32 : 0)) - (in ? 0 : G * 8)
+                                        : k_head + at + (in ? d * 32 + G * 8 : 0);
+                const half8 x = *reinterpret_cast<const half8 *>(p);
+                kf[half][d] = in ? x : half8{0, 0, 0, 0, 0, 0, 0, 0};
+            }
+        }
+    };
+    auto load_v = [&](int t0, const Halves &w) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            int64_t at = 0;
+            if constexpr (!UNI) at = row_of(token_of(t0, i));
+#pragma unroll
+            for (int part = 0; part < VW / VP; ++part) {
+                const int col = part * 128 + c * VP;
+                const bool in = (FULL && 16 * VW == 32 * D32) || col < width;
+                const _Float16 *p = UNI ? v_head + w.at[i / 4] + (i & 3) * a.pool.token_stride + (v_lane + (in ? col : 0))
+                                        : v_head + at + (in ? col : 0);
+                if constexpr (VW == 4) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(p);
+                    vr[i][0] = in ? x.x : 0, vr[i][1] = in ? x.y : 0;
+                } else {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+                    vr[i][part * 4] = in ? x.x : 0, vr[i][part * 4 + 1] = in ? x.y : 0;
+                    vr[i][part * 4 + 2] = in ? x.z : 0, vr[i][part * 4 + 3] = in ? x.w : 0;
+                }
+            }
+        }
+    };
+
+    int t0 = begin + wave * kStep;
+    const bool any = t0 < end;
+    Halves here{}, next{};
+    if (any) {
+        if constexpr (UNI) here = find(t0);
+        load_k(t0, here);
+        load_v(t0, here);
+    }
 
     // q columns: column c is head c % 8 of each tile, its high (c < 8) or low part
+    const float low = c < 8 ? 0.0f : -1.0f;
     half8 qf[NT][D32];
     float undo[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int h = nt * 8 + (c & 7);
-        const int64_t row = s * a.q_stride + (int64_t)(head0 + (h < heads ? h : 0)) * width;
+        const int64_t q_row = s * a.q_stride + (int64_t)(head0 + (h < heads ? h : 0)) * width;
+        const float scale = h < heads ? a.scale_log2 : 0.0f;
         float v[D32][8], top = 0.0f;
 #pragma unroll
-        for (int d = 0; d < D32; ++d)
+        for (int d = 0; d < D32; ++d) {
+            const bool in = FULL || d * 32 + G * 8 < width;
+            load_query(a, q_row + (in ? d * 32 + G * 8 : 0), v[d]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int at = d * 32 + G * 8 + i;
-                v[d][i] = h < heads && (FAST || at < width) ? load_query(a, row + at) * a.scale_log2 : 0.0f;
+                v[d][i] = in ? v[d][i] * scale : 0.0f;
                 top = fmaxf(top, fabsf(v[d][i]));
             }
+        }
         top = across_groups_max(top);
         // 2^e with top * 2^e in [2^10, 2^11); Inf stays as it is
         const int exponent = static_cast<int>((__float_as_uint(top) >> 23) & 0xff) - 127;
@@ -169,8 +292,8 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float x = ldexpf(v[d][i], e);
-                const _Float16 hi = static_cast<_Float16>(x);
-                qf[nt][d][i] = c < 8 ? hi : static_cast<_Float16>(x - static_cast<float>(hi));
+                const _Float16 high = static_cast<_Float16>(x);
+                qf[nt][d][i] = c < 8 ? high : static_cast<_Float16>(x - static_cast<float>(high));
             }
     }
 
@@ -184,82 +307,43 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
         for (int j = 0; j < VW; ++j) acc[nt][j] = float4v{0, 0, 0, 0};
     }
 
-    const _Float16 *k_head = a.k + (int64_t)kvh * a.pool.head_stride;
-    const _Float16 *v_head = a.v + (int64_t)kvh * a.pool.head_stride;
-    // element offset of token t's row (t in the chunk); `ok` false where its page is missing
-    auto row_of = [&](int t, bool &ok) -> int64_t {
-        const int p = a.pool.per_page.div(t);
-        const int id = page_ids[p - page0];
-        ok = id >= 0;
-        return (int64_t)max(id, 0) * a.pool.page_stride + (int64_t)(t - p * a.pool.page_tokens) * a.pool.token_stride;
-    };
+    if (any) for (;;) {
+        const int t1 = t0 + kWaves * kStep;
+        const bool more = t1 < end;
+        if constexpr (UNI) if (more) next = find(t1);
+        // a step with tokens that are not the chunk's, or whose page is missing
+        const bool masked = t0 < lo || t0 + kStep > end || (UNI ? !(here.ok[0] && here.ok[1]) : holes);
+        auto there = [&](int i) {
+            const int t = token_of(t0, i);
+            bool ok = t >= lo && t <= hi;
+            if constexpr (UNI) ok = ok && here.ok[i / 4];
+            else ok = ok && page_ids[a.pool.per_page.div(min(max(t, lo), hi)) - page0] >= 0;
+            return ok;
+        };
 
-    auto step = [&](int t0, auto masked_) {
-        constexpr bool masked = decltype(masked_)::value;
-        const int lo = max(first, begin), hi = end - 1;
-        half8 kf[2][D32];
-        uint32_t vr[8][VR];
-        bool ok[8];
+        float4v scores[NT][2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            int t = t0 + half * 16 + c;
-            if (masked) t = min(max(t, lo), hi);
-            bool there;
-            const _Float16 *row = k_head + row_of(t, there);
+        for (int nt = 0; nt < NT; ++nt) {
+            scores[nt][0] = scores[nt][1] = float4v{0, 0, 0, 0};
 #pragma unroll
             for (int d = 0; d < D32; ++d) {
-                const int at = d * 32 + G * 8;
-                if (FAST || at < width) kf[half][d] = *reinterpret_cast<const half8 *>(row + at);
-                else kf[half][d] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+                scores[nt][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][d], qf[nt][d], scores[nt][0], 0, 0, 0);
+                scores[nt][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][d], qf[nt][d], scores[nt][1], 0, 0, 0);
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int want = t0 + (i < 4 ? 0 : 16) + G * 4 + (i & 3);
-            int t = want;
-            ok[i] = true;
-            bool there;
-            if (masked) {
-                t = min(max(t, lo), hi);
-                ok[i] = t == want;
-            }
-            const _Float16 *row = v_head + row_of(t, there);
-            ok[i] = ok[i] && there;
-#pragma unroll
-            for (int part = 0; part < (VW + 7) / 8; ++part) {
-                const int at = part * 128 + c * (VW < 8 ? VW : 8);
-                if (FAST || at < width) {
-                    if constexpr (VW == 4) {
-                        const uint2 x = *reinterpret_cast<const uint2 *>(row + at);
-                        vr[i][0] = x.x, vr[i][1] = x.y;
-                    } else {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(row + at);
-                        vr[i][part * 4] = x.x, vr[i][part * 4 + 1] = x.y;
-                        vr[i][part * 4 + 2] = x.z, vr[i][part * 4 + 3] = x.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < (VW < 8 ? 2 : 4); ++u) vr[i][part * 4 + u] = 0;
-                }
-            }
-            if (masked && !ok[i]) {                  // 0 * NaN would reach the sums
-#pragma unroll
-                for (int u = 0; u < VR; ++u) vr[i][u] = 0;
-            }
-        }
+        // the next step's K rows are on their way during the weights and the second product, its V rows
+        // during the next scores
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_k(t1, next);
+        __builtin_amdgcn_sched_barrier(0);
+
         half8 pf[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float4v tile_s[2] = {float4v{0, 0, 0, 0}, float4v{0, 0, 0, 0}};
-#pragma unroll
-            for (int d = 0; d < D32; ++d) {
-                tile_s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][d], qf[nt][d], tile_s[0], 0, 0, 0);
-                tile_s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][d], qf[nt][d], tile_s[1], 0, 0, 0);
-            }
             float sc[8], sum = 0.0f, top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float part = tile_s[i / 4][i % 4];
+                const float part = scores[nt][i / 4][i % 4];
                 sc[i] = (part + other_part(part)) * undo[nt];
                 sum += sc[i];
             }
@@ -268,19 +352,20 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
                 // (its low part gives NaN or the other sign)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float part = tile_s[i / 4][i % 4], other = other_part(part);
+                    const float part = scores[nt][i / 4][i % 4], other = other_part(part);
                     const float high = c < 8 ? part : other;
                     if (fabsf(high) == INFINITY) sc[i] = high;
                 }
             }
+            if (masked) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (masked && !ok[i]) sc[i] = -INFINITY;
-                top = fmaxf(top, sc[i]);
+                for (int i = 0; i < 8; ++i) sc[i] = there(i) ? sc[i] : -INFINITY;
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, sc[i]);
             top = fmaxf(m[nt], across_groups_max(top));
             if (__any(top > m[nt])) {
-                const float alpha = top > m[nt] ? exp2f(m[nt] - top) : 1.0f;   // 0 from no token yet
+                const float alpha = top > m[nt] ? __builtin_amdgcn_exp2f(m[nt] - top) : 1.0f;   // 0 from no token yet
                 l[nt] *= alpha;
 #pragma unroll
                 for (int j = 0; j < VW; ++j) acc[nt][j] *= alpha;
@@ -292,7 +377,15 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
                 const float p = __builtin_amdgcn_exp2f(sc[i] + shift);
                 l[nt] += p;
                 const _Float16 high = static_cast<_Float16>(p);
-                pf[nt][i] = c < 8 ? high : static_cast<_Float16>(p - static_cast<float>(high));
+                pf[nt][i] = static_cast<_Float16>(fmaf(low, static_cast<float>(high), p));
+            }
+        }
+        if (masked) {                                // 0 * NaN would reach the sums
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool ok = there(i);
+#pragma unroll
+                for (int u = 0; u < VR; ++u) vr[i][u] = ok ? vr[i][u] : 0;
             }
         }
 #pragma unroll
@@ -307,13 +400,14 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
             for (int nt = 0; nt < NT; ++nt)
                 acc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, pf[nt], acc[nt][j], 0, 0, 0);
         }
-    };
-
-    for (int t0 = begin + wave * kStep; t0 < end; t0 += kWaves * kStep) {
-        if (t0 >= first && t0 + kStep <= end && !holes) step(t0, std::false_type{});
-        else step(t0, std::true_type{});
+        if (!more) break;
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(t1, next);
+        __builtin_amdgcn_sched_barrier(0);
+        t0 = t1;
+        here = next;
     }
-    __syncthreads();                                 // page_ids are read; the sums go over them
+    if constexpr (!UNI) __syncthreads();             // page_ids are read; the sums go over them
 
     // the waves' sums side by side, then one sum per value
     float *wave_ml = lds, *wave_o = lds + kWaves * NT * 8 * 2;
@@ -326,14 +420,16 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
             wave_ml[(wave * NT * 8 + h) * 2] = m[nt];
             wave_ml[(wave * NT * 8 + h) * 2 + 1] = total;
         }
+        // row 4G + r of product j is value VP * (4G + r) + j % 8 of half j / 8
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < VW; ++j) {
-                const float v = acc[nt][j][r] + other_part(acc[nt][j][r]);
-                // row 4G + r of product j is value VW * (4G + r) + j (two halves of 128 at VW 16)
-                const int d = (j / 8) * 128 + (4 * G + r) * (VW < 8 ? VW : 8) + j % 8;
-                if (mine) wave_o[(wave * heads + h) * DPad + d] = v;
+            for (int j = 0; j < VW; j += 4) {
+                float4v v;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = acc[nt][j + u][r] + other_part(acc[nt][j + u][r]);
+                if (mine)
+                    *reinterpret_cast<float4v *>(wave_o + (wave * heads + h) * DPad + (j / 8) * 128 + (4 * G + r) * VP + j % 8) = v;
             }
     }
     __syncthreads();
@@ -345,7 +441,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             const float mw = wave_ml[(w * NT * 8 + h) * 2];
-            const float scale = mw == -INFINITY ? 0.0f : exp2f(mw - top);
+            const float scale = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
             total += scale * wave_ml[(w * NT * 8 + h) * 2 + 1];
             sum += scale * wave_o[(w * heads + h) * DPad + d];
         }
@@ -362,24 +458,63 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     }
 }
 
-// Joins the chunks of one query head: y = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
+// Joins the chunks of one query head: y = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. Weights by
+// one thread per chunk; then groups of threads take the chunks in turn, 4 values
+// each, and the groups' sums are added in order.
+constexpr int kJoinRun = 1024;                       // chunks whose weights wait in LDS at a time
 __global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
-    const int h = blockIdx.x, s = blockIdx.y, width = a.pool.width;
+    __shared__ float weights[kJoinRun];
+    __shared__ float4v sums[kThreads];
+    __shared__ float reduce[kWaves];
+    const int h = blockIdx.x, s = blockIdx.y, width = a.pool.width, tid = threadIdx.x;
     const int len = length_of(a, s, false);
     const int base = (a.window > 0 ? max(0, len - a.window) : 0) & ~(kStep - 1);
     if (len - base <= a.chunk) return;               // written by its one chunk
     const int n = (len - base + a.chunk - 1) / a.chunk;
     const int64_t at = ((int64_t)s * a.query_heads + h) * a.chunks;
-    for (int d = threadIdx.x; d < width; d += kThreads) {
-        float top = -INFINITY, total = 0.0f, sum = 0.0f;
-        for (int i = 0; i < n; ++i) top = fmaxf(top, a.part_ml[(at + i) * 2]);
-        for (int i = 0; i < n; ++i) {
-            const float mi = a.part_ml[(at + i) * 2];
-            const float scale = mi == -INFINITY ? 0.0f : exp2f(mi - top);
-            total += scale * a.part_ml[(at + i) * 2 + 1];
-            sum += scale * a.part_o[(at + i) * width + d];
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
+    const float4v *o = reinterpret_cast<const float4v *>(a.part_o + at * width);
+    const int vectors = width / 4, groups = kThreads / vectors;
+    const int group = tid / vectors, at4 = tid - group * vectors;
+
+    float top = -INFINITY;
+    for (int i = tid; i < n; i += kThreads) top = fmaxf(top, ml[i].x);
+    top = kk::wave_max(top);
+    if (tid % kWave == 0) reduce[tid / kWave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, reduce[w]);
+    __syncthreads();
+
+    float total = 0.0f;
+    float4v sum{0, 0, 0, 0};
+    for (int i0 = 0; i0 < n; i0 += kJoinRun) {
+        const int run = min(kJoinRun, n - i0);
+        for (int i = tid; i < run; i += kThreads) {
+            const float2 x = ml[i0 + i];
+            const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - top);
+            weights[i] = w;
+            total += w * x.y;
         }
-        store_output(a, s * a.y_stride + (int64_t)h * width + d, total == 0.0f ? 0.0f : sum / total);
+        __syncthreads();
+        if (group < groups) {
+#pragma unroll 8
+            for (int i = group; i < run; i += groups) sum += weights[i] * o[(int64_t)(i0 + i) * vectors + at4];
+        }
+        __syncthreads();
+    }
+    total = kk::wave_sum(total);
+    if (tid % kWave == 0) reduce[tid / kWave] = total;
+    sums[tid] = sum;
+    __syncthreads();
+    total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += reduce[w];
+    if (tid < vectors) {
+        for (int g = 1; g < groups; ++g) sum += sums[g * vectors + tid];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            store_output(a, s * a.y_stride + (int64_t)h * width + tid * 4 + i, total == 0.0f ? 0.0f : sum[i] / total);
     }
 }
 
@@ -394,32 +529,40 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     r.tiles = (r.group + 8 * r.nt - 1) / (8 * r.nt);
     const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
-    const int64_t wanted = (longest * rows + 4 * cus - 1) / (4 * cus);   // tokens per workgroup, four to a CU
-    r.chunk = static_cast<int>(std::min<int64_t>(kMaxChunk, std::max<int64_t>(kMinChunk, (wanted + kMinChunk - 1) / kMinChunk * kMinChunk)));
+    // two workgroups' tokens to a CU: fewer leave the last ones alone (32 x 4096 tokens x 32 heads: chunks of 512
+    // 209 us, of 2048 218), and a sequence split further costs the join (1 x 32768 x 8: 512 30.5 us, 256 32.5)
+    const int64_t wanted = std::max<int64_t>((longest * rows + 2 * cus - 1) / (2 * cus), kMinChunk);
+    const int64_t chunk = std::max<int64_t>(std::min<int64_t>(wanted, kMaxChunk), (longest + kMostChunks - 1) / kMostChunks);
+    r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
     return r;
 }
 
-template <int D32, int VW, int NT, bool FAST>
+template <int D32, int VW, int NT, bool UNI, bool FULL>
 hipError_t launch(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
-    const size_t ids = (p.chunk / a.pool.page_tokens + 2) * sizeof(int);
+    const size_t ids = UNI ? 0 : (p.chunk / a.pool.page_tokens + 2) * sizeof(int);
     const size_t sums = (size_t)kWaves * (NT * 8 * 2 + std::min(p.group, 8 * NT) * 16 * VW) * sizeof(float);
     const size_t lds = std::max(ids, sums);          // at most 33 KiB
-    hipLaunchKernelGGL((attend<D32, VW, NT, FAST>), dim3(heads * p.tiles, p.chunks, sequences), dim3(kThreads), lds,
+    hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL>), dim3(heads * p.tiles, p.chunks, sequences), dim3(kThreads), lds,
                        stream, a);
     return hipGetLastError();
 }
 
+template <int D32, int VW, int NT>
+hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
+    // lane offsets within 16 tokens are 32-bit
+    const bool uni = a.pool.page_tokens % 16 == 0 && a.pool.token_stride < (1 << 26);
+    if (!uni) return launch<D32, VW, NT, false, false>(a, p, sequences, heads, stream);
+    if (a.pool.width == 32 * D32) return launch<D32, VW, NT, true, true>(a, p, sequences, heads, stream);
+    return launch<D32, VW, NT, true, false>(a, p, sequences, heads, stream);
+}
+
 template <int D32, int VW>
 hipError_t launch_width(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
-    const bool fast = a.pool.width == 32 * D32 && a.pool.page_tokens % 4 == 0;
     if constexpr (VW <= 8) {
-        if (p.nt == 2)
-            return fast ? launch<D32, VW, 2, true>(a, p, sequences, heads, stream)
-                        : launch<D32, VW, 2, false>(a, p, sequences, heads, stream);
+        if (p.nt == 2) return launch_tiles<D32, VW, 2>(a, p, sequences, heads, stream);
     }
-    return fast ? launch<D32, VW, 1, true>(a, p, sequences, heads, stream)
-                : launch<D32, VW, 1, false>(a, p, sequences, heads, stream);
+    return launch_tiles<D32, VW, 1>(a, p, sequences, heads, stream);
 }
 
 } // namespace
@@ -434,7 +577,7 @@ extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const v
                        const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, void *workspace,
                        int *status, int cus, hipStream_t stream) {
     const Plan r = plan_of(c, p, cus);
-    if (c.width <= 0 || c.width > 256 || c.width % 8 || p.sequences > 65535 || r.chunks > 65535 ||
+    if (c.width <= 0 || c.width > 256 || c.width % 8 || p.sequences > 65535 || r.chunks > kMostChunks ||
         (r.chunks > 1 && !workspace))
         return hipErrorInvalidValue;
     AttendArgs a;
@@ -459,6 +602,7 @@ extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const v
     a.chunk = r.chunk;
     a.chunks = r.chunks;
     a.f16 = p.type == kunlun::InputType::f16;
+    a.q_wide = (uintptr_t)q % 16 == 0 && p.q_stride % (a.f16 ? 8 : 4) == 0;
     a.scale_log2 = p.scale * 1.44269504088896340736f;
     hipError_t rc;
     if (c.width <= 64) rc = launch_width<2, 4>(a, r, p.sequences, c.heads, stream);

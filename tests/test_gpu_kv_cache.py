@@ -162,6 +162,10 @@ ATTENTION = [
     ([9001, 700, 64], 2, 8, 128, 16, 1, False, "heads", 0),  # the newest token alone
     ([3000, 65], 2, 8, 128, 16, 64, True, "heads", 0),
     ([20000], 8, 8, 128, 128, 0, True, "heads", 0),
+    ([70, 16], 2, 8, 96, 16, 0, False, "heads", 0),
+    ([70, 16], 2, 2, 192, 32, 40, False, "tokens", 0),
+    ([70, 16], 1, 12, 56, 16, 0, True, "heads", 0),
+    ([2100, 300], 1, 20, 128, 48, 500, False, "heads", 1),
 ]
 
 
