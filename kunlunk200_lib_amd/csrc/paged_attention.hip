@@ -43,6 +43,8 @@ using kk::kWave;
 using kk::PoolView;
 
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
@@ -125,11 +127,18 @@ __device__ __forceinline__ void load_query(const AttendArgs &a, int64_t at, floa
     }
 }
 
+// A lane's part of a cache row; ONCE: with the non-temporal hint.
+template <typename T, bool ONCE>
+__device__ __forceinline__ T load_row(const _Float16 *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T *>(p));
+    else return *reinterpret_cast<const T *>(p);
+}
+
 // D32: 32-value pieces of a head (width <= 32 * D32; FULL: equal). VW: values a lane loads of a V
 // row (16 lanes: width <= 16 * VW). NT: column tiles (8 query heads each). UNI: page_tokens % 16
 // == 0, so that a half step of 16 tokens lies in one page: its address is scalar, its page id a
 // scalar load. Otherwise the chunk's page ids wait in LDS and each lane finds its rows there.
-template <int D32, int VW, int NT, bool UNI, bool FULL>
+template <int D32, int VW, int NT, bool UNI, bool FULL, bool ONCE>
 __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     static_assert(VW == 4 || VW == 8 || VW == 16, "4, 8 or 2 x 8 values of a V row per lane");
     constexpr int VP = VW < 8 ? VW : 8;              // values of one load
@@ -142,6 +151,16 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     const int head0 = kvh * a.group + tile * 8 * NT;                        // first query head
     const int heads = min(8 * NT, a.group - tile * 8 * NT);
     const int width = FULL ? 32 * D32 : a.pool.width;
+
+    // the queries' values are on their way while the sequence's length and pages are read
+    float q[NT][D32][8];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int h = nt * 8 + (c & 7);
+        const int64_t q_row = s * a.q_stride + (int64_t)(head0 + (h < heads ? h : 0)) * width;
+#pragma unroll
+        for (int d = 0; d < D32; ++d) load_query(a, q_row + (FULL || d * 32 + G * 8 < width ? d * 32 + G * 8 : 0), q[nt][d]);
+    }
 
     const int len = length_of(a, s, tid == 0 && chunk == 0 && blockIdx.x == 0);
     const int first = a.window > 0 ? max(0, len - a.window) : 0;
@@ -225,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
                 const bool in = FULL || d * 32 + G * 8 < width;
                 const _Float16 *p = UNI ? k_head + w.at[half] + (k_lane + (in ? d * 32 : 0)) - (in ? 0 : G * 8)
                                         : k_head + at + (in ? d * 32 + G * 8 : 0);
-                const half8 x = *reinterpret_cast<const half8 *>(p);
+                const half8 x = load_row<half8, ONCE>(p);
                 kf[half][d] = in ? x : half8{0, 0, 0, 0, 0, 0, 0, 0};
             }
         }
@@ -242,12 +261,12 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
                 const _Float16 *p = UNI ? v_head + w.at[i / 4] + (i & 3) * a.pool.token_stride + (v_lane + (in ? col : 0))
                                         : v_head + at + (in ? col : 0);
                 if constexpr (VW == 4) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(p);
-                    vr[i][0] = in ? x.x : 0, vr[i][1] = in ? x.y : 0;
+                    const uint2v x = load_row<uint2v, ONCE>(p);
+                    vr[i][0] = in ? x[0] : 0, vr[i][1] = in ? x[1] : 0;
                 } else {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(p);
-                    vr[i][part * 4] = in ? x.x : 0, vr[i][part * 4 + 1] = in ? x.y : 0;
-                    vr[i][part * 4 + 2] = in ? x.z : 0, vr[i][part * 4 + 3] = in ? x.w : 0;
+                    const uint4v x = load_row<uint4v, ONCE>(p);
+                    vr[i][part * 4] = in ? x[0] : 0, vr[i][part * 4 + 1] = in ? x[1] : 0;
+                    vr[i][part * 4 + 2] = in ? x[2] : 0, vr[i][part * 4 + 3] = in ? x[3] : 0;
                 }
             }
         }
@@ -261,6 +280,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
         load_k(t0, here);
         load_v(t0, here);
     }
+    __builtin_amdgcn_sched_barrier(0);
 
     // q columns: column c is head c % 8 of each tile, its high (c < 8) or low part
     const float low = c < 8 ? 0.0f : -1.0f;
@@ -268,18 +288,15 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     float undo[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int h = nt * 8 + (c & 7);
-        const int64_t q_row = s * a.q_stride + (int64_t)(head0 + (h < heads ? h : 0)) * width;
-        const float scale = h < heads ? a.scale_log2 : 0.0f;
-        float v[D32][8], top = 0.0f;
+        const float scale = nt * 8 + (c & 7) < heads ? a.scale_log2 : 0.0f;
+        float top = 0.0f;
 #pragma unroll
         for (int d = 0; d < D32; ++d) {
             const bool in = FULL || d * 32 + G * 8 < width;
-            load_query(a, q_row + (in ? d * 32 + G * 8 : 0), v[d]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                v[d][i] = in ? v[d][i] * scale : 0.0f;
-                top = fmaxf(top, fabsf(v[d][i]));
+                q[nt][d][i] = in ? q[nt][d][i] * scale : 0.0f;
+                top = fmaxf(top, fabsf(q[nt][d][i]));
             }
         }
         top = across_groups_max(top);
@@ -291,7 +308,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
         for (int d = 0; d < D32; ++d)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float x = ldexpf(v[d][i], e);
+                const float x = ldexpf(q[nt][d][i], e);
                 const _Float16 high = static_cast<_Float16>(x);
                 qf[nt][d][i] = c < 8 ? high : static_cast<_Float16>(x - static_cast<float>(high));
             }
@@ -496,10 +513,20 @@ __global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
             weights[i] = w;
             total += w * x.y;
         }
-        __syncthreads();
-        if (group < groups) {
-#pragma unroll 8
-            for (int i = group; i < run; i += groups) sum += weights[i] * o[(int64_t)(i0 + i) * vectors + at4];
+        // the values of up to 8 chunks a thread are on their way before the weights are known
+        for (int j0 = group; j0 < run || j0 == group; j0 += 8 * groups) {
+            float4v v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = j0 + u * groups;
+                v[u] = group < groups && i < run ? o[(int64_t)(i0 + i) * vectors + at4] : float4v{0, 0, 0, 0};
+            }
+            if (j0 == group) __syncthreads();
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = j0 + u * groups;
+                if (group < groups && i < run) sum += weights[i] * v[u];
+            }
         }
         __syncthreads();
     }
@@ -520,6 +547,7 @@ __global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
 
 struct Plan {
     int group, nt, tiles, chunk, chunks;
+    bool once;
 };
 
 Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus) {
@@ -535,16 +563,22 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int64_t chunk = std::max<int64_t>(std::min<int64_t>(wanted, kMaxChunk), (longest + kMostChunks - 1) / kMostChunks);
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
+    // The non-temporal hint, for reads that fill the 256 MiB cache with nothing that is read again: one tile, a head's
+    // rows one after the other, more than a quarter of it (32 x 4096 tokens x 32 heads 209 us, with the hint 192;
+    // 64 x 1024 tokens x 8 heads of 64 34.9 / 30.7; 16 x 1024 x 8 of 128 19.0 / 20.3; tiles that read the same
+    // rows 104 / 137; rows that share cache lines, 64 x 1024 x 8 of 80, 50 / 55).
+    r.once = r.tiles == 1 && c.token_stride == c.width &&
+             (int64_t)p.sequences * longest * c.heads * c.width * 4 > (64 << 20);
     return r;
 }
 
-template <int D32, int VW, int NT, bool UNI, bool FULL>
+template <int D32, int VW, int NT, bool UNI, bool FULL, bool ONCE>
 hipError_t launch(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     const size_t ids = UNI ? 0 : (p.chunk / a.pool.page_tokens + 2) * sizeof(int);
     const size_t sums = (size_t)kWaves * (NT * 8 * 2 + std::min(p.group, 8 * NT) * 16 * VW) * sizeof(float);
     const size_t lds = std::max(ids, sums);          // at most 33 KiB
-    hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL>), dim3(heads * p.tiles, p.chunks, sequences), dim3(kThreads), lds,
-                       stream, a);
+    hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL, ONCE>), dim3(heads * p.tiles, p.chunks, sequences), dim3(kThreads),
+                       lds, stream, a);
     return hipGetLastError();
 }
 
@@ -552,9 +586,10 @@ template <int D32, int VW, int NT>
 hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     // lane offsets within 16 tokens are 32-bit
     const bool uni = a.pool.page_tokens % 16 == 0 && a.pool.token_stride < (1 << 26);
-    if (!uni) return launch<D32, VW, NT, false, false>(a, p, sequences, heads, stream);
-    if (a.pool.width == 32 * D32) return launch<D32, VW, NT, true, true>(a, p, sequences, heads, stream);
-    return launch<D32, VW, NT, true, false>(a, p, sequences, heads, stream);
+    if (!uni) return launch<D32, VW, NT, false, false, false>(a, p, sequences, heads, stream);
+    if (a.pool.width != 32 * D32) return launch<D32, VW, NT, true, false, false>(a, p, sequences, heads, stream);
+    return p.once ? launch<D32, VW, NT, true, true, true>(a, p, sequences, heads, stream)
+                  : launch<D32, VW, NT, true, true, false>(a, p, sequences, heads, stream);
 }
 
 template <int D32, int VW>
