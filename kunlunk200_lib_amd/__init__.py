@@ -134,6 +134,8 @@ C_FUNCTIONS = [
 def load(path: str | None = None) -> ctypes.CDLL:
     """Load the HIP library (once) and declare every C entry point."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lib_lock:
         if _lib is not None:
             return _lib
@@ -168,6 +170,8 @@ class CopyKind(enum.IntEnum):
 
 
 def _ptr(value) -> int | None:
+    if type(value) is int:      # the address itself, as torch's data_ptr() gives it
+        return value
     if value is None:
         return None
     if isinstance(value, Buffer):
