@@ -46,11 +46,11 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kWideWaves = 8;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kStep = 32;                // tokens of a wave's step
 constexpr int kMinChunk = kWaves * kStep;
-constexpr int kMaxChunk = 512;
+constexpr int kMaxChunk = 512, kMaxChunkMany = 1024;
 constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr float kWeightLog2 = 14.0f;     // weights are scaled by 2^14
 
@@ -138,12 +138,13 @@ __device__ __forceinline__ T load_row(const _Float16 *p) {
 // row (16 lanes: width <= 16 * VW). NT: column tiles (8 query heads each). UNI: page_tokens % 16
 // == 0, so that a half step of 16 tokens lies in one page: its address is scalar, its page id a
 // scalar load. Otherwise the chunk's page ids wait in LDS and each lane finds its rows there.
-template <int D32, int VW, int NT, bool UNI, bool FULL, bool ONCE>
-__global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
+template <int D32, int VW, int NT, bool UNI, bool FULL, bool ONCE, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
     static_assert(VW == 4 || VW == 8 || VW == 16, "4, 8 or 2 x 8 values of a V row per lane");
     constexpr int VP = VW < 8 ? VW : 8;              // values of one load
     constexpr int VR = VW / 2;                       // dwords of a lane's part of a V row
     constexpr int DPad = 16 * VW;
+    constexpr int kGroup = WAVES * kWave;
     extern __shared__ float lds[];
     const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, G = lane >> 4;
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     const bool single = len - base <= a.chunk;
     if (begin >= end) {
         if (chunk == 0)                              // no tokens: zeros
-            for (int i = tid; i < heads * width; i += kThreads)
+            for (int i = tid; i < heads * width; i += kGroup)
                 store_output(a, s * a.y_stride + (int64_t)(head0 + i / width) * width + i % width, 0.0f);
         return;
     }
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     if constexpr (!UNI) {
         const int last_page = a.pool.per_page.div(hi);
         bool bad = false;
-        for (int i = tid; i <= last_page - page0; i += kThreads) {
+        for (int i = tid; i <= last_page - page0; i += kGroup) {
             int id = row[page0 + i];
             if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool.pages)) {
                 bad = true;
@@ -325,7 +326,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     }
 
     if (any) for (;;) {
-        const int t1 = t0 + kWaves * kStep;
+        const int t1 = t0 + WAVES * kStep;
         const bool more = t1 < end;
         if constexpr (UNI) if (more) next = find(t1);
         // a step with tokens that are not the chunk's, or whose page is missing
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
     if constexpr (!UNI) __syncthreads();             // page_ids are read; the sums go over them
 
     // the waves' sums side by side, then one sum per value
-    float *wave_ml = lds, *wave_o = lds + kWaves * NT * 8 * 2;
+    float *wave_ml = lds, *wave_o = lds + WAVES * NT * 8 * 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const float total = across_groups_sum(l[nt]);
@@ -450,13 +451,13 @@ __global__ __launch_bounds__(kThreads) void attend(AttendArgs a) {
             }
     }
     __syncthreads();
-    for (int i = tid; i < heads * width; i += kThreads) {
+    for (int i = tid; i < heads * width; i += kGroup) {
         const int h = i / width, d = i - h * width;
         float top = -INFINITY, total = 0.0f, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_ml[(w * NT * 8 + h) * 2]);
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, wave_ml[(w * NT * 8 + h) * 2]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float mw = wave_ml[(w * NT * 8 + h) * 2];
             const float scale = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
             total += scale * wave_ml[(w * NT * 8 + h) * 2 + 1];
@@ -547,7 +548,7 @@ __global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
 
 struct Plan {
     int group, nt, tiles, chunk, chunks;
-    bool once;
+    bool once, wide;
 };
 
 Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus) {
@@ -557,10 +558,22 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     r.tiles = (r.group + 8 * r.nt - 1) / (8 * r.nt);
     const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
-    // two workgroups' tokens to a CU: fewer leave the last ones alone (32 x 4096 tokens x 32 heads: chunks of 512
-    // 209 us, of 2048 218), and a sequence split further costs the join (1 x 32768 x 8: 512 30.5 us, 256 32.5)
-    const int64_t wanted = std::max<int64_t>((longest * rows + 2 * cus - 1) / (2 * cus), kMinChunk);
-    const int64_t chunk = std::max<int64_t>(std::min<int64_t>(wanted, kMaxChunk), (longest + kMostChunks - 1) / kMostChunks);
+    // No split, so no second launch: eight waves to a workgroup for rows of up to 512 tokens, or 1024 where they
+    // leave few CUs idle (us, against the split: 4 x 160 / 320 / 512 tokens x 8 heads 7.0 / 7.8 / 8.8, 10.5 split; at 768
+    // 12.3 / 11.3; 32 x 512 / 1024 x 8 heads 13.9 / 27.8, split 19.1 / 30.5), four for more rows of up to 512.
+    const int whole = kMaxChunk + kStep;             // a window starts up to kStep - 1 tokens early
+    r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
+             longest <= (rows > cus / 2 ? 2 * whole : whole);
+    const int64_t least = r.wide ? longest : rows > cus && longest <= whole ? longest : kMinChunk;
+    // Otherwise two workgroups' tokens to a CU, in parts of one size. Parts of up to 512 tokens; with two rows and more to
+    // a CU whole rows of up to 1024 and, above, at least three parts of up to 1024: each part costs its start and its
+    // end, and few long ones wait for the last (1 x 32768 tokens x 8 heads 29 us, parts of 256 31.7; 64 x 1024 x 8
+    // 46, split in two 54; ragged to 1500, 128 x 8: two parts 117, three 94, four 102; ragged to 3000: 168, of 512 176).
+    const int64_t most = rows >= 2 * cus ? kMaxChunkMany : kMaxChunk;
+    const int64_t wanted = std::min<int64_t>((longest * rows + 2 * cus - 1) / (2 * cus), most);
+    const int64_t split = std::max({wanted, least, (int64_t)(longest + kMostChunks - 1) / kMostChunks});
+    const int64_t least_parts = rows >= 2 * cus && longest > kMaxChunkMany ? 3 : 1;
+    const int64_t parts = std::max((longest + split - 1) / split, least_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
     // The non-temporal hint, for reads that fill the 256 MiB cache with nothing that is read again: one tile, a head's
@@ -572,32 +585,35 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     return r;
 }
 
-template <int D32, int VW, int NT, bool UNI, bool FULL, bool ONCE>
+template <int D32, int VW, int NT, bool UNI, bool FULL, bool ONCE, int WAVES>
 hipError_t launch(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     const size_t ids = UNI ? 0 : (p.chunk / a.pool.page_tokens + 2) * sizeof(int);
-    const size_t sums = (size_t)kWaves * (NT * 8 * 2 + std::min(p.group, 8 * NT) * 16 * VW) * sizeof(float);
+    const size_t sums = (size_t)WAVES * (NT * 8 * 2 + std::min(p.group, 8 * NT) * 16 * VW) * sizeof(float);
     const size_t lds = std::max(ids, sums);          // at most 33 KiB
-    hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL, ONCE>), dim3(heads * p.tiles, p.chunks, sequences), dim3(kThreads),
-                       lds, stream, a);
+    hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL, ONCE, WAVES>), dim3(heads * p.tiles, p.chunks, sequences),
+                       dim3(WAVES * kWave), lds, stream, a);
     return hipGetLastError();
 }
 
-template <int D32, int VW, int NT>
+template <int D32, int VW, int NT, int WAVES>
 hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     // lane offsets within 16 tokens are 32-bit
     const bool uni = a.pool.page_tokens % 16 == 0 && a.pool.token_stride < (1 << 26);
-    if (!uni) return launch<D32, VW, NT, false, false, false>(a, p, sequences, heads, stream);
-    if (a.pool.width != 32 * D32) return launch<D32, VW, NT, true, false, false>(a, p, sequences, heads, stream);
-    return p.once ? launch<D32, VW, NT, true, true, true>(a, p, sequences, heads, stream)
-                  : launch<D32, VW, NT, true, true, false>(a, p, sequences, heads, stream);
+    if (!uni) return launch<D32, VW, NT, false, false, false, WAVES>(a, p, sequences, heads, stream);
+    if (a.pool.width != 32 * D32) return launch<D32, VW, NT, true, false, false, WAVES>(a, p, sequences, heads, stream);
+    if constexpr (WAVES == kWaves) {
+        if (p.once) return launch<D32, VW, NT, true, true, true, WAVES>(a, p, sequences, heads, stream);
+    }
+    return launch<D32, VW, NT, true, true, false, WAVES>(a, p, sequences, heads, stream);
 }
 
 template <int D32, int VW>
 hipError_t launch_width(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     if constexpr (VW <= 8) {
-        if (p.nt == 2) return launch_tiles<D32, VW, 2>(a, p, sequences, heads, stream);
+        if (p.nt == 2) return launch_tiles<D32, VW, 2, kWaves>(a, p, sequences, heads, stream);
+        if (p.wide) return launch_tiles<D32, VW, 1, kWideWaves>(a, p, sequences, heads, stream);
     }
-    return launch_tiles<D32, VW, 1>(a, p, sequences, heads, stream);
+    return launch_tiles<D32, VW, 1, kWaves>(a, p, sequences, heads, stream);
 }
 
 } // namespace
