@@ -148,11 +148,34 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
     extern __shared__ float lds[];
     const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, G = lane >> 4;
-    const int s = blockIdx.z, chunk = blockIdx.y, kvh = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
+    int s = blockIdx.y, chunk = blockIdx.z, kvh = blockIdx.x, tile = 0;
+    if (a.tiles > 1) {
+        // Workgroups go round the eight XCDs: numbered so that the tiles of one chunk, which read the same rows, are a
+        // multiple of eight apart, on one XCD and its L2, and start together (last: fewer than eight chunks)
+        const uint32_t number = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+        const uint32_t items = gridDim.x / a.tiles * gridDim.y * gridDim.z, even = items & ~7u;
+        const bool whole = number < even * a.tiles;
+        const uint32_t side = whole ? 8 : items - even, at = whole ? number : number - even * a.tiles;
+        const uint32_t set = at / (side * a.tiles), in_set = at - set * side * a.tiles;
+        tile = in_set / side;
+        const uint32_t item = (whole ? set * 8 : even) + in_set - tile * side, heads_of_cache = gridDim.x / a.tiles;
+        const uint32_t row_chunk = item / heads_of_cache;
+        kvh = item - row_chunk * heads_of_cache;
+        chunk = row_chunk / gridDim.y;
+        s = row_chunk - chunk * gridDim.y;
+    }
+    // Workgroups also go round the CUs, wherever one has room: parts that are there first (part number slowest: those
+    // past a sequence's end come last and at once), and sequences turned within each eight, so that long and
+    // short ones that take turns do not meet on the same CUs (sequences of 1000 tokens where `longest` is 32768: 121 us in
+    // order of sequences, 48 so; 64 x 8 heads ragged to 2048, every other one long: 70, in order 83, turned 63)
+    const int eight = s / 8, first_of = eight * 8, size = min(8, static_cast<int>(gridDim.y) - first_of);
+    s = first_of + (s - first_of + eight + eight / 4 + chunk) % size;
     const int head0 = kvh * a.group + tile * 8 * NT;                        // first query head
     const int heads = min(8 * NT, a.group - tile * 8 * NT);
     const int width = FULL ? 32 * D32 : a.pool.width;
 
+    // a part past the sequence's end, before it asks for anything
+    if (chunk > 0 && a.window == 0 && chunk * a.chunk >= scalar_load(a.lengths + s)) return;
     // the queries' values are on their way while the sequence's length and pages are read
     float q[NT][D32][8];
 #pragma unroll
@@ -163,7 +186,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
         for (int d = 0; d < D32; ++d) load_query(a, q_row + (FULL || d * 32 + G * 8 < width ? d * 32 + G * 8 : 0), q[nt][d]);
     }
 
-    const int len = length_of(a, s, tid == 0 && chunk == 0 && blockIdx.x == 0);
+    const int len = length_of(a, s, tid == 0 && chunk == 0 && kvh == 0 && tile == 0);
     const int first = a.window > 0 ? max(0, len - a.window) : 0;
     const int base = first & ~(kStep - 1);
     const int begin = base + chunk * a.chunk;
@@ -569,11 +592,16 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     // a CU whole rows of up to 1024 and, above, at least three parts of up to 1024: each part costs its start and its
     // end, and few long ones wait for the last (1 x 32768 tokens x 8 heads 29 us, parts of 256 31.7; 64 x 1024 x 8
     // 46, split in two 54; ragged to 1500, 128 x 8: two parts 117, three 94, four 102; ragged to 3000: 168, of 512 176).
-    const int64_t most = rows >= 2 * cus ? kMaxChunkMany : kMaxChunk;
+    // (of workgroups that a CU holds one or two of instead of three, twice as many: 64 x 2048 x 8 heads of 256 210 us in
+    // three parts, 174 whole; groups of 16 query heads 128 / 92).
+    const int many = c.width > 128 || r.nt == 2 ? 2 * kMaxChunkMany : kMaxChunkMany;
+    const int64_t most = rows >= 2 * cus ? many : kMaxChunk;
     const int64_t wanted = std::min<int64_t>((longest * rows + 2 * cus - 1) / (2 * cus), most);
     const int64_t split = std::max({wanted, least, (int64_t)(longest + kMostChunks - 1) / kMostChunks});
-    const int64_t least_parts = rows >= 2 * cus && longest > kMaxChunkMany ? 3 : 1;
-    const int64_t parts = std::max((longest + split - 1) / split, least_parts), chunk = (longest + parts - 1) / parts;
+    const int64_t least_parts = rows >= 2 * cus && longest > many ? 3 : 1;
+    // and a bound on the workgroups that find no tokens where `longest` is far above the lengths
+    const int64_t most_parts = std::max<int64_t>((1 << 12) / rows, least_parts);
+    const int64_t parts = std::min(std::max((longest + split - 1) / split, least_parts), most_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
     // The non-temporal hint, for reads that fill the 256 MiB cache with nothing that is read again: one tile, a head's
@@ -590,7 +618,7 @@ hipError_t launch(const AttendArgs &a, const Plan &p, int sequences, int heads, 
     const size_t ids = UNI ? 0 : (p.chunk / a.pool.page_tokens + 2) * sizeof(int);
     const size_t sums = (size_t)WAVES * (NT * 8 * 2 + std::min(p.group, 8 * NT) * 16 * VW) * sizeof(float);
     const size_t lds = std::max(ids, sums);          // at most 33 KiB
-    hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL, ONCE, WAVES>), dim3(heads * p.tiles, p.chunks, sequences),
+    hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL, ONCE, WAVES>), dim3(heads * p.tiles, sequences, p.chunks),
                        dim3(WAVES * kWave), lds, stream, a);
     return hipGetLastError();
 }
