@@ -38,10 +38,10 @@ __device__ __forceinline__ T scalar_load(const T *p) {
 template <int VPT, bool VEC>
 __global__ __launch_bounds__(kThreads) void process(LogitsArgs a) {
     constexpr int kSlice = slice_of(VPT);
-    // counts, then the places of bias entries, then their values
+    // counts, then bias entries: their place in the list + 1 above their value, so that the largest word is the last entry
     __shared__ uint4 words[3 * kSlice / 4];
-    uint32_t *counts = reinterpret_cast<uint32_t *>(words), *entries = counts + kSlice;
-    float *biases = reinterpret_cast<float *>(entries + kSlice);
+    uint32_t *counts = reinterpret_cast<uint32_t *>(words);
+    unsigned long long *entries = reinterpret_cast<unsigned long long *>(counts + kSlice);
     const int tid = threadIdx.x, row = blockIdx.y, first = blockIdx.x * kSlice;
     const int n = min(kSlice, a.vocabulary - first);
     const bool counted = a.history != nullptr, biased = a.bias_ids != nullptr;
@@ -88,18 +88,15 @@ __global__ __launch_bounds__(kThreads) void process(LogitsArgs a) {
     if (past > 0 || given > 0) {
 #pragma unroll
         for (int u = 0; u < 3 * VPT; ++u) words[u * kThreads + tid] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
+        kk::lds_barrier();                           // the loads stay in flight
         auto count = [&](int token) {
             const uint32_t t = place(token);
             if (t < static_cast<uint32_t>(n)) atomicAdd(&counts[t], 1u);
         };
-        auto enter = [&](int token, int i) {
+        auto enter = [&](int token, int i, float x) {
             const uint32_t t = place(token);
-            if (t < static_cast<uint32_t>(n)) atomicMax(&entries[t], static_cast<uint32_t>(i) + 1);
-        };
-        auto deliver = [&](int token, int i, float x) {
-            const uint32_t t = place(token);
-            if (t < static_cast<uint32_t>(n) && entries[t] == static_cast<uint32_t>(i) + 1) biases[t] = x;
+            if (t < static_cast<uint32_t>(n))
+                atomicMax(&entries[t], static_cast<unsigned long long>(i + 1) << 32 | __float_as_uint(x));
         };
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) count(seen[u]);
@@ -110,26 +107,24 @@ __global__ __launch_bounds__(kThreads) void process(LogitsArgs a) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) count(token[u]);
         }
-        if (given > 0) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) enter(id[u], u * kThreads + tid);
-            for (int i = 2 * kThreads + tid; i < given; i += kThreads) enter(ids[i], i);
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < 2; ++u) deliver(id[u], u * kThreads + tid, value[u]);
-            for (int i = 2 * kThreads + tid; i < given; i += kThreads) deliver(ids[i], i, values[i]);
-        }
-        __syncthreads();
+        for (int u = 0; u < 2; ++u) enter(id[u], u * kThreads + tid, value[u]);
+        for (int i = 2 * kThreads + tid; i < given; i += kThreads) enter(ids[i], i, values[i]);
+        kk::lds_barrier();
 #pragma unroll
         for (int u = 0; u < VPT; ++u) {
             const uint4 met = reinterpret_cast<const uint4 *>(counts)[u * kThreads + tid];
-            const float4 b = reinterpret_cast<const float4 *>(biases)[u * kThreads + tid];
-            auto one = [&](float x, uint32_t times, float bias) {
-                const float less = (x > 0.0f ? x / r : x * r) - static_cast<float>(times) * f - p;
-                return (times ? less : x) + bias;
+            const uint4 b01 = reinterpret_cast<const uint4 *>(entries)[(u * kThreads + tid) * 2];
+            const uint4 b23 = reinterpret_cast<const uint4 *>(entries)[(u * kThreads + tid) * 2 + 1];
+            auto less = [&](float x, uint32_t times) {
+                return times ? (x > 0.0f ? x / r : x * r) - static_cast<float>(times) * f - p : x;
             };
-            z[u] = make_float4(one(z[u].x, met.x, b.x), one(z[u].y, met.y, b.y), one(z[u].z, met.z, b.z),
-                               one(z[u].w, met.w, b.w));
+            if (met.x | met.y | met.z | met.w)       // few waves: a division is ten instructions
+                z[u] = make_float4(less(z[u].x, met.x), less(z[u].y, met.y), less(z[u].z, met.z), less(z[u].w, met.w));
+            z[u].x += __uint_as_float(b01.x);
+            z[u].y += __uint_as_float(b01.z);
+            z[u].z += __uint_as_float(b23.x);
+            z[u].w += __uint_as_float(b23.z);
         }
     }
 #pragma unroll
