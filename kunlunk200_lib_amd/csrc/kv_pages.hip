@@ -287,57 +287,68 @@ __global__ __launch_bounds__(kCopyThreads) void free_rows(PagesArgs a, const int
 
 // ---- kv_compact ----------------------------------------------------------------------------
 
-// One workgroup: U, then the lists of holes below U and of used pages from U up.
-__global__ __launch_bounds__(kPlanThreads) void compact_plan(const int *references, int *references_out, int pages,
-                                                             int *used_out, int *moves, int *holes, int *movers,
-                                                             int *place) {
-    __shared__ long long scratch[kPlanWaves];
-    int used = 0;
-    for (int p0 = 0; p0 < pages; p0 += kTile) {
-        const Counts<kPerThread> c(references, pages, p0);
-        long long mine = 0, total;
+// Used pages among the first n, by the whole workgroup.
+__device__ __forceinline__ int used_among(const int *references, int n, int *scratch) {
+    int mine = 0, total;
+    int p = threadIdx.x;
+    for (; p + 7 * kPlanThreads < n; p += 8 * kPlanThreads) {
+        int r[8];
 #pragma unroll
-        for (int u = 0; u < kPerThread; ++u) mine += c.r[u] > 0;
-        prefix<long long>(mine, total, scratch);
-        used += static_cast<int>(total);
+        for (int u = 0; u < 8; ++u) r[u] = references[p + u * kPlanThreads];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mine += r[u] > 0;
     }
-    // both lists in one pass: holes counted in the low half of a word, movers in the high half
-    int n_holes = 0, n_movers = 0;
-    for (int p0 = 0; p0 < pages; p0 += kTile) {
+    for (; p < n; p += kPlanThreads) mine += references[p] > 0;
+    prefix<int>(mine, total, scratch);
+    return total;
+}
+
+// What becomes of a page: a used page below U stays, a hole takes another page's values, a free page above U and a used
+// one, whose rank among those is the place of its hole in the list.
+constexpr int kStays = -1, kHole = -2;
+
+// U and, one workgroup a tile of pages, the lists of holes below U and of used pages from U up. Each workgroup
+// counts all pages for itself, from the L2 (the call on 128 Ki pages of 16 bytes: 226 us where one workgroup goes through
+// them in turn, 59 so; 1 Mi pages 1990 and 416).
+__global__ __launch_bounds__(kPlanThreads) void compact_plan(const int *references, int pages, int *used_out, int *moves,
+                                                             int *holes, int *movers, int *fate) {
+    __shared__ int scratch[kPlanWaves];
+    __shared__ long long sums[kPlanWaves];
+    const int used = used_among(references, pages, scratch);
+    const int used_below = used_among(references, used, scratch);      // of the first U pages
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *used_out = used;
+        *moves = used - used_below;
+    }
+    for (int p0 = blockIdx.x * kTile; p0 < pages; p0 += gridDim.x * kTile) {
+        // holes before a tile are its pages below U less the used ones; used pages from U up likewise
+        const int before = used_among(references, p0, scratch);
+        const int n_holes = p0 <= used ? p0 - before : 0, n_movers = p0 <= used ? 0 : before - used_below;
         const Counts<kPerThread> c(references, pages, p0);
+        // both in one prefix: holes in the low half of a word, movers in the high half
         long long mine = 0, total;
 #pragma unroll
         for (int u = 0; u < kPerThread; ++u) {
-            const int p = c.first + u;
-            if (p < used) mine += c.r[u] <= 0;
+            if (c.first + u < used) mine += c.r[u] <= 0;
             else if (c.r[u] > 0) mine += 1ll << 32;
         }
-        const long long before = prefix<long long>(mine, total, scratch);
-        int h = n_holes + static_cast<int>(before), m = n_movers + static_cast<int>(before >> 32);
+        const long long prior = prefix<long long>(mine, total, sums);
+        int h = n_holes + static_cast<int>(prior), m = n_movers + static_cast<int>(prior >> 32);
 #pragma unroll
         for (int u = 0; u < kPerThread; ++u) {
             const int p = c.first + u;
             if (p >= pages) break;
             const bool taken = c.r[u] > 0;
-            if (p < used && !taken) holes[h++] = p;
-            if (p >= used && taken) movers[m++] = p;
-            if (p >= used && !taken) place[p] = p;   // named by no count: a row that names it keeps it
+            int what = kStays;
+            if (p < used && !taken) {
+                holes[h++] = p;
+                what = kHole;
+            } else if (p >= used && taken) {
+                what = m;
+                movers[m++] = p;
+            }
+            fate[p] = what;
         }
-        n_holes += static_cast<int>(total);
-        n_movers += static_cast<int>(total >> 32);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_movers; i += kPlanThreads) place[movers[i]] = holes[i];
-    // counts: the used pages below U keep theirs, holes take their mover's; then 0 from U up
-    if (references_out != references)
-        for (int p = threadIdx.x; p < used; p += kPlanThreads) references_out[p] = references[p];
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_movers; i += kPlanThreads) references_out[holes[i]] = references[movers[i]];
-    __syncthreads();
-    for (int p = used + threadIdx.x; p < pages; p += kPlanThreads) references_out[p] = 0;
-    if (threadIdx.x == 0) {
-        *used_out = used;
-        *moves = n_movers;
     }
 }
 
@@ -385,26 +396,41 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages(PagesArgs a, const in
     copy_pairs<DENSE>(a, sources, destinations, count, parts, blockIdx.x, gridDim.x);
 }
 
-// The first row_groups workgroups rewrite the table, the others move the pages.
+// The first `groups` workgroups rewrite the table and the counts, the others move the pages.
 template <bool DENSE>
-__global__ __launch_bounds__(kCopyThreads) void compact_apply(PagesArgs a, const int *table, const int *used,
-                                                              const int *moves, const int *holes, const int *movers,
-                                                              const int *place, int parts, int row_groups) {
-    if (static_cast<int>(blockIdx.x) >= row_groups) {
-        copy_pairs<DENSE>(a, movers, holes, *moves, parts, blockIdx.x - row_groups, gridDim.x - row_groups);
+__global__ __launch_bounds__(kCopyThreads) void compact_apply(PagesArgs a, const int *table, const int *references,
+                                                              int *references_out, const int *used, const int *moves,
+                                                              const int *holes, const int *movers, const int *fate,
+                                                              int parts, int groups) {
+    if (static_cast<int>(blockIdx.x) >= groups) {
+        copy_pairs<DENSE>(a, movers, holes, *moves, parts, blockIdx.x - groups, gridDim.x - groups);
         return;
     }
     const int u = *used;
-    for (int s = blockIdx.x; s < a.sequences; s += row_groups) {
+    for (int s = blockIdx.x; s < a.sequences; s += groups) {
         const int n = pages_of(a, length_of(a, s));
         for (int j = threadIdx.x; j < a.row_pages; j += kCopyThreads) {
             const int64_t at = (int64_t)s * a.row_pages + j;
             int page = table[at];
             if (j < n) {
-                if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.pages)) kk::report(a.status, kk::kBadPage);
-                else if (page >= u) page = place[page];
+                if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.pages)) {
+                    kk::report(a.status, kk::kBadPage);
+                } else if (page >= u) {              // a row that names a free page keeps it
+                    const int rank = fate[page];
+                    page = rank >= 0 ? holes[rank] : page;
+                }
             }
             a.table[at] = page;
+        }
+    }
+    // each page's thread writes its own count, a mover's its hole's too; holes' threads touch none
+    for (int p = blockIdx.x * kCopyThreads + threadIdx.x; p < a.pool.pages; p += groups * kCopyThreads) {
+        const int what = fate[p];
+        if (p < u) {
+            if (what == kStays && references_out != references) references_out[p] = references[p];
+        } else {
+            if (what >= 0) references_out[holes[what]] = references[p];
+            references_out[p] = 0;
         }
     }
 }
@@ -483,18 +509,20 @@ extern "C" size_t kk_kv_compact_workspace_bytes(const kunlun::KVCacheLayout &c) 
 extern "C" int kk_kv_compact(void *k, void *v, int *table_out, int *references_out, int *used, const int *table,
                   const int *lengths, const int *references, const kunlun::KVCacheLayout &c,
                   const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus, hipStream_t stream) {
-    int *moves = static_cast<int *>(workspace), *holes = moves + 64, *movers = holes + c.pages, *place = movers + c.pages;
-    hipLaunchKernelGGL(compact_plan, dim3(1), dim3(kPlanThreads), 0, stream, references, references_out, c.pages, used,
-                       moves, holes, movers, place);
+    int *moves = static_cast<int *>(workspace), *holes = moves + 64, *movers = holes + c.pages, *fate = movers + c.pages;
+    const int tiles = (c.pages + kTile - 1) / kTile;
+    hipLaunchKernelGGL(compact_plan, dim3(std::min(tiles, cus)), dim3(kPlanThreads), 0, stream, references, c.pages, used,
+                       moves, holes, movers, fate);
     const PagesArgs a = args_of(k, v, table_out, const_cast<int *>(lengths), nullptr, c, p, status);
-    const int groups = std::min(p.sequences, 256), parts = parts_of(c);
+    const int groups = std::min(std::max(p.sequences, (c.pages + 4 * kCopyThreads - 1) / (4 * kCopyThreads)), 256);
+    const int parts = parts_of(c);
     const dim3 grid(groups + 8 * cus);
     if (dense(c))
-        hipLaunchKernelGGL(compact_apply<true>, grid, dim3(kCopyThreads), 0, stream, a, table, used, moves, holes,
-                           movers, place, parts, groups);
+        hipLaunchKernelGGL(compact_apply<true>, grid, dim3(kCopyThreads), 0, stream, a, table, references, references_out,
+                           used, moves, holes, movers, fate, parts, groups);
     else
-        hipLaunchKernelGGL(compact_apply<false>, grid, dim3(kCopyThreads), 0, stream, a, table, used, moves, holes,
-                           movers, place, parts, groups);
+        hipLaunchKernelGGL(compact_apply<false>, grid, dim3(kCopyThreads), 0, stream, a, table, references, references_out,
+                           used, moves, holes, movers, fate, parts, groups);
     return hipGetLastError();
 }
 

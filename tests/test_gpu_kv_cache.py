@@ -781,3 +781,26 @@ def test_logits(gpu, case):
         size = np.abs(z) * 2 + 2 + past + 30
         assert np.all(same | (np.abs(y - gold) <= 4 * 2.0 ** -24 * size))
     assert not np.any(np.isposinf(gold) ^ np.isposinf(y))
+
+
+def test_compact_large_pool(gpu):
+    """Lists over several workgroups: more pages than one takes, holes and used pages anywhere, counts in place and apart."""
+    rng = np.random.default_rng(51)
+    for pages, share in ((20000, 0.5), (20000, 0.97), (30001, 0.05), (8192, 1.0), (8193, 0.0)):
+        book = Book(rng, 50, pages // 50 + 1, pages, 1, heads=1, width=8, layers=1)
+        ids = rng.permutation(pages)[: int(pages * share)]
+        for s, part in enumerate(np.array_split(ids, 50)):
+            book.table[s, :len(part)], book.lengths[s] = part, len(part)
+        book.references[ids] = rng.integers(1, 4, len(ids))
+        book.upload()
+        used, = lists([-1])
+        args = (book.cache.layout, book.pages)
+        t, c = upload(np.zeros_like(book.table)), upload(np.full_like(book.references, 77))
+        total = book.compact()
+        assert kl.kv_compact(book.kernel, 0, *book.pools, t.data, c.data, used.data, *book.p, *args)
+        finish()
+        assert used.download(1, np.int32)[0] == total == len(ids)
+        assert np.array_equal(t.download(book.table.shape, np.int32), book.table)
+        assert np.array_equal(c.download(book.references.shape, np.int32), book.references)
+        assert kl.kv_compact(book.kernel, 0, *book.pools, book.p[0], book.p[2], used.data, *book.p, *args)
+        book.check()
