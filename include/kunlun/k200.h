@@ -6,7 +6,8 @@
 // so a consumer of that subset rebuilds against this library unchanged.
 // Declarations of the reference that are not on the matmul path (attention,
 // Q6_K, KV caches, row gathers) are not
-// declared here. matmul_swiglu has no reference counterpart (see below).
+// declared here. matmul_swiglu, the paged key-value cache with its attention and
+// process_logits have no reference counterpart (see below).
 //
 // Device numbering: the reference drives the two processing dies of one
 // Kunlun card as devices 0 and 1. Here a device is one HIP device (one GPU);

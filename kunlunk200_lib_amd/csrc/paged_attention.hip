@@ -6,7 +6,7 @@
 // F32, exponents in base 2 (log2(e) goes into q).
 //
 // A workgroup takes one key-value head of one sequence (all of its query heads,
-// so that the cache is read once) over one chunk of tokens; its four waves
+// so that the cache is read once) over one chunk of its tokens; its four (or eight) waves
 // take steps of 32 tokens in turn. Both products run on
 // v_mfma_f32_16x16x32_f16 with the cache's rows as one operand:
 //   scores  [16 tokens x 16 columns] += K rows (as stored)  x  q columns
@@ -21,15 +21,22 @@
 // into fp16 parts x = hi + lo (hi 11 bits, lo the next 11), hi in column c and lo in
 // column c + 8 of one tile; the two columns' sums are added at the end. So F32
 // queries and weights cost no instruction more than F16 ones with 8 query heads
-// or fewer, and errors stay at 2^-22. q is scaled by a power of two
+// or fewer, and errors stay at 2^-22 (against 64 bits 1.4e-7 relative over 4096 tokens, where
+// products in F32 one by one leave 2.4e-7). q is scaled by a power of two
 // (max |q| in [2^10, 2^11)) and the weights by 2^14, so that what the low
 // parts lose below 2^-24 stays far below that.
 //
-// What bounds it: reading the cache (4 * width bytes per token and head).
+// What bounds it: reading the cache (4 * width bytes per token and head). A step's K rows
+// are reloaded behind its scores and its V rows behind its second product, so a wave has 8
+// to 16 KiB on their way at any time, three workgroups to a CU; 32 sequences of up to 4096 tokens x 32 heads of
+// 128 (1.2 GB) take 187..196 us, 6.2 TB/s, what a kernel that only reads reaches; one of 32768 tokens x 8 heads
+// 24.5 us (5.5 TB/s) and 4.5 for the join. Below some ten MB it is the chain of latencies (length and pages, rows,
+// two products, the waves' sums): 33 tokens x 32 heads 5.6 us of kernel.
 //
 // Sequences of more than one chunk leave (sum w v, m, sum w) per chunk in the
 // workspace; a second launch joins them in order, so results do not
-// depend on the order in which chunks end.
+// depend on the order in which chunks end. (Joined by the workgroup that ends last instead, the sums have to
+// go past the XCDs' own L2s: 1 x 32768 tokens 49 us against 29, and 100 with fences that write the L2s back.)
 #include "device_common.h"
 #include "launch.h"
 #include "paged.h"
@@ -503,10 +510,11 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
 // one thread per chunk; then groups of threads take the chunks in turn, 4 values
 // each, and the groups' sums are added in order.
 constexpr int kJoinRun = 1024;                       // chunks whose weights wait in LDS at a time
-__global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void join_chunks(AttendArgs a) {
     __shared__ float weights[kJoinRun];
-    __shared__ float4v sums[kThreads];
-    __shared__ float reduce[kWaves];
+    __shared__ float4v sums[THREADS];
+    __shared__ float reduce[THREADS / kWave];
     const int h = blockIdx.x, s = blockIdx.y, width = a.pool.width, tid = threadIdx.x;
     const int len = length_of(a, s, false);
     const int base = (a.window > 0 ? max(0, len - a.window) : 0) & ~(kStep - 1);
@@ -515,23 +523,23 @@ __global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
     const int64_t at = ((int64_t)s * a.query_heads + h) * a.chunks;
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
     const float4v *o = reinterpret_cast<const float4v *>(a.part_o + at * width);
-    const int vectors = width / 4, groups = kThreads / vectors;
+    const int vectors = width / 4, groups = THREADS / vectors;
     const int group = tid / vectors, at4 = tid - group * vectors;
 
     float top = -INFINITY;
-    for (int i = tid; i < n; i += kThreads) top = fmaxf(top, ml[i].x);
+    for (int i = tid; i < n; i += THREADS) top = fmaxf(top, ml[i].x);
     top = kk::wave_max(top);
     if (tid % kWave == 0) reduce[tid / kWave] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, reduce[w]);
+    for (int w = 0; w < THREADS / kWave; ++w) top = fmaxf(top, reduce[w]);
     __syncthreads();
 
     float total = 0.0f;
     float4v sum{0, 0, 0, 0};
     for (int i0 = 0; i0 < n; i0 += kJoinRun) {
         const int run = min(kJoinRun, n - i0);
-        for (int i = tid; i < run; i += kThreads) {
+        for (int i = tid; i < run; i += THREADS) {
             const float2 x = ml[i0 + i];
             const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - top);
             weights[i] = w;
@@ -560,7 +568,7 @@ __global__ __launch_bounds__(kThreads) void join_chunks(AttendArgs a) {
     __syncthreads();
     total = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += reduce[w];
+    for (int w = 0; w < THREADS / kWave; ++w) total += reduce[w];
     if (tid < vectors) {
         for (int g = 1; g < groups; ++g) sum += sums[g * vectors + tid];
 #pragma unroll
@@ -617,7 +625,7 @@ template <int D32, int VW, int NT, bool UNI, bool FULL, bool ONCE, int WAVES>
 hipError_t launch(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     const size_t ids = UNI ? 0 : (p.chunk / a.pool.page_tokens + 2) * sizeof(int);
     const size_t sums = (size_t)WAVES * (NT * 8 * 2 + std::min(p.group, 8 * NT) * 16 * VW) * sizeof(float);
-    const size_t lds = std::max(ids, sums);          // at most 33 KiB
+    const size_t lds = std::max(ids, sums);          // up to 33 KiB
     hipLaunchKernelGGL((attend<D32, VW, NT, UNI, FULL, ONCE, WAVES>), dim3(heads * p.tiles, sequences, p.chunks),
                        dim3(WAVES * kWave), lds, stream, a);
     return hipGetLastError();
@@ -690,6 +698,8 @@ extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const v
     else if (c.width <= 192) rc = launch_width<6, 16>(a, r, p.sequences, c.heads, stream);
     else rc = launch_width<8, 16>(a, r, p.sequences, c.heads, stream);
     if (rc != hipSuccess || r.chunks == 1) return rc;
-    hipLaunchKernelGGL(join_chunks, dim3(p.query_heads, p.sequences), dim3(kThreads), 0, stream, a);
+    // one wave where there is little to join
+    if (r.chunks <= 4) hipLaunchKernelGGL(join_chunks<kWave>, dim3(p.query_heads, p.sequences), dim3(kWave), 0, stream, a);
+    else hipLaunchKernelGGL(join_chunks<kThreads>, dim3(p.query_heads, p.sequences), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
