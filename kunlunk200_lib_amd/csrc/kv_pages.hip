@@ -314,17 +314,27 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan(const int *referenc
                                                              int *holes, int *movers, int *fate) {
     __shared__ int scratch[kPlanWaves];
     __shared__ long long sums[kPlanWaves];
-    const int used = used_among(references, pages, scratch);
-    const int used_below = used_among(references, used, scratch);      // of the first U pages
+    // a pool of one tile is read once: its counts stay in registers
+    const bool one = pages <= kTile;
+    const Counts<kPerThread> all(references, one ? pages : 0, 0);
+    auto used_here = [&](int n) {
+        int mine = 0, total;
+#pragma unroll
+        for (int u = 0; u < kPerThread; ++u) mine += all.r[u] > 0 && all.first + u < n;
+        prefix<int>(mine, total, scratch);
+        return total;
+    };
+    const int used = one ? used_here(pages) : used_among(references, pages, scratch);
+    const int used_below = one ? used_here(used) : used_among(references, used, scratch);      // of the first U pages
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         *used_out = used;
         *moves = used - used_below;
     }
     for (int p0 = blockIdx.x * kTile; p0 < pages; p0 += gridDim.x * kTile) {
         // holes before a tile are its pages below U less the used ones; used pages from U up likewise
-        const int before = used_among(references, p0, scratch);
+        const int before = p0 > 0 ? used_among(references, p0, scratch) : 0;
         const int n_holes = p0 <= used ? p0 - before : 0, n_movers = p0 <= used ? 0 : before - used_below;
-        const Counts<kPerThread> c(references, pages, p0);
+        const Counts<kPerThread> c = one ? all : Counts<kPerThread>(references, pages, p0);
         // both in one prefix: holes in the low half of a word, movers in the high half
         long long mine = 0, total;
 #pragma unroll

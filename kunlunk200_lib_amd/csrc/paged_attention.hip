@@ -6,7 +6,7 @@
 // F32, exponents in base 2 (log2(e) goes into q).
 //
 // A workgroup takes one key-value head of one sequence (all of its query heads,
-// so that the cache is read once) over one chunk of its tokens; its four (or eight) waves
+// so that the cache is read once) over one chunk of its tokens; its four (one, eight) waves
 // take steps of 32 tokens in turn. Both products run on
 // v_mfma_f32_16x16x32_f16 with the cache's rows as one operand:
 //   scores  [16 tokens x 16 columns] += K rows (as stored)  x  q columns
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(THREADS) void join_chunks(AttendArgs a) {
 
 struct Plan {
     int group, nt, tiles, chunk, chunks;
-    bool once, wide;
+    bool once, wide, narrow;
 };
 
 Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus) {
@@ -612,6 +612,10 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int64_t parts = std::min(std::max((longest + split - 1) / split, least_parts), most_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
+    // One wave to a workgroup for many rows of up to four steps (512 sequences x 8 heads: 2 / 64 / 128 tokens 33 / 41 / 60 us
+    // on four waves, 17 / 33 / 55 on one, 256 tokens 97 / 102; 64 x 8: 128 tokens 10.6 / 11.2; width 256, 60 x 64 tokens x 32
+    // heads 61 / 35)
+    r.narrow = r.nt == 1 && rows > 2 * cus && longest <= 4 * kStep;
     // The non-temporal hint, for reads that fill the 256 MiB cache with nothing that is read again: one tile, a head's
     // rows one after the other, more than a quarter of it (32 x 4096 tokens x 32 heads 209 us, with the hint 192;
     // 64 x 1024 tokens x 8 heads of 64 34.9 / 30.7; 16 x 1024 x 8 of 128 19.0 / 20.3; tiles that read the same
@@ -645,6 +649,7 @@ hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int h
 
 template <int D32, int VW>
 hipError_t launch_width(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
+    if (p.narrow) return launch_tiles<D32, VW, 1, 1>(a, p, sequences, heads, stream);
     if constexpr (VW <= 8) {
         if (p.nt == 2) return launch_tiles<D32, VW, 2, kWaves>(a, p, sequences, heads, stream);
         if (p.wide) return launch_tiles<D32, VW, 1, kWideWaves>(a, p, sequences, heads, stream);
