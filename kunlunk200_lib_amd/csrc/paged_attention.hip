@@ -59,6 +59,7 @@ constexpr int kStep = 32;                // tokens of a wave's step
 constexpr int kMinChunk = kWaves * kStep;
 constexpr int kMaxChunk = 512, kMaxChunkMany = 1024;
 constexpr int kMostChunks = 65535;       // the grid's limit
+constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
 constexpr float kWeightLog2 = 14.0f;     // weights are scaled by 2^14
 
 struct AttendArgs {
@@ -577,13 +578,17 @@ __global__ __launch_bounds__(THREADS) void join_chunks(AttendArgs a) {
     }
 }
 
+// Whether the 16 tokens of a half step are in one page; lane offsets within them are 32-bit.
+bool in_halves(const kunlun::KVCacheLayout &c) { return c.page_tokens % 16 == 0 && c.token_stride < (1 << 26); }
+
 struct Plan {
     int group, nt, tiles, chunk, chunks;
-    bool once, wide, narrow;
+    bool halves, once, wide, narrow;
 };
 
 Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus) {
     Plan r;
+    r.halves = in_halves(c);
     r.group = p.query_heads / c.heads;
     r.nt = r.group > 8 && c.width <= 128 ? 2 : 1;
     r.tiles = (r.group + 8 * r.nt - 1) / (8 * r.nt);
@@ -608,8 +613,10 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int64_t split = std::max({wanted, least, (int64_t)(longest + kMostChunks - 1) / kMostChunks});
     const int64_t least_parts = rows >= 2 * cus && longest > many ? 3 : 1;
     // and a bound on the workgroups that find no tokens where `longest` is far above the lengths
-    const int64_t most_parts = std::max<int64_t>((1 << 12) / rows, least_parts);
-    const int64_t parts = std::min(std::max((longest + split - 1) / split, least_parts), most_parts), chunk = (longest + parts - 1) / parts;
+    // (but page ids that wait in LDS have to fit)
+    const int64_t id_parts = r.halves ? 1 : (longest + kMostIds * c.page_tokens - 1) / (kMostIds * (int64_t)c.page_tokens);
+    const int64_t most_parts = std::max({(1 << 12) / rows, least_parts, id_parts});
+    const int64_t parts = std::max(std::min(std::max((longest + split - 1) / split, least_parts), most_parts), id_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
     // One wave to a workgroup for many rows of up to four steps (512 sequences x 8 heads: 2 / 64 / 128 tokens 33 / 41 / 60 us
@@ -637,9 +644,7 @@ hipError_t launch(const AttendArgs &a, const Plan &p, int sequences, int heads, 
 
 template <int D32, int VW, int NT, int WAVES>
 hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
-    // lane offsets within 16 tokens are 32-bit
-    const bool uni = a.pool.page_tokens % 16 == 0 && a.pool.token_stride < (1 << 26);
-    if (!uni) return launch<D32, VW, NT, false, false, false, WAVES>(a, p, sequences, heads, stream);
+    if (!p.halves) return launch<D32, VW, NT, false, false, false, WAVES>(a, p, sequences, heads, stream);
     if (a.pool.width != 32 * D32) return launch<D32, VW, NT, true, false, false, WAVES>(a, p, sequences, heads, stream);
     if constexpr (WAVES == kWaves) {
         if (p.once) return launch<D32, VW, NT, true, true, true, WAVES>(a, p, sequences, heads, stream);

@@ -804,3 +804,52 @@ def test_compact_large_pool(gpu):
         assert np.array_equal(c.download(book.references.shape, np.int32), book.references)
         assert kl.kv_compact(book.kernel, 0, *book.pools, book.p[0], book.p[2], used.data, *book.p, *args)
         book.check()
+
+
+@pytest.mark.parametrize("page_tokens", [1, 3, 16])
+@pytest.mark.parametrize("sequences,heads", [(1, 1), (70, 8)])
+def test_attention_loose_bound(gpu, page_tokens, sequences, heads):
+    """`longest` far above the lengths: rows of many entries, most of which are never read."""
+    rng = np.random.default_rng(61)
+    longest = 1 << 20 if sequences == 1 else 150000
+    lengths = [int(n) for n in rng.integers(1, 40, sequences)]
+    lengths[-1] = 700
+    pages = sum(-(-n // page_tokens) for n in lengths) + 1
+    cache = Cache(rng, pages, page_tokens, heads, 64)
+    table = table_of(rng, lengths, page_tokens, pages, -(-longest // page_tokens), rest=-7)
+    q = rng.standard_normal((sequences, heads, 64)).astype(np.float32)
+    y, _ = run_attention(cache, table, lengths, q, longest=longest)
+    gold, tol = gold_attention(cache, table, lengths, q, 0, 0.125)
+    check(y, gold, tol)
+    assert gpu.kv_cache_status(0) == 0
+
+
+def test_attention_subnormal_values(gpu):
+    """F16 values below 2^-14 count in full, as keys and as values."""
+    rng = np.random.default_rng(62)
+    lengths = [100, 33]
+    cache = Cache(rng, 20, 16, 2, 64)
+    cache.flat[1][:] = (rng.integers(-1023, 1024, cache.flat[1].size) * 2.0 ** -24).astype(np.float16)
+    cache.flat[0][:] = (rng.integers(-1023, 1024, cache.flat[0].size) * 2.0 ** -24).astype(np.float16)
+    table = table_of(rng, lengths, 16, 20, 7)
+    q = rng.standard_normal((2, 4, 64)).astype(np.float32)
+    y, _ = run_attention(cache, table, lengths, q, scale=4096.0)
+    gold, tol = gold_attention(cache, table, lengths, q, 0, 4096.0)
+    assert np.abs(gold).max() < 2.0 ** -14 and np.abs(gold).max() > 2.0 ** -18
+    check(y, gold, tol)
+
+
+def test_attention_many_rows(gpu):
+    """More rows than the card holds at once, short and ragged: one wave to a workgroup and whole rows."""
+    rng = np.random.default_rng(63)
+    for most, width in ((3, 64), (97, 72), (128, 128), (129, 64), (500, 64)):
+        lengths = [int(n) for n in rng.integers(0, most + 1, 140)]
+        lengths[7] = most
+        pages = sum(-(-n // 16) for n in lengths) + 1
+        cache = Cache(rng, pages, 16, 8, width)
+        table = table_of(rng, lengths, 16, pages, -(-most // 16), rest=99999999)
+        q = rng.standard_normal((140, 8, width)).astype(np.float32)
+        y, route = run_attention(cache, table, lengths, q)
+        assert route == "paged_attention"
+        gold, tol = gold_attention(cache, table, lengths, q, 0, width ** -0.5)
+        check(y, gold, tol)
