@@ -595,18 +595,18 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
     // No split, so no second launch: eight waves to a workgroup for rows of up to 512 tokens, or 1024 where they
-    // leave few CUs idle (us, against the split: 4 x 160 / 320 / 512 tokens x 8 heads 7.0 / 7.8 / 8.8, 10.5 split; at 768
-    // 12.3 / 11.3; 32 x 512 / 1024 x 8 heads 13.9 / 27.8, split 19.1 / 30.5), four for more rows of up to 512.
+    // leave few CUs idle (us, against the split: 4 x 160 / 320 / 512 tokens x 8 heads 7.2 / 8.0 / 9.1, 10.3 / 10.5 / 10.6 split;
+    // eight waves at 768 12.3, split 11.8; 32 x 512 / 1024 x 8 heads 14.2 / 28.3, split 18.7 / 29.9), four for more rows of up to 512.
     const int whole = kMaxChunk + kStep;             // a window starts up to kStep - 1 tokens early
     r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
              longest <= (rows > cus / 2 ? 2 * whole : whole);
     const int64_t least = r.wide ? longest : rows > cus && longest <= whole ? longest : kMinChunk;
-    // Otherwise two workgroups' tokens to a CU, in parts of one size. Parts of up to 512 tokens; with two rows and more to
-    // a CU whole rows of up to 1024 and, above, at least three parts of up to 1024: each part costs its start and its
-    // end, and few long ones wait for the last (1 x 32768 tokens x 8 heads 29 us, parts of 256 31.7; 64 x 1024 x 8
-    // 46, split in two 54; ragged to 1500, 128 x 8: two parts 117, three 94, four 102; ragged to 3000: 168, of 512 176).
-    // (of workgroups that a CU holds one or two of instead of three, twice as many: 64 x 2048 x 8 heads of 256 210 us in
-    // three parts, 174 whole; groups of 16 query heads 128 / 92).
+    // Otherwise two workgroups' tokens to a CU, in parts of one size: of up to 512 tokens (1 x 32768 tokens x 8 heads
+    // 29.1 us, of 256 32.0); with two rows and more to a CU whole rows of up to 1024 (64 x 640 / 1024 tokens x 8 heads
+    // 30 / 46, in parts of 512 40 / 54) and, above, at least three parts of up to 1024 (64 x 8 heads ragged to 2048: two
+    // parts 64.7, three 61.9, four 61.1; all of 2048: 92.9, 94.0, 95.7); of workgroups that a CU holds one or two of
+    // instead of three, twice as many tokens (64 x 2048 x 8 heads of 256 175 whole, 204 in three parts; groups of 16 query
+    // heads 92 / 117).
     const int many = c.width > 128 || r.nt == 2 ? 2 * kMaxChunkMany : kMaxChunkMany;
     const int64_t most = rows >= 2 * cus ? many : kMaxChunk;
     const int64_t wanted = std::min<int64_t>((longest * rows + 2 * cus - 1) / (2 * cus), most);
@@ -619,16 +619,15 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int64_t parts = std::max(std::min(std::max((longest + split - 1) / split, least_parts), most_parts), id_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
-    // One wave to a workgroup for many rows of up to four steps (512 sequences x 8 heads: 2 / 64 / 128 tokens 33 / 41 / 60 us
-    // on four waves, 17 / 33 / 55 on one, 256 tokens 97 / 102; 64 x 8: 128 tokens 10.6 / 11.2; width 256, 60 x 64 tokens x 32
+    // One wave to a workgroup for many rows of up to four steps (512 sequences x 8 heads: 2 / 64 / 128 tokens 32 / 41 / 59 us
+    // on four waves, 17 / 32 / 55 on one, 256 tokens 97 / 102; 64 x 8: 128 tokens 10.6 / 11.2; width 256, 60 x 64 tokens x 32
     // heads 61 / 35)
     r.narrow = r.nt == 1 && rows > 2 * cus && longest <= 4 * kStep;
-    // The non-temporal hint, for reads that fill the 256 MiB cache with nothing that is read again: one tile, a head's
-    // rows one after the other, more than a quarter of it (32 x 4096 tokens x 32 heads 209 us, with the hint 192;
-    // 64 x 1024 tokens x 8 heads of 64 34.9 / 30.7; 16 x 1024 x 8 of 128 19.0 / 20.3; tiles that read the same
-    // rows 104 / 137; rows that share cache lines, 64 x 1024 x 8 of 80, 50 / 55).
-    r.once = r.tiles == 1 && c.token_stride == c.width &&
-             (int64_t)p.sequences * longest * c.heads * c.width * 4 > (64 << 20);
+    // The non-temporal hint, for reads of whole cache lines that fill more than a quarter of the 256 MiB cache with
+    // nothing that is read again (us, with the hint and without: 32 x 4096 tokens x 32 heads 196 / 218; 64 x 4096 x 8 in
+    // token order 198 / 207; 64 x 1024 x 8 of 64 25.4 / 28.3; 16 x 1024 x 8, 67 MB, 20.1 / 18.9; tiles that read the same
+    // rows, 32 query heads on one, 107 / 96; rows that share lines, 64 x 1024 x 8 of 80, 40.5 / 38.4).
+    r.once = r.tiles == 1 && (int64_t)p.sequences * longest * c.heads * c.width * 4 > (64 << 20);
     return r;
 }
 
