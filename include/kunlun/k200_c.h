@@ -278,7 +278,8 @@ const char *kunlun_paged_attention_reason(const kunlun_kv_cache_layout *cache,
 const char *kunlun_kv_append_reason(const kunlun_kv_cache_layout *cache, const kunlun_kv_append_layout *call);
 const char *kunlun_kv_pages_reason(const kunlun_kv_cache_layout *cache, const kunlun_kv_pages_layout *pages);
 const char *kunlun_logits_reason(const kunlun_logits_layout *call);
-/* kv_cache_status(): completes the device's work; what its kernels met since the last call (a sum of these), -1: no such device. */
+/* kv_cache_status(): completes the device's work; what its kernels met since the
+ * last call (a sum of these), -1: no such device. */
 enum { KUNLUN_KV_BAD_PAGE = 1, KUNLUN_KV_BAD_INDEX = 2, KUNLUN_KV_NO_PAGE = 4 };
 int kunlun_kv_cache_status(int device);
 int kunlun_paged_attention(kunlun_kernel *kernel, int device, void *y, const void *q, const void *k, const void *v,

@@ -227,7 +227,8 @@ const char * kv_pages_reason(const KVCacheLayout & c, const KVPagesLayout & p) {
     if (*cache) return cache;
     if (p.sequences <= 0 || p.row_pages <= 0 || p.layers <= 0 || p.layers > 65535) return "shape";
     if ((int64_t)p.row_pages * c.page_tokens > kMostTokens) return "length";
-    if (p.layers > 1 && (p.layer_stride < pool_elements(c) || p.layer_stride > (INT64_MAX / 4) / p.layers || p.layer_stride % 8))
+    if (p.layers > 1 && (p.layer_stride < pool_elements(c) || p.layer_stride > (INT64_MAX / 4) / p.layers ||
+                         p.layer_stride % 8))
         return "stride";
     return "";
 }
@@ -395,7 +396,8 @@ bool process_logits(Kernel & kernel, int id, void * y, const void * logits, cons
         return false;
     const Span out = rows_span(y, p.rows, p.y_stride, p.vocabulary, 4);
     const Span in = rows_span(logits, p.rows, p.logits_stride, p.vocabulary, 4);
-    const Span past = ints(history, (int64_t)p.rows * p.history_stride), pasts = ints(history ? history_lengths : nullptr, p.rows);
+    const Span past = ints(history, (int64_t)p.rows * p.history_stride);
+    const Span pasts = ints(history ? history_lengths : nullptr, p.rows);
     const Span factors = ints(history ? penalties : nullptr, (int64_t)3 * p.rows);
     const Span ids = ints(bias_ids, (int64_t)p.rows * p.bias_stride);
     const Span biases = ints(bias_ids ? bias_values : nullptr, (int64_t)p.rows * p.bias_stride);

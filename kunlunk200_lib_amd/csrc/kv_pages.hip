@@ -515,7 +515,9 @@ extern "C" int kk_kv_free(int *table, int *lengths, int *references, const int *
     return hipGetLastError();
 }
 
-extern "C" size_t kk_kv_compact_workspace_bytes(const kunlun::KVCacheLayout &c) { return ((size_t)3 * c.pages + 64) * sizeof(int); }
+extern "C" size_t kk_kv_compact_workspace_bytes(const kunlun::KVCacheLayout &c) {
+    return ((size_t)3 * c.pages + 64) * sizeof(int);
+}
 extern "C" int kk_kv_compact(void *k, void *v, int *table_out, int *references_out, int *used, const int *table,
                   const int *lengths, const int *references, const kunlun::KVCacheLayout &c,
                   const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus, hipStream_t stream) {

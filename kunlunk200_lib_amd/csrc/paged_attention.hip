@@ -478,7 +478,8 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) v[u] = acc[nt][j + u][r] + other_part(acc[nt][j + u][r]);
                 if (mine)
-                    *reinterpret_cast<float4v *>(wave_o + (wave * heads + h) * DPad + (j / 8) * 128 + (4 * G + r) * VP + j % 8) = v;
+                    *reinterpret_cast<float4v *>(wave_o + (wave * heads + h) * DPad + (j / 8) * 128 + (4 * G + r) * VP +
+                                                 j % 8) = v;
             }
     }
     __syncthreads();
@@ -595,8 +596,9 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
     // No split, so no second launch: eight waves to a workgroup for rows of up to 512 tokens, or 1024 where they
-    // leave few CUs idle (us, against the split: 4 x 160 / 320 / 512 tokens x 8 heads 7.2 / 8.0 / 9.1, 10.3 / 10.5 / 10.6 split;
-    // eight waves at 768 12.3, split 11.8; 32 x 512 / 1024 x 8 heads 14.2 / 28.3, split 18.7 / 29.9), four for more rows of up to 512.
+    // leave few CUs idle, four for more rows of up to 512 (us, against the split: 4 x 160 / 320 / 512 tokens x 8 heads
+    // 7.2 / 8.0 / 9.1, split 10.3 / 10.5 / 10.6; eight waves at 768 12.3, split 11.8; 32 x 512 / 1024 x 8 heads
+    // 14.2 / 28.3, split 18.7 / 29.9).
     const int whole = kMaxChunk + kStep;             // a window starts up to kStep - 1 tokens early
     r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
              longest <= (rows > cus / 2 ? 2 * whole : whole);
@@ -616,7 +618,8 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     // (but page ids that wait in LDS have to fit)
     const int64_t id_parts = r.halves ? 1 : (longest + kMostIds * c.page_tokens - 1) / (kMostIds * (int64_t)c.page_tokens);
     const int64_t most_parts = std::max({(1 << 12) / rows, least_parts, id_parts});
-    const int64_t parts = std::max(std::min(std::max((longest + split - 1) / split, least_parts), most_parts), id_parts), chunk = (longest + parts - 1) / parts;
+    const int64_t asked = std::max((longest + split - 1) / split, least_parts);
+    const int64_t parts = std::max(std::min(asked, most_parts), id_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
     // One wave to a workgroup for many rows of up to four steps (512 sequences x 8 heads: 2 / 64 / 128 tokens 32 / 41 / 59 us
