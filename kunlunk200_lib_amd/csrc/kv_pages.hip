@@ -27,6 +27,7 @@ struct PagesArgs {
     int *table, *lengths, *references;
     int *status;
     PoolView pool;
+    kk::FastDiv per_row;                 // 16-byte vectors of a token's head
     int64_t layer_stride;
     int sequences, row_pages, layers;
 };
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(kCopyThreads) void fork_apply(PagesArgs a, const in
         const _Float16 *src = base + page * a.pool.page_stride;
         _Float16 *dst = base + note.page * a.pool.page_stride;
         for (int x = threadIdx.x; x < vectors; x += kCopyThreads) {
-            const int token = x / row_vectors, at = x - token * row_vectors;
+            const int token = a.per_row.div(x), at = x - token * row_vectors;
             const int64_t off = token * a.pool.token_stride + at * 8;
             *reinterpret_cast<uint4 *>(dst + off) = *reinterpret_cast<const uint4 *>(src + off);
         }
@@ -369,12 +370,12 @@ __device__ __forceinline__ void copy_page(const PagesArgs &a, _Float16 *pool, in
     const _Float16 *from = pool + src * a.pool.page_stride;
     _Float16 *to = pool + dst * a.pool.page_stride;
     const int row_vectors = a.pool.width / 8;
-    const int64_t vectors = (int64_t)a.pool.heads * a.pool.page_tokens * row_vectors;
-    for (int64_t x = (int64_t)part * kCopyThreads + threadIdx.x; x < vectors; x += (int64_t)parts * kCopyThreads) {
-        int64_t off = x * 8;
+    // up to 1024 x 65536 x 32 vectors
+    const uint32_t vectors = static_cast<uint32_t>(a.pool.heads) * a.pool.page_tokens * row_vectors;
+    for (uint32_t x = part * kCopyThreads + threadIdx.x; x < vectors; x += parts * kCopyThreads) {
+        int64_t off = (int64_t)x * 8;
         if constexpr (!DENSE) {
-            const int64_t row = x / row_vectors;
-            const int head = static_cast<int>(row / a.pool.page_tokens), token = static_cast<int>(row % a.pool.page_tokens);
+            const uint32_t row = a.per_row.div(x), head = a.pool.per_page.div(row), token = row - head * a.pool.page_tokens;
             off = head * a.pool.head_stride + token * a.pool.token_stride + (x - row * row_vectors) * 8;
         }
         *reinterpret_cast<uint4 *>(to + off) = *reinterpret_cast<const uint4 *>(from + off);
@@ -455,6 +456,7 @@ PagesArgs args_of(void *k, void *v, int *table, int *lengths, int *references, c
     a.references = references;
     a.status = status;
     a.pool = PoolView(c);
+    a.per_row = kk::FastDiv(static_cast<uint32_t>(c.width / 8));
     a.layer_stride = p.layer_stride;
     a.sequences = p.sequences;
     a.row_pages = p.row_pages;
