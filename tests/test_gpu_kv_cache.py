@@ -681,6 +681,25 @@ def test_pages_report(gpu):
     book.check(kl.KV_BAD_PAGE)
 
 
+def test_reserve_named_twice(gpu):
+    """Of two reservations for one sequence one counts; the other, which would end past the row, is reported."""
+    rng = np.random.default_rng(33)
+    book = Book(rng, 3, 5, 24, 8)
+    book.upload()
+    args = (book.cache.layout, book.pages)
+    r, a = lists([1, 0, 1], [30, 9, 30])
+    assert kl.kv_reserve(book.kernel, 0, *book.p, r.data, a.data, 3, *args)
+    finish()
+    assert kl.kv_cache_status(0) == kl.KV_BAD_INDEX
+    table, lengths, references = (b.download(x.shape, np.int32)
+                                  for b, x in zip(book.b, (book.table, book.lengths, book.references)))
+    assert lengths.tolist() == [9, 30, 0]
+    assert table[0].tolist() == [4, 5, -1, -1, -1] and table[2].tolist() == [-1] * 5
+    assert table[1].tolist() in ([0, 1, 2, 3, -1], [6, 7, 8, 9, -1])
+    held = np.bincount(table[table >= 0], minlength=24)
+    assert np.array_equal(references, held)
+
+
 @pytest.mark.parametrize("order,pad,count", [("heads", 0, 1), ("tokens", 0, 40), ("heads", 1, 40), ("tokens", 1, 3)])
 def test_copy_pages(gpu, order, pad, count):
     rng = np.random.default_rng(33)
