@@ -193,7 +193,7 @@ struct ForkNote {
 // Workgroup 0 finds the pages; workgroup 1 + i copies the parent's row aside (a
 // parent may be a child whose row the second launch overwrites).
 __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int *parents, const int *children,
-                                                          int count, ForkNote *notes, int *found, int *rows) {
+                                                          int count, ForkNote *notes, int *found, int *rows, int *claims) {
     if (blockIdx.x > 0) {
         const int i = blockIdx.x - 1, s = parents[i];
         if (static_cast<unsigned>(s) >= static_cast<unsigned>(a.sequences)) return;
@@ -207,7 +207,10 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
         const int i = i0 + threadIdx.x;
         int length = -1;
-        if (i < count && sequence_ok(a, parents[i]) && sequence_ok(a, children[i])) length = length_of(a, parents[i]);
+        if (i < count && sequence_ok(a, parents[i]) && sequence_ok(a, children[i])) {
+            length = length_of(a, parents[i]);
+            claims[children[i]] = i;             // of forks to one child the last store's is made
+        }
         const bool part = length > 0 && length % a.pool.page_tokens != 0;
         int total;
         const int at = wanted + prefix<int>(part, total, scratch);
@@ -216,7 +219,14 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int
     }
     const int have = free_pages(a.references, a.pool.pages, min(wanted, a.pool.pages), found, scratch);
     for (int i = threadIdx.x; i < count; i += kPlanThreads) {
-        const int at = notes[i].page;
+        const ForkNote note = notes[i];
+        if (note.length < 0) continue;
+        if (claims[children[i]] != i) {
+            notes[i].length = -1;
+            kk::report(a.status, kk::kBadIndex);
+            continue;
+        }
+        const int at = note.page;
         if (at >= 0) notes[i].page = at < have ? found[at] : -2;
         if (at >= have && at >= 0) kk::report(a.status, kk::kNoPage);
     }
@@ -505,16 +515,17 @@ extern "C" int kk_kv_reserve(int *table, int *lengths, int *references, const in
 }
 
 extern "C" size_t kk_kv_fork_workspace_bytes(const kunlun::KVPagesLayout &p, int count) {
-    return (size_t)count * (sizeof(ForkNote) + sizeof(int) + (size_t)p.row_pages * sizeof(int));
+    return (size_t)count * (sizeof(ForkNote) + sizeof(int) + (size_t)p.row_pages * sizeof(int)) +
+           (size_t)p.sequences * sizeof(int);
 }
 extern "C" int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *references, const int *parents, const int *children,
                int count, const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
                hipStream_t stream) {
     const PagesArgs a = args_of(k, v, table, lengths, references, c, p, status);
     ForkNote *notes = static_cast<ForkNote *>(workspace);
-    int *found = reinterpret_cast<int *>(notes + count), *rows = found + count;
+    int *found = reinterpret_cast<int *>(notes + count), *claims = found + count, *rows = claims + p.sequences;
     hipLaunchKernelGGL(fork_plan, dim3(1 + count), dim3(kPlanThreads), 0, stream, a, parents, children, count, notes,
-                       found, rows);
+                       found, rows, claims);
     // at most eight (layer, pool, head) blocks of the last page per workgroup
     const int blocks = p.layers * 2 * c.heads, copiers = std::max(1, std::min(blocks, 4096 / count));
     hipLaunchKernelGGL(fork_apply, dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);

@@ -700,6 +700,34 @@ def test_reserve_named_twice(gpu):
     assert np.array_equal(references, held)
 
 
+def test_fork_named_twice(gpu):
+    """Of two forks to one child one is made; the other is reported, and every count is its page's rows."""
+    rng = np.random.default_rng(34)
+    book = Book(rng, 4, 5, 24, 8)
+    book.upload()
+    args = (book.cache.layout, book.pages)
+    r, a = lists([0, 1, 2], [30, 17, 9])
+    book.reserve([0, 1, 2], [30, 17, 9])
+    assert kl.kv_reserve(book.kernel, 0, *book.p, r.data, a.data, 3, *args)
+    p, c = lists([0, 1, 0], [2, 2, 3])
+    assert kl.kv_fork(book.kernel, 0, *book.pools, *book.p, p.data, c.data, 3, *args)
+    finish()
+    assert kl.kv_cache_status(0) == kl.KV_BAD_INDEX
+    table, lengths, references = (b.download(x.shape, np.int32)
+                                  for b, x in zip(book.b, (book.table, book.lengths, book.references)))
+    assert lengths[[0, 1, 3]].tolist() == [30, 17, 30] and lengths[2] in (30, 17)
+    assert np.array_equal(table[:2], book.table[:2])
+    parent = 0 if lengths[2] == 30 else 1
+    for child, of in ((2, parent), (3, 0)):
+        full = int(lengths[of]) // 8
+        assert np.array_equal(table[child, :full], book.table[of, :full])
+        assert np.all(table[child, full + 1:] == -1)
+        for view, pool in zip(book.cache.download()[1], book.want):
+            rest = int(lengths[of]) % 8
+            assert np.array_equal(view[:, table[child, full], :, :rest], pool[:, book.table[of, full], :, :rest])
+    assert np.array_equal(references, np.bincount(table[table >= 0], minlength=24))
+
+
 @pytest.mark.parametrize("order,pad,count", [("heads", 0, 1), ("tokens", 0, 40), ("heads", 1, 40), ("tokens", 1, 3)])
 def test_copy_pages(gpu, order, pad, count):
     rng = np.random.default_rng(33)
