@@ -142,6 +142,105 @@ __device__ __forceinline__ T load_row(const _Float16 *p) {
     else return *reinterpret_cast<const T *>(p);
 }
 
+// q columns: column c is head c % 8 of each tile, its high (c < 8) or low part; the scores times `undo` are in base 2.
+template <int D32, int NT, bool FULL>
+__device__ __forceinline__ void split_queries(float scale_log2, int heads, int width, int c, int G, float (&q)[NT][D32][8],
+                                              half8 (&qf)[NT][D32], float (&undo)[NT]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float scale = nt * 8 + (c & 7) < heads ? scale_log2 : 0.0f;
+        float top = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D32; ++d) {
+            const bool in = FULL || d * 32 + G * 8 < width;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                q[nt][d][i] = in ? q[nt][d][i] * scale : 0.0f;
+                top = fmaxf(top, fabsf(q[nt][d][i]));
+            }
+        }
+        top = across_groups_max(top);
+        // 2^e with top * 2^e in [2^10, 2^11); Inf stays as it is
+        const int exponent = static_cast<int>((__float_as_uint(top) >> 23) & 0xff) - 127;
+        const int e = top == 0.0f || exponent == 128 ? 0 : min(10 - exponent, 100);
+        undo[nt] = ldexpf(1.0f, -e);
+#pragma unroll
+        for (int d = 0; d < D32; ++d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = ldexpf(q[nt][d][i], e);
+                const _Float16 high = static_cast<_Float16>(x);
+                qf[nt][d][i] = c < 8 ? high : static_cast<_Float16>(x - static_cast<float>(high));
+            }
+    }
+}
+
+// A step's scores to weights, high and low parts as the second product's columns; the maxima and sums so far move
+// along. there(i): whether the lane's token i counts, asked where `masked`.
+template <int VW, int NT, typename There>
+__device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const float (&undo)[NT], bool masked, There there, int c,
+                                      float (&m)[NT], float (&l)[NT], float4v (&acc)[NT][VW], half8 (&pf)[NT]) {
+    const float low = c < 8 ? 0.0f : -1.0f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float sc[8], sum = 0.0f, top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float part = scores[nt][i / 4][i % 4];
+            sc[i] = (part + other_part(part)) * undo[nt];
+            sum += sc[i];
+        }
+        if (__any(!(fabsf(sum) < INFINITY))) {
+            // infinite keys or queries: the high part's infinity, as F32 products have it
+            // (its low part gives NaN or the other sign)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float part = scores[nt][i / 4][i % 4], other = other_part(part);
+                const float high = c < 8 ? part : other;
+                if (fabsf(high) == INFINITY) sc[i] = high;
+            }
+        }
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sc[i] = there(i) ? sc[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, sc[i]);
+        top = fmaxf(m[nt], across_groups_max(top));
+        if (__any(top > m[nt])) {
+            const float alpha = top > m[nt] ? __builtin_amdgcn_exp2f(m[nt] - top) : 1.0f;   // 0 from no token yet
+            l[nt] *= alpha;
+#pragma unroll
+            for (int j = 0; j < VW; ++j) acc[nt][j] *= alpha;
+            m[nt] = top;
+        }
+        const float shift = kWeightLog2 - (top == -INFINITY ? 0.0f : top);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p = __builtin_amdgcn_exp2f(sc[i] + shift);
+            l[nt] += p;
+            const _Float16 high = static_cast<_Float16>(p);
+            pf[nt][i] = static_cast<_Float16>(fmaf(low, static_cast<float>(high), p));
+        }
+    }
+}
+
+// The second product: value j of a lane's eight tokens, picked out of their rows, times the weights.
+template <int VW, int NT>
+__device__ __forceinline__ void add_values(const uint32_t (&vr)[8][VW / 2], const half8 (&pf)[NT], float4v (&acc)[NT][VW]) {
+#pragma unroll
+    for (int j = 0; j < VW; ++j) {
+        union { uint32_t u[4]; half8 h; } vf;
+        const int word = (j / 8) * 4 + (j % 8) / 2;
+        const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) vf.u[u] = __builtin_amdgcn_perm(vr[2 * u + 1][word], vr[2 * u][word], pick);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            acc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, pf[nt], acc[nt][j], 0, 0, 0);
+    }
+}
+
 // D32: 32-value pieces of a head (width <= 32 * D32; FULL: equal). VW: values a lane loads of a V
 // row (16 lanes: width <= 16 * VW). NT: column tiles (8 query heads each). UNI: page_tokens % 16
 // == 0, so that a half step of 16 tokens lies in one page: its address is scalar, its page id a
@@ -288,17 +387,19 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
             if constexpr (!UNI) at = row_of(token_of(t0, i));
 #pragma unroll
             for (int part = 0; part < VW / VP; ++part) {
+                // a column past the width gives values past it, which are not stored: any part of the row will do (zeros
+                // in its place make the wave wait for the row here: 64 x 1024 tokens x 8 heads of 80 36.4 us, with them 38.4)
                 const int col = part * 128 + c * VP;
                 const bool in = (FULL && 16 * VW == 32 * D32) || col < width;
                 const _Float16 *p = UNI ? v_head + w.at[i / 4] + (i & 3) * a.pool.token_stride + (v_lane + (in ? col : 0))
                                         : v_head + at + (in ? col : 0);
                 if constexpr (VW == 4) {
                     const uint2v x = load_row<uint2v, ONCE>(p);
-                    vr[i][0] = in ? x[0] : 0, vr[i][1] = in ? x[1] : 0;
+                    vr[i][0] = x[0], vr[i][1] = x[1];
                 } else {
                     const uint4v x = load_row<uint4v, ONCE>(p);
-                    vr[i][part * 4] = in ? x[0] : 0, vr[i][part * 4 + 1] = in ? x[1] : 0;
-                    vr[i][part * 4 + 2] = in ? x[2] : 0, vr[i][part * 4 + 3] = in ? x[3] : 0;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) vr[i][part * 4 + u] = x[u];
                 }
             }
         }
@@ -314,37 +415,9 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
     }
     __builtin_amdgcn_sched_barrier(0);
 
-    // q columns: column c is head c % 8 of each tile, its high (c < 8) or low part
-    const float low = c < 8 ? 0.0f : -1.0f;
     half8 qf[NT][D32];
     float undo[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const float scale = nt * 8 + (c & 7) < heads ? a.scale_log2 : 0.0f;
-        float top = 0.0f;
-#pragma unroll
-        for (int d = 0; d < D32; ++d) {
-            const bool in = FULL || d * 32 + G * 8 < width;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[nt][d][i] = in ? q[nt][d][i] * scale : 0.0f;
-                top = fmaxf(top, fabsf(q[nt][d][i]));
-            }
-        }
-        top = across_groups_max(top);
-        // 2^e with top * 2^e in [2^10, 2^11); Inf stays as it is
-        const int exponent = static_cast<int>((__float_as_uint(top) >> 23) & 0xff) - 127;
-        const int e = top == 0.0f || exponent == 128 ? 0 : min(10 - exponent, 100);
-        undo[nt] = ldexpf(1.0f, -e);
-#pragma unroll
-        for (int d = 0; d < D32; ++d)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = ldexpf(q[nt][d][i], e);
-                const _Float16 high = static_cast<_Float16>(x);
-                qf[nt][d][i] = c < 8 ? high : static_cast<_Float16>(x - static_cast<float>(high));
-            }
-    }
+    split_queries<D32, NT, FULL>(a.scale_log2, heads, width, c, G, q, qf, undo);
 
     float4v acc[NT][VW];
     float m[NT], l[NT];
@@ -387,48 +460,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
         __builtin_amdgcn_sched_barrier(0);
 
         half8 pf[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float sc[8], sum = 0.0f, top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float part = scores[nt][i / 4][i % 4];
-                sc[i] = (part + other_part(part)) * undo[nt];
-                sum += sc[i];
-            }
-            if (__any(!(fabsf(sum) < INFINITY))) {
-                // infinite keys or queries: the high part's infinity, as F32 products have it
-                // (its low part gives NaN or the other sign)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float part = scores[nt][i / 4][i % 4], other = other_part(part);
-                    const float high = c < 8 ? part : other;
-                    if (fabsf(high) == INFINITY) sc[i] = high;
-                }
-            }
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sc[i] = there(i) ? sc[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, sc[i]);
-            top = fmaxf(m[nt], across_groups_max(top));
-            if (__any(top > m[nt])) {
-                const float alpha = top > m[nt] ? __builtin_amdgcn_exp2f(m[nt] - top) : 1.0f;   // 0 from no token yet
-                l[nt] *= alpha;
-#pragma unroll
-                for (int j = 0; j < VW; ++j) acc[nt][j] *= alpha;
-                m[nt] = top;
-            }
-            const float shift = kWeightLog2 - (top == -INFINITY ? 0.0f : top);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = __builtin_amdgcn_exp2f(sc[i] + shift);
-                l[nt] += p;
-                const _Float16 high = static_cast<_Float16>(p);
-                pf[nt][i] = static_cast<_Float16>(fmaf(low, static_cast<float>(high), p));
-            }
-        }
+        weigh<VW, NT>(scores, undo, masked, there, c, m, l, acc, pf);
         if (masked) {                                // 0 * NaN would reach the sums
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -437,18 +469,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
                 for (int u = 0; u < VR; ++u) vr[i][u] = ok ? vr[i][u] : 0;
             }
         }
-#pragma unroll
-        for (int j = 0; j < VW; ++j) {
-            union { uint32_t u[4]; half8 h; } vf;
-            const int word = (j / 8) * 4 + (j % 8) / 2;
-            const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                vf.u[u] = __builtin_amdgcn_perm(vr[2 * u + 1][word], vr[2 * u][word], pick);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                acc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, pf[nt], acc[nt][j], 0, 0, 0);
-        }
+        add_values<VW, NT>(vr, pf, acc);
         if (!more) break;
         __builtin_amdgcn_sched_barrier(0);
         load_v(t1, next);
