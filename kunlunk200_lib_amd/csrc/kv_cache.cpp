@@ -150,7 +150,7 @@ bool paged_attention(Kernel & kernel, int id, void * y, const void * q, const vo
     detail::check_hip((hipError_t)kk_paged_attention(y, q, k, v, table, lengths, c, p, room, ctx.status + 1, ctx.cus,
                                                      ctx.stream),
                       "kk_paged_attention");
-    note(impl, id, room ? "paged_attention_split" : "paged_attention");
+    note(impl, id, kk_paged_attention_route(c, p, ctx.cus));
     return true;
 }
 

@@ -150,6 +150,7 @@ int kk_i8_matmul(const void *workspace, const int8_t *w, const float *scales, co
 // sequences split over several workgroups.
 size_t kk_paged_attention_workspace_bytes(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p,
                                           int cus);
+const char *kk_paged_attention_route(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus);
 int kk_paged_attention(void *y, const void *q, const void *k, const void *v, const int *table, const int *lengths,
                        const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, void *workspace,
                        int *status, int cus, hipStream_t stream);

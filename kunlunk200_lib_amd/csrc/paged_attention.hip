@@ -28,10 +28,11 @@
 //
 // What bounds it: reading the cache (4 * width bytes per token and head). A step's K rows
 // are reloaded behind its scores and its V rows behind its second product, so a wave has 8
-// to 16 KiB on their way at any time, three workgroups to a CU; 32 sequences of up to 4096 tokens x 32 heads of
-// 128 (1.2 GB) take 187..196 us, 6.2 TB/s, what a kernel that only reads reaches; one of 32768 tokens x 8 heads
-// 24.5 us (5.5 TB/s) and 4.5 for the join. Below some ten MB it is the chain of latencies (length and pages, rows,
-// two products, the waves' sums): 33 tokens x 32 heads 5.6 us of kernel.
+// to 16 KiB on their way at any time, three workgroups to a CU; one sequence of 32768 tokens x 8 heads takes
+// 24.5 us (5.5 TB/s) and 4.5 for the join. Long ragged rows go to attend_even, below: 32 sequences of up to
+// 4096 tokens x 32 heads of 128 (1.2 GB) 180..185 us, 6.6 TB/s, what a kernel that only reads reaches. Below some
+// ten MB it is the chain of latencies (length and pages, rows, two products, the waves' sums): 33 tokens x 32 heads
+// 5.6 us of kernel.
 //
 // Sequences of more than one chunk leave (sum w v, m, sum w) per chunk in the
 // workspace; a second launch joins them in order, so results do not
@@ -60,6 +61,8 @@ constexpr int kMinChunk = kWaves * kStep;
 constexpr int kMaxChunk = 512, kMaxChunkMany = 1024;
 constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
+constexpr int kRowSteps = 1;             // what beginning a row counts in a share
+constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even goes through
 constexpr float kWeightLog2 = 14.0f;     // weights are scaled by 2^14
 
 struct AttendArgs {
@@ -73,6 +76,10 @@ struct AttendArgs {
     int64_t q_stride, y_stride;
     int query_heads, group, tiles, longest, window, row_pages, chunk, chunks, f16, q_wide;
     float scale_log2;
+    // attend_even: (sequence, four heads) -> where the row's sums stand in the workspace, and of how many workgroups
+    int2 *spans;
+    kk::FastDiv shares;                  // attend_even's workgroups
+    int sequences;
 };
 
 // A word that no lane writes during the launch, read through the scalar cache.
@@ -529,28 +536,331 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
     }
 }
 
+// The steps of a row: from the one that holds its first token on.
+__device__ __forceinline__ int base_of(const AttendArgs &a, int len) {
+    return (a.window > 0 ? max(0, len - a.window) : 0) & ~(kStep - 1);
+}
+__device__ __forceinline__ int steps_of(const AttendArgs &a, int len) { return (len - base_of(a, len) + kStep - 1) / kStep; }
+
+// Sum over the lanes up to this one: within 16 lanes by row shifts, then the rows' last lanes on.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ int add_shifted(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int sum_to_lane(int v) {
+    v = add_shifted<0x111, 0xf>(v);
+    v = add_shifted<0x112, 0xf>(v);
+    v = add_shifted<0x114, 0xf>(v);
+    v = add_shifted<0x118, 0xf>(v);
+    v = add_shifted<0x142, 0xa>(v);
+    return add_shifted<0x143, 0xc>(v);
+}
+
+// The part of one workgroup of attend_even: of all steps in the order (sequence, four heads, step), `left` from `at` on.
+// A row's first kRowSteps steps are empty: what it costs to begin it.
+struct Share {
+    int at, left;
+    int s, four, step;                               // where `at` is
+    int per, extra;                                  // steps of a share; the first `extra` shares have one more
+    __device__ __forceinline__ int holder(int step_number) const {
+        const int cut = extra * (per + 1);
+        return step_number < cut ? step_number / (per + 1) : extra + (step_number - cut) / per;
+    }
+};
+
+__device__ __forceinline__ Share share_of(const AttendArgs &a, int number, int fours, int lane, bool tell) {
+    auto steps = [&](int s) {
+        if (s >= a.sequences) return 0;
+        int len = a.lengths[s];
+        if (len < 0 || len > a.longest) {
+            if (tell) kk::report(a.status, kk::kBadIndex);
+            len = len < 0 ? 0 : a.longest;
+        }
+        const int n = steps_of(a, len);
+        return n ? (n + kRowSteps) * fours : 0;
+    };
+    const int mine = steps(lane), mine_to_lane = sum_to_lane(mine);        // of the first 64 sequences; more are read twice
+    int total = __builtin_amdgcn_readlane(mine_to_lane, kWave - 1);
+    if (a.sequences > kWave) {
+        int more = 0;
+#pragma unroll 4
+        for (int s = lane + kWave; s < a.sequences; s += kWave) more += steps(s);
+        total += __builtin_amdgcn_readlane(sum_to_lane(more), kWave - 1);
+    }
+    Share r;
+    r.per = max(static_cast<int>(a.shares.div(total)), 1);
+    r.extra = max(0, total - r.per * static_cast<int>(a.shares.d));
+    r.at = number * r.per + min(number, r.extra);
+    r.left = max(0, min(r.per + (number < r.extra ? 1 : 0), total - r.at));
+    if (r.left == 0) return r;
+    int before = 0;
+    for (int s0 = 0;; s0 += kWave) {                 // ends: at < total
+        const int own = s0 == 0 ? mine : steps(s0 + lane), sum = s0 == 0 ? mine_to_lane : sum_to_lane(own);
+        if (const uint64_t past = __ballot(before + sum > r.at)) {
+            const int found = __builtin_ctzll(past);
+            const int held = __builtin_amdgcn_readlane(own, found);
+            const int in_row = r.at - before - __builtin_amdgcn_readlane(sum, found) + held, per_four = held / fours;
+            r.s = s0 + found;
+            r.four = in_row / per_four;
+            r.step = in_row - r.four * per_four;
+            return r;
+        }
+        before += __builtin_amdgcn_readlane(sum, kWave - 1);
+    }
+}
+
+// The same sums by one workgroup to a CU (width 64: two), each an equal share of the steps of all rows. Its waves take four
+// neighbouring key-value heads, so that what it reads lies together in either order within a page (64 x 4096 tokens x 8
+// heads, token by token: 200 us by `attend`, 5.4 TB/s; 174 so, 6.2), and a wave's sums are its head's: no barrier, no LDS.
+// Four waves with a step on its way each keep up with the memory (two workgroups to a CU: 172 for 169 with 64 x 4096 head by
+// head; width 64: 92 for 98). A new row costs a chain of latencies - length, page, rows - of some 4 us: the next row is
+// looked up while this one's first rows are on their way, its first rows are asked for behind this one's last scores, and
+// beginning it counts as a step of a share (64 sequences ragged to 2048 x 8 heads: 63 us without all that, 58 with; `attend` 66).
+template <int D32, int VW>
+__global__ __launch_bounds__(kThreads, 1) void attend_even(AttendArgs a) {
+    constexpr int VP = VW < 8 ? VW : 8, VR = VW / 2, width = 32 * D32;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int c = lane & 15, G = lane >> 4;
+    const int fours = a.pool.heads / kWaves, heads = a.group;
+    const Share share = share_of(a, blockIdx.x, fours, lane, blockIdx.x == 0 && wave == 0);
+    if (share.left == 0 || share.step + share.left <= kRowSteps) return;     // (or ends among a row's empty steps)
+
+    // what a share has of one row
+    struct Run {
+        int s, four, step, steps, take;              // the row's steps, and this run's from `step` on, empty ones included
+        int lo, hi, t0;                              // its tokens, and the first of its first step
+        const int *row;
+        const _Float16 *k, *v;
+    };
+    auto run_at = [&](int s, int four, int step, int left) {
+        Run r;
+        const int len = length_of(a, s, false), base = base_of(a, len), kvh = four * kWaves + wave;
+        r.s = s;
+        r.four = four;
+        r.step = step;
+        r.steps = (len - base + kStep - 1) / kStep + kRowSteps;
+        r.take = min(left, r.steps - step);
+        r.t0 = base + max(0, step - kRowSteps) * kStep;
+        r.lo = max(r.t0, a.window > 0 ? len - a.window : 0);
+        r.hi = min(len, base + (step + r.take - kRowSteps) * kStep) - 1;
+        r.row = a.table + (int64_t)s * a.row_pages;
+        r.k = a.k + (int64_t)kvh * a.pool.head_stride;
+        r.v = a.v + (int64_t)kvh * a.pool.head_stride;
+        return r;
+    };
+    auto run_after = [&](const Run &r, int left) {   // left > 0: there is a row with tokens
+        int s = r.s, four = r.four + 1;
+        if (four == fours) {
+            four = 0;
+            do ++s;
+            while (length_of(a, s, false) == 0);
+        }
+        return run_at(s, four, 0, left);
+    };
+
+    half8 kf[2][D32];
+    uint32_t vr[8][VR];
+    struct Halves {
+        int64_t at[2];
+        bool ok[2];
+    };
+    auto find = [&](const Run &r, int t0) {
+        Halves w;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int t = min(max(t0 + half * 16, r.lo & ~15), r.hi & ~15);
+            const int p = a.pool.per_page.div(t);
+            int id = scalar_load(r.row + p);
+            w.ok[half] = static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages);
+            if (!w.ok[half]) {
+                if (lane == 0) kk::report(a.status, kk::kBadPage);
+                id = 0;
+            }
+            w.at[half] = (int64_t)id * a.pool.page_stride + (int64_t)(t - p * a.pool.page_tokens) * a.pool.token_stride;
+        }
+        return w;
+    };
+    const uint32_t k_lane = static_cast<uint32_t>(c * a.pool.token_stride) + G * 8;
+    const uint32_t v_lane = static_cast<uint32_t>(G * 4 * a.pool.token_stride);
+    auto load_k = [&](const _Float16 *k, const Halves &w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int d = 0; d < D32; ++d) kf[half][d] = load_row<half8, true>(k + w.at[half] + (k_lane + d * 32));
+    };
+    auto load_v = [&](const _Float16 *v, const Halves &w) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int part = 0; part < VW / VP; ++part) {
+                const int col = part * 128 + c * VP;
+                const bool in = 16 * VW == width || col < width;
+                const _Float16 *p = v + w.at[i / 4] + (i & 3) * a.pool.token_stride + (v_lane + (in ? col : 0));
+                if constexpr (VW == 4) {
+                    const uint2v x = load_row<uint2v, true>(p);
+                    vr[i][0] = x[0], vr[i][1] = x[1];
+                } else {
+                    const uint4v x = load_row<uint4v, true>(p);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) vr[i][part * 4 + u] = x[u];
+                }
+            }
+    };
+    float q[1][D32][8];
+    auto load_queries = [&](const Run &r) {
+        const int64_t at = r.s * a.q_stride + (int64_t)((r.four * kWaves + wave) * a.group + (c & 7) % heads) * width;
+#pragma unroll
+        for (int d = 0; d < D32; ++d) load_query(a, at + d * 32 + G * 8, q[0][d]);
+    };
+
+    Run now = run_at(share.s, share.four, share.step, share.left);
+    load_queries(now);
+    Halves here = find(now, now.t0);
+    load_k(now.k, here);
+    load_v(now.v, here);
+    __builtin_amdgcn_sched_barrier(0);
+    half8 qf[1][D32];
+    float undo[1], m[1], l[1];
+    float4v acc[1][VW];
+    auto start = [&] {
+        split_queries<D32, 1, true>(a.scale_log2, heads, width, c, G, q, qf, undo);
+        m[0] = -INFINITY;
+        l[0] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VW; ++j) acc[0][j] = float4v{0, 0, 0, 0};
+    };
+    int left = share.left, t0 = now.t0, run_from = share.at;     // run_from: the number of the run's first step
+    // where the next run begins, found while this one's first rows are on their way
+    bool again;
+    Run then;
+    Halves first_of_then;
+    auto look_ahead = [&] {
+        again = left - now.take > kRowSteps;
+        if (again) {
+            then = run_after(now, left - now.take);
+            first_of_then = find(then, then.t0);
+        }
+    };
+    look_ahead();
+    start();
+
+    for (;;) {
+        const bool last = t0 + kStep > now.hi;       // the run's last step
+        const bool more = !last || again;
+        Halves next = first_of_then;
+        if (!last) next = find(now, t0 + kStep);
+        const _Float16 *k_next = last ? then.k : now.k, *v_next = last ? then.v : now.v;
+        const bool masked = t0 < now.lo || t0 + kStep > now.hi + 1 || !(here.ok[0] && here.ok[1]);
+        auto there = [&](int i) {
+            const int t = t0 + (i < 4 ? 0 : 16) + G * 4 + (i & 3);
+            return t >= now.lo && t <= now.hi && here.ok[i / 4];
+        };
+        float4v scores[1][2] = {{float4v{0, 0, 0, 0}, float4v{0, 0, 0, 0}}};
+#pragma unroll
+        for (int d = 0; d < D32; ++d) {
+            scores[0][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][d], qf[0][d], scores[0][0], 0, 0, 0);
+            scores[0][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][d], qf[0][d], scores[0][1], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_k(k_next, next);
+        if (last && more) load_queries(then);
+        __builtin_amdgcn_sched_barrier(0);
+        half8 pf[1];
+        weigh<VW, 1>(scores, undo, masked, there, c, m, l, acc, pf);
+        if (masked) {                                // 0 * NaN would reach the sums
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool ok = there(i);
+#pragma unroll
+                for (int u = 0; u < VR; ++u) vr[i][u] = ok ? vr[i][u] : 0;
+            }
+        }
+        add_values<VW, 1>(vr, pf, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) load_v(v_next, next);
+        __builtin_amdgcn_sched_barrier(0);
+        if (last) {
+            // sums to the output, or to place (workgroup + row): consecutive for the workgroups of one row
+            const int row = now.s * fours + now.four, slot = blockIdx.x + row, head0 = (now.four * kWaves + wave) * a.group;
+            const bool single = now.step <= kRowSteps && now.step + now.take == now.steps;
+            if (now.step <= kRowSteps && tid == 0)
+                a.spans[row] = int2{slot, share.holder(run_from - now.step + now.steps - 1) - static_cast<int>(blockIdx.x) + 1};
+            const float total = across_groups_sum(l[0]);
+            const int64_t at = ((int64_t)slot * kWaves + wave) * a.group + c;
+            const bool mine = c < heads;
+            if (mine && G == 0 && !single) {
+                a.part_ml[at * 2] = m[0];
+                a.part_ml[at * 2 + 1] = total;
+            }
+            // row 4G + r of product j is value VP * (4G + r) + j % 8 of half j / 8
+#pragma unroll
+            for (int j = 0; j < VW; j += 4)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = (j / 8) * 128 + (4 * G + r) * VP + j % 8;
+                    float4v v;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[u] = acc[0][j + u][r] + other_part(acc[0][j + u][r]);
+                    if (!mine || d >= width) continue;
+                    if (single) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            store_output(a, now.s * a.y_stride + (int64_t)(head0 + c) * width + d + u,
+                                         total == 0.0f ? 0.0f : v[u] / total);
+                    } else {
+                        *reinterpret_cast<float4v *>(a.part_o + at * width + d) = v;
+                    }
+                }
+            if (!more) return;
+            run_from += now.take;
+            left -= now.take;
+            now = then;
+            look_ahead();
+            start();
+            t0 = now.t0;
+        } else {
+            t0 += kStep;
+        }
+        here = next;
+    }
+}
+
 // Joins the chunks of one query head: y = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. Weights by
 // one thread per chunk; then groups of threads take the chunks in turn, 4 values
 // each, and the groups' sums are added in order.
 constexpr int kJoinRun = 1024;                       // chunks whose weights wait in LDS at a time
-template <int THREADS>
+template <int THREADS, bool EVEN>
 __global__ __launch_bounds__(THREADS) void join_chunks(AttendArgs a) {
     __shared__ float weights[kJoinRun];
     __shared__ float4v sums[THREADS];
     __shared__ float reduce[THREADS / kWave];
     const int h = blockIdx.x, s = blockIdx.y, width = a.pool.width, tid = threadIdx.x;
     const int len = length_of(a, s, false);
-    const int base = (a.window > 0 ? max(0, len - a.window) : 0) & ~(kStep - 1);
-    if (len - base <= a.chunk) return;               // written by its one chunk
-    const int n = (len - base + a.chunk - 1) / a.chunk;
-    const int64_t at = ((int64_t)s * a.query_heads + h) * a.chunks;
+    int n, step;                                     // chunks, and how many places they are apart
+    int64_t at;
+    if constexpr (EVEN) {
+        const int kvh = h / a.group;
+        const int2 span = a.spans[s * (a.pool.heads / kWaves) + kvh / kWaves];
+        if (len == 0) {                              // no tokens: zeros
+            for (int i = tid; i < width; i += THREADS) store_output(a, s * a.y_stride + (int64_t)h * width + i, 0.0f);
+            return;
+        }
+        n = span.y;
+        step = kWaves * a.group;
+        at = (int64_t)span.x * step + kvh % kWaves * a.group + h - kvh * a.group;
+    } else {
+        n = (len - base_of(a, len) + a.chunk - 1) / a.chunk;
+        step = 1;
+        at = ((int64_t)s * a.query_heads + h) * a.chunks;
+    }
+    if (n <= 1) return;                              // written by its one chunk
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + at;
     const float4v *o = reinterpret_cast<const float4v *>(a.part_o + at * width);
     const int vectors = width / 4, groups = THREADS / vectors;
     const int group = tid / vectors, at4 = tid - group * vectors;
 
     float top = -INFINITY;
-    for (int i = tid; i < n; i += THREADS) top = fmaxf(top, ml[i].x);
+    for (int i = tid; i < n; i += THREADS) top = fmaxf(top, ml[(int64_t)i * step].x);
     top = kk::wave_max(top);
     if (tid % kWave == 0) reduce[tid / kWave] = top;
     __syncthreads();
@@ -563,7 +873,7 @@ __global__ __launch_bounds__(THREADS) void join_chunks(AttendArgs a) {
     for (int i0 = 0; i0 < n; i0 += kJoinRun) {
         const int run = min(kJoinRun, n - i0);
         for (int i = tid; i < run; i += THREADS) {
-            const float2 x = ml[i0 + i];
+            const float2 x = ml[(int64_t)(i0 + i) * step];
             const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - top);
             weights[i] = w;
             total += w * x.y;
@@ -574,7 +884,7 @@ __global__ __launch_bounds__(THREADS) void join_chunks(AttendArgs a) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const int i = j0 + u * groups;
-                v[u] = group < groups && i < run ? o[(int64_t)(i0 + i) * vectors + at4] : float4v{0, 0, 0, 0};
+                v[u] = group < groups && i < run ? o[(int64_t)(i0 + i) * step * vectors + at4] : float4v{0, 0, 0, 0};
             }
             if (j0 == group) __syncthreads();
 #pragma unroll
@@ -606,6 +916,7 @@ bool in_halves(const kunlun::KVCacheLayout &c) { return c.page_tokens % 16 == 0 
 struct Plan {
     int group, nt, tiles, chunk, chunks;
     bool halves, once, wide, narrow;
+    int shares;                                      // attend_even: workgroups, else 0
 };
 
 Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus) {
@@ -624,6 +935,7 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
              longest <= (rows > cus / 2 ? 2 * whole : whole);
     const int64_t least = r.wide ? longest : rows > cus && longest <= whole ? longest : kMinChunk;
+    // (The figures of parts of rows that attend_even takes now, below, are `attend`'s.)
     // Otherwise two workgroups' tokens to a CU, in parts of one size: of up to 512 tokens (1 x 32768 tokens x 8 heads
     // 29.1 us, of 256 32.0); with two rows and more to a CU whole rows of up to 1024 (64 x 640 / 1024 tokens x 8 heads
     // 30 / 46, in parts of 512 40 / 54) and, above, at least three parts of up to 1024 (64 x 8 heads ragged to 2048: two
@@ -648,10 +960,21 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     // heads 61 / 35)
     r.narrow = r.nt == 1 && rows > 2 * cus && longest <= 4 * kStep;
     // The non-temporal hint, for reads of whole cache lines that fill more than a quarter of the 256 MiB cache with
-    // nothing that is read again (us, with the hint and without: 32 x 4096 tokens x 32 heads 196 / 218; 64 x 4096 x 8 in
+    // nothing that is read again (us by `attend`, with the hint and without: 32 x 4096 tokens x 32 heads 196 / 218; 64 x 4096 x 8 in
     // token order 198 / 207; 64 x 1024 x 8 of 64 25.4 / 28.3; 16 x 1024 x 8, 67 MB, 20.1 / 18.9; tiles that read the same
     // rows, 32 query heads on one, 107 / 96; rows that share lines, 64 x 1024 x 8 of 80, 40.5 / 38.4).
     r.once = r.tiles == 1 && (int64_t)p.sequences * longest * c.heads * c.width * 4 > (64 << 20);
+    // Equal shares where rows would be split and there is enough to read (us, by `attend` and in shares, 8 heads of 128, head by
+    // head / token by token: 64 sequences uniform to 1536 48 and 45 / 53 and 45, to 4096 110 and 97 / 121 and 99; 16 to
+    // 2048 25.4 and 20.9 / 27.8 and 21.3, all 2048 29.9 and 32.0 / 32.7 and 31.9; width 256, 16 to 16384 201 and 157; 1 x
+    // 131072 98 and 92). Rows that one workgroup takes whole stay with it (64 x 1024 46.9 and 52.4; uniform to 1024 34.9 and
+    // 36.3), and so does one sequence, which is even by itself, until the last round of its parts counts little (1 x 32768
+    // 30.5 and 31.8). Where `longest` is ten times the lengths the shares lose 2 to 5 us (64 to 153 of 1536: 12.7 and 17.3).
+    r.shares = 0;
+    if (r.chunks > 1 && r.halves && r.once && r.nt == 1 && c.heads % kWaves == 0 && (c.width % 64 == 0 || c.width == 96) &&
+        p.sequences <= kMostEven && (p.sequences > 1 || (int64_t)longest * c.heads * c.width * 4 > (256 << 20)) &&
+        (int64_t)p.sequences * c.heads * (longest / kStep + 3) < INT32_MAX)
+        r.shares = c.width <= 64 ? 2 * cus : cus;
     return r;
 }
 
@@ -669,6 +992,12 @@ template <int D32, int VW, int NT, int WAVES>
 hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     if (!p.halves) return launch<D32, VW, NT, false, false, false, WAVES>(a, p, sequences, heads, stream);
     if (a.pool.width != 32 * D32) return launch<D32, VW, NT, true, false, false, WAVES>(a, p, sequences, heads, stream);
+    if constexpr (WAVES == kWaves && NT == 1) {
+        if (p.shares) {
+            hipLaunchKernelGGL((attend_even<D32, VW>), dim3(p.shares), dim3(kThreads), 0, stream, a);
+            return hipGetLastError();
+        }
+    }
     if constexpr (WAVES == kWaves) {
         if (p.once) return launch<D32, VW, NT, true, true, true, WAVES>(a, p, sequences, heads, stream);
     }
@@ -685,12 +1014,25 @@ hipError_t launch_width(const AttendArgs &a, const Plan &p, int sequences, int h
     return launch_tiles<D32, VW, 1, kWaves>(a, p, sequences, heads, stream);
 }
 
+// Places of attend_even's sums: every workgroup begins one and every row, for each of its four heads' query heads.
+size_t even_parts(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, const Plan &r) {
+    return ((size_t)p.sequences * (c.heads / kWaves) + r.shares) * kWaves * r.group;
+}
+
 } // namespace
 
 extern "C" size_t kk_paged_attention_workspace_bytes(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p,
                                           int cus) {
     const Plan r = plan_of(c, p, cus);
+    if (r.shares)
+        return even_parts(c, p, r) * (c.width + 2) * sizeof(float) + (size_t)p.sequences * (c.heads / kWaves) * sizeof(int2);
     return r.chunks == 1 ? 0 : (size_t)p.sequences * p.query_heads * r.chunks * (c.width + 2) * sizeof(float);
+}
+
+extern "C" const char *kk_paged_attention_route(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p,
+                                                int cus) {
+    const Plan r = plan_of(c, p, cus);
+    return r.shares ? "paged_attention_even" : r.chunks > 1 ? "paged_attention_split" : "paged_attention";
 }
 
 extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const void *v, const int *table, const int *lengths,
@@ -698,7 +1040,7 @@ extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const v
                        int *status, int cus, hipStream_t stream) {
     const Plan r = plan_of(c, p, cus);
     if (c.width <= 0 || c.width > 256 || c.width % 8 || p.sequences > 65535 || r.chunks > kMostChunks ||
-        (r.chunks > 1 && !workspace))
+        ((r.chunks > 1 || r.shares) && !workspace))
         return hipErrorInvalidValue;
     AttendArgs a;
     a.k = static_cast<const _Float16 *>(k);
@@ -708,7 +1050,11 @@ extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const v
     a.q = q;
     a.y = y;
     a.part_o = static_cast<float *>(workspace);
-    a.part_ml = a.part_o + (size_t)p.sequences * p.query_heads * r.chunks * c.width;
+    const size_t parts = r.shares ? even_parts(c, p, r) : (size_t)p.sequences * p.query_heads * r.chunks;
+    a.part_ml = a.part_o + parts * c.width;
+    a.spans = reinterpret_cast<int2 *>(a.part_ml + parts * 2);
+    a.shares = kk::FastDiv(std::max(r.shares, 1));
+    a.sequences = p.sequences;
     a.status = status;
     a.pool = PoolView(c);
     a.q_stride = p.q_stride;
@@ -730,9 +1076,13 @@ extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const v
     else if (c.width <= 128) rc = launch_width<4, 8>(a, r, p.sequences, c.heads, stream);
     else if (c.width <= 192) rc = launch_width<6, 16>(a, r, p.sequences, c.heads, stream);
     else rc = launch_width<8, 16>(a, r, p.sequences, c.heads, stream);
-    if (rc != hipSuccess || r.chunks == 1) return rc;
+    if (rc != hipSuccess || (r.chunks == 1 && !r.shares)) return rc;
     // one wave where there is little to join
-    if (r.chunks <= 4) hipLaunchKernelGGL(join_chunks<kWave>, dim3(p.query_heads, p.sequences), dim3(kWave), 0, stream, a);
-    else hipLaunchKernelGGL(join_chunks<kThreads>, dim3(p.query_heads, p.sequences), dim3(kThreads), 0, stream, a);
+    const bool little = r.shares ? r.shares <= 4 * (int64_t)p.sequences * (c.heads / kWaves) : r.chunks <= 4;
+    const dim3 grid(p.query_heads, p.sequences);
+    if (r.shares && little) hipLaunchKernelGGL((join_chunks<kWave, true>), grid, dim3(kWave), 0, stream, a);
+    else if (r.shares) hipLaunchKernelGGL((join_chunks<kThreads, true>), grid, dim3(kThreads), 0, stream, a);
+    else if (little) hipLaunchKernelGGL((join_chunks<kWave, false>), grid, dim3(kWave), 0, stream, a);
+    else hipLaunchKernelGGL((join_chunks<kThreads, false>), grid, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }

@@ -900,3 +900,79 @@ def test_attention_many_rows(gpu):
         assert route == "paged_attention"
         gold, tol = gold_attention(cache, table, lengths, q, 0, width ** -0.5)
         check(y, gold, tol)
+
+
+# lengths, heads, query heads, width, tokens of a page, window, F16, order, `longest`
+EVEN = [
+    ([0, 1, 33, 0, 0, 700, 32, 31, 2500, 64, 5, 0], 4, 4, 128, 16, 0, False, "heads", 2816),
+    ([0] * 12, 4, 8, 128, 16, 0, False, "heads", 2816),
+    ([1] * 12, 4, 8, 128, 16, 0, True, "tokens", 2816),
+    ([2816, 1, 1, 2815, 16, 17, 129, 0], 8, 32, 128, 32, 0, True, "tokens", 2816),
+    ([40, 41, 1500, 3, 1301, 999, 0, 7, 8, 9, 10, 11] * 2, 4, 28, 64, 48, 0, False, "tokens", 2816),
+    ([300, 2100, 33, 70], 8, 8, 256, 16, 0, False, "heads", 2560),
+    ([7000, 5033, 10, 4999], 4, 16, 256, 16, 5000, True, "tokens", 7008),
+    ([4000, 1501, 1500, 1499, 0, 20, 3000, 2000], 8, 24, 192, 32, 1500, False, "heads", 4000),
+    ([1800, 90, 0, 1, 640, 33, 34, 35], 12, 12, 96, 16, 0, True, "tokens", 2000),
+    ([3000], 4, 32, 256, 64, 0, False, "tokens", 66048),
+    ([i * 37 % 61 for i in range(130)], 4, 8, 64, 16, 0, False, "heads", 1104),
+    ([i * 53 % 101 if i > 99 else 0 for i in range(200)], 4, 4, 128, 16, 0, False, "tokens", 1104),
+]
+
+
+@pytest.mark.parametrize("case", range(len(EVEN)))
+def test_attention_even(gpu, case):
+    """Equal shares of all sequences' tokens: parts that begin and end anywhere, in rows of any length and of none."""
+    lengths, heads, query_heads, width, page_tokens, window, half, order, longest = EVEN[case]
+    rng = np.random.default_rng(1500 + case)
+    row_pages = -(-longest // page_tokens)
+    pages = sum(-(-n // page_tokens) for n in lengths) + 2
+    cache = Cache(rng, pages, page_tokens, heads, width, order, case % 2)
+    table = table_of(rng, lengths, page_tokens, pages, row_pages, rest=2 ** 30)
+    q = (rng.standard_normal((len(lengths), query_heads, width)) * 2).astype(np.float16 if half else np.float32)
+    owned = np.zeros((pages, page_tokens), bool)
+    for s, n in enumerate(lengths):
+        t = np.arange(n)
+        owned[table[s, t // page_tokens], t % page_tokens] = True
+    for pool in (cache.k, cache.v):
+        pool[0].transpose(0, 2, 1, 3)[~owned] = np.nan
+    y, route = run_attention(cache, table, lengths, q, window, longest=longest, pad=3)
+    assert route == "paged_attention_even"
+    gold, tol = gold_attention(cache, table, lengths, q, window, width ** -0.5)
+    check(y, gold, tol)
+    again, _ = run_attention(cache, table, lengths, q, window, longest=longest, pad=3)
+    assert np.array_equal(y, again), "the same call gives other bits"
+    assert gpu.kv_cache_status(0) == 0
+
+
+def test_attention_even_reports(gpu):
+    """Bad pages and lengths among even shares; what is not a number stays in its sequence and heads."""
+    rng = np.random.default_rng(71)
+    lengths = [500, 40, 0, 900, 33, 1, 320, 1200]
+    cache = Cache(rng, 260, 16, 8, 128)
+    table = table_of(rng, lengths, 16, 260, 176)
+    q = rng.standard_normal((8, 8, 128)).astype(np.float32)
+    gold, tol = gold_attention(cache, table, lengths, q, 0, 128 ** -0.5)
+    bad = table.copy()
+    bad[0, 3], bad[3, 20], bad[4, 0] = 260, -1, 2 ** 31 - 1
+    y, route = run_attention(cache, bad, lengths, q, longest=2816)
+    assert route == "paged_attention_even"
+    assert gpu.kv_cache_status(0) == kl.KV_BAD_PAGE
+    safe = bad.copy()
+    safe[0, 3] = safe[4, 0] = -1
+    check(y, *gold_attention(cache, safe, lengths, q, 0, 128 ** -0.5, skip=(-1,)))
+    wrong = [500, 40, -5, 900, 33, 1, 320, 2 ** 30]
+    table[7] = np.resize(table[7, :75], 176)
+    y, _ = run_attention(cache, table, wrong, q, longest=2816)
+    assert gpu.kv_cache_status(0) == kl.KV_BAD_INDEX
+    check(y[:7], gold[:7], tol[:7])
+    gold_cut, tol_cut = gold_attention(cache, table, [0] * 7 + [2816], q, 0, 128 ** -0.5)
+    check(y[7], gold_cut[7], tol_cut[7])
+    cache.k[0, table[3, 30], 5, 2, 9] = np.nan
+    cache.v[0, table[6, 1], 2, 2, 9] = np.inf
+    q[1, 6, 77] = np.nan
+    y, _ = run_attention(cache, table, lengths, q, longest=2816)
+    odd = np.zeros(y.shape, bool)
+    odd[3, 5] = odd[1, 6] = odd[6, 2, 9] = True
+    assert np.array_equal(~np.isfinite(y), odd)
+    gold, tol = gold_attention(cache, table, lengths, q, 0, 128 ** -0.5)
+    check(np.where(odd, 0, y), np.where(odd, 0, gold), np.where(odd, 0, tol))
