@@ -992,12 +992,6 @@ template <int D32, int VW, int NT, int WAVES>
 hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     if (!p.halves) return launch<D32, VW, NT, false, false, false, WAVES>(a, p, sequences, heads, stream);
     if (a.pool.width != 32 * D32) return launch<D32, VW, NT, true, false, false, WAVES>(a, p, sequences, heads, stream);
-    if constexpr (WAVES == kWaves && NT == 1) {
-        if (p.shares) {
-            hipLaunchKernelGGL((attend_even<D32, VW>), dim3(p.shares), dim3(kThreads), 0, stream, a);
-            return hipGetLastError();
-        }
-    }
     if constexpr (WAVES == kWaves) {
         if (p.once) return launch<D32, VW, NT, true, true, true, WAVES>(a, p, sequences, heads, stream);
     }
@@ -1006,6 +1000,11 @@ hipError_t launch_tiles(const AttendArgs &a, const Plan &p, int sequences, int h
 
 template <int D32, int VW>
 hipError_t launch_width(const AttendArgs &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
+    if (p.shares) {                                  // before any other choice: the join reads what only this kernel writes
+        if (a.pool.width != 32 * D32 || !p.halves || p.nt != 1) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((attend_even<D32, VW>), dim3(p.shares), dim3(kThreads), 0, stream, a);
+        return hipGetLastError();
+    }
     if (p.narrow) return launch_tiles<D32, VW, 1, 1>(a, p, sequences, heads, stream);
     if constexpr (VW <= 8) {
         if (p.nt == 2) return launch_tiles<D32, VW, 2, kWaves>(a, p, sequences, heads, stream);
