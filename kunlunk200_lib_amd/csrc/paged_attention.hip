@@ -967,12 +967,18 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     // Equal shares where rows would be split and there is enough to read (us, by `attend` and in shares, 8 heads of 128, head by
     // head / token by token: 64 sequences uniform to 1536 48 and 45 / 53 and 45, to 4096 110 and 97 / 121 and 99; 16 to
     // 2048 25.4 and 20.9 / 27.8 and 21.3, all 2048 29.9 and 32.0 / 32.7 and 31.9; width 256, 16 to 16384 201 and 157; 1 x
-    // 131072 98 and 92). Rows that one workgroup takes whole stay with it (64 x 1024 46.9 and 52.4; uniform to 1024 34.9 and
-    // 36.3), and so does one sequence, which is even by itself, until the last round of its parts counts little (1 x 32768
+    // 131072 98 and 92). One sequence is even by itself, until the last round of its parts counts little (1 x 32768
     // 30.5 and 31.8). Where `longest` is ten times the lengths the shares lose 2 to 5 us (64 to 153 of 1536: 12.7 and 17.3).
+    // Rows that one workgroup takes whole stay with it (64 x 1024 47 and 52, uniform to 1024 35 and 37), unless they lie
+    // token by token (256 x 1024 190 and 177, uniform 119 and 109; to 768 even) or few workgroups fit on a CU (width
+    // 256, 64 uniform to 768 / 2048 55 and 49 / 129 and 103; width 192 44 and 43 / 105 and 87, all 2048 138 and 141; 256
+    // uniform to 512 99 and 102).
+    const bool together = c.head_stride < c.token_stride;
+    const bool share_whole = !r.wide && (c.width > 128 ? longest > kMaxChunk : together && longest > 6 * kMinChunk);
     r.shares = 0;
-    if (r.chunks > 1 && r.halves && r.once && r.nt == 1 && c.heads % kWaves == 0 && (c.width % 64 == 0 || c.width == 96) &&
-        p.sequences <= kMostEven && (p.sequences > 1 || (int64_t)longest * c.heads * c.width * 4 > (256 << 20)) &&
+    if ((r.chunks > 1 || share_whole) && r.halves && r.once && r.nt == 1 && c.heads % kWaves == 0 &&
+        (c.width % 64 == 0 || c.width == 96) && p.sequences <= kMostEven &&
+        (p.sequences > 1 || (int64_t)longest * c.heads * c.width * 4 > (256 << 20)) &&
         (int64_t)p.sequences * c.heads * (longest / kStep + 3) < INT32_MAX)
         r.shares = c.width <= 64 ? 2 * cus : cus;
     return r;

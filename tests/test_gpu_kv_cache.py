@@ -916,6 +916,8 @@ EVEN = [
     ([3000], 4, 32, 256, 64, 0, False, "tokens", 66048),
     ([i * 37 % 61 for i in range(130)], 4, 8, 64, 16, 0, False, "heads", 1104),
     ([i * 53 % 101 if i > 99 else 0 for i in range(200)], 4, 4, 128, 16, 0, False, "tokens", 1104),
+    ([i * 71 % 601 for i in range(40)], 4, 8, 256, 16, 0, False, "heads", 608),
+    ([i * 71 % 901 for i in range(70)], 8, 8, 64, 32, 0, True, "tokens", 928),
 ]
 
 
@@ -942,6 +944,31 @@ def test_attention_even(gpu, case):
     again, _ = run_attention(cache, table, lengths, q, window, longest=longest, pad=3)
     assert np.array_equal(y, again), "the same call gives other bits"
     assert gpu.kv_cache_status(0) == 0
+
+
+@pytest.mark.parametrize("sequences,heads,width,page_tokens,order,longest", [
+    (1000, 8, 256, 32, "heads", 64),            # one wave a workgroup
+    (1000, 4, 128, 16, "tokens", 128),
+    (32, 8, 128, 16, "tokens", 1024),           # eight waves
+    (600, 4, 256, 16, "heads", 512),            # whole rows
+    (64, 8, 160, 16, "tokens", 2048),           # a width between
+    (64, 6, 128, 16, "tokens", 2048),           # heads that are not fours
+    (64, 8, 128, 24, "heads", 2048),            # pages that are not whole half steps
+    (1100, 4, 128, 16, "heads", 1040),          # more sequences than are shared out
+])
+def test_attention_not_even(gpu, sequences, heads, width, page_tokens, order, longest):
+    """Large calls beside those that are shared out."""
+    rng = np.random.default_rng(72)
+    lengths = [int(n) for n in rng.integers(0, 40, sequences)]
+    lengths[sequences // 3] = longest
+    pages = sum(-(-n // page_tokens) for n in lengths) + 1
+    cache = Cache(rng, pages, page_tokens, heads, width, order)
+    table = table_of(rng, lengths, page_tokens, pages, -(-longest // page_tokens), rest=-7)
+    q = rng.standard_normal((sequences, heads, width)).astype(np.float32)
+    y, route = run_attention(cache, table, lengths, q, longest=longest)
+    assert route != "paged_attention_even"
+    gold, tol = gold_attention(cache, table, lengths, q, 0, width ** -0.5)
+    check(y, gold, tol)
 
 
 def test_attention_even_reports(gpu):
