@@ -116,6 +116,11 @@ __device__ __forceinline__ float across_groups_sum(float v) {
 }
 // The value of the lane eight columns on (row_ror:8): a column's other part.
 __device__ __forceinline__ float other_part(float v) { return kk::dpp_move<0x128>(v); }
+// Both parts' sum, in the high part's lanes; where that is infinite (infinite values), the low part has NaN or the other sign.
+__device__ __forceinline__ float both_parts(float high) {
+    const float low = other_part(high);
+    return fabsf(high) == INFINITY ? high : high + low;
+}
 
 // Eight values of a row of q (16-byte loads where a.q_wide allows).
 __device__ __forceinline__ void load_query(const AttendArgs &a, int64_t at, float (&v)[8]) {
@@ -504,7 +509,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
             for (int j = 0; j < VW; j += 4) {
                 float4v v;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = acc[nt][j + u][r] + other_part(acc[nt][j + u][r]);
+                for (int u = 0; u < 4; ++u) v[u] = both_parts(acc[nt][j + u][r]);
                 if (mine)
                     *reinterpret_cast<float4v *>(wave_o + (wave * heads + h) * DPad + (j / 8) * 128 + (4 * G + r) * VP +
                                                  j % 8) = v;
@@ -800,7 +805,7 @@ __global__ __launch_bounds__(kThreads, 1) void attend_even(AttendArgs a) {
                     const int d = (j / 8) * 128 + (4 * G + r) * VP + j % 8;
                     float4v v;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) v[u] = acc[0][j + u][r] + other_part(acc[0][j + u][r]);
+                    for (int u = 0; u < 4; ++u) v[u] = both_parts(acc[0][j + u][r]);
                     if (!mine || d >= width) continue;
                     if (single) {
 #pragma unroll

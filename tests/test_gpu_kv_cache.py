@@ -243,6 +243,26 @@ def test_attention_infinite_keys(gpu, half):
     check(y, gold, tol)
 
 
+@pytest.mark.parametrize("width,longest", [(64, 150), (128, 2816)])
+def test_attention_infinite_values(gpu, width, longest):
+    """An infinite value gives its infinity to the output's column, two of both signs what is not a number."""
+    rng = np.random.default_rng(11)
+    lengths = [150, 40, 1, 0, 70, 33, 1, 2]
+    cache = Cache(rng, 30, 16, 8, width)
+    table = table_of(rng, lengths, 16, 30, 176)
+    q = rng.standard_normal((8, 8, width)).astype(np.float32)
+    for t, d, x in ((0, 3, np.inf), (77, 4, -np.inf), (5, 5, np.inf), (149, 5, -np.inf)):
+        cache.v[0, table[0, t // 16], 1, t % 16, d] = x
+    cache.v[0, table[2, 0], 6, 0, 9] = -np.inf
+    y, _ = run_attention(cache, table, lengths, q, longest=longest)
+    with np.errstate(invalid="ignore"):
+        gold, tol = gold_attention(cache, table, lengths, q, 0, width ** -0.5)
+    assert gold[0, 1, 3] == np.inf and gold[0, 1, 4] == -np.inf and np.isnan(gold[0, 1, 5]) and gold[2, 6, 9] == -np.inf
+    odd = ~np.isfinite(gold)
+    assert np.array_equal(y[odd], gold[odd].astype(np.float32), equal_nan=True)
+    check(np.where(odd, 0, y), np.where(odd, 0, gold), np.where(odd, 0, tol))
+
+
 def test_attention_not_a_number(gpu):
     """NaN among the keys or the query reaches the heads that read it and no others."""
     rng = np.random.default_rng(8)
