@@ -263,7 +263,7 @@ bool kv_reserve(Kernel & kernel, int id, int * table, int * lengths, int * refer
     Kernel::Impl & impl = *kernel.impl_;
     if (!usable(impl, id)) return false;
     detail::DeviceContext & ctx = detail::context(id);
-    void * room = workspace(impl, id, ctx, kk_kv_reserve_workspace_bytes(c, count));
+    void * room = workspace(impl, id, ctx, kk_kv_reserve_workspace_bytes(c, p, count));
     if (!room) return false;
     detail::check_hip((hipError_t)kk_kv_reserve(table, lengths, references, rows, added, count, c, p, room,
                                                 ctx.status + 1, ctx.stream),

@@ -12,6 +12,7 @@
 #include "paged.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace {
 
@@ -125,24 +126,53 @@ __device__ __forceinline__ void release_row(const PagesArgs &a, const int *row, 
     }
 }
 
+// Which entry of a list counts for the sequence it names: the first of those that claim it. Claims stand in LDS
+// where the table has few sequences, else in the workspace.
+constexpr int kNearClaims = 4096;
+
+__device__ __forceinline__ int *cleared_claims(int *near, int *far, int sequences, const int *list, int count) {
+    if (sequences <= kNearClaims) {
+        for (int s = threadIdx.x; s < sequences; s += kPlanThreads) near[s] = INT_MAX;
+    } else {
+        for (int i = threadIdx.x; i < count; i += kPlanThreads)
+            if (static_cast<unsigned>(list[i]) < static_cast<unsigned>(sequences)) far[list[i]] = INT_MAX;
+    }
+    __syncthreads();
+    return sequences <= kNearClaims ? near : far;
+}
+__device__ __forceinline__ void claim(int *claims, int s, int i) { atomicMin(&claims[s], i); }
+// After a barrier; past the vector cache, which may hold the word from before the claims.
+__device__ __forceinline__ bool claimed(const int *claims, int s, int i) {
+    return __hip_atomic_load(&claims[s], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == i;
+}
+
 // ---- kv_reserve ----------------------------------------------------------------------------
 
 __global__ __launch_bounds__(kPlanThreads) void reserve(PagesArgs a, const int *rows, const int *added, int count,
-                                                        int *need_of, int *first_of, int *length_was, int *held_of,
-                                                        int *found) {
-    __shared__ int scratch[kPlanWaves];
+                                                        int *need_of, int *first_of, int *end_of, int *found,
+                                                        int *far_claims) {
+    __shared__ int scratch[kPlanWaves], near_claims[kNearClaims];
     __shared__ long long sums[kPlanWaves];
+    int *claims = cleared_claims(near_claims, far_claims, a.sequences, rows, count);
     int64_t wanted = 0;
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
         const int i = i0 + threadIdx.x;
         int need = -1;                           // -1: left out
         if (i < count && sequence_ok(a, rows[i])) {
-            length_was[i] = a.lengths[rows[i]];
-            const int64_t len = length_in_row(a, length_was[i]), more = added[i];
-            if (more >= 0 && len + more <= (int64_t)a.row_pages * a.pool.page_tokens)
-                need = pages_of(a, static_cast<int>(len + more)) - pages_of(a, static_cast<int>(len));
-            else
+            const int64_t len = length_of(a, rows[i]), more = added[i];
+            if (more >= 0 && len + more <= (int64_t)a.row_pages * a.pool.page_tokens) {
+                end_of[i] = static_cast<int>(len + more);
+                need = pages_of(a, end_of[i]) - pages_of(a, static_cast<int>(len));
+                claim(claims, rows[i], i);
+            } else {
                 kk::report(a.status, kk::kBadIndex);
+            }
+        }
+        __syncthreads();
+        // a claim of this step never takes a sequence from an earlier one: entries come in order
+        if (need >= 0 && !claimed(claims, rows[i], i)) {
+            kk::report(a.status, kk::kBadIndex);
+            need = -1;
         }
         long long total;
         const int64_t at = wanted + prefix<long long>(max(need, 0), total, sums);
@@ -159,21 +189,19 @@ __global__ __launch_bounds__(kPlanThreads) void reserve(PagesArgs a, const int *
     for (int i = threadIdx.x; i < count; i += kPlanThreads) {
         const int need = need_of[i];
         if (need < 0) continue;
-        const int was = length_was[i], len = length_in_row(a, was);
-        int bad = 0;
-        if (need > 0 && (int64_t)first_of[i] + need > have) bad = kk::kNoPage;
-        // of two entries that name one sequence only one finds its length; the other would end past the row
-        else if (atomicCAS(&a.lengths[rows[i]], was, len + added[i]) != was) bad = kk::kBadIndex;
-        if (bad) kk::report(a.status, bad);
-        need_of[i] = bad ? 0 : need;
-        held_of[i] = pages_of(a, len);
+        if (need > 0 && (int64_t)first_of[i] + need > have) {
+            kk::report(a.status, kk::kNoPage);
+            need_of[i] = 0;
+            continue;
+        }
+        a.lengths[rows[i]] = end_of[i];
     }
     __syncthreads();
     // a wave for each listed sequence
     for (int i = threadIdx.x / kWave; i < count; i += kPlanWaves) {
         const int need = need_of[i], first = first_of[i];
         if (need <= 0) continue;
-        int *row = a.table + (int64_t)rows[i] * a.row_pages + held_of[i];
+        int *row = a.table + (int64_t)rows[i] * a.row_pages + pages_of(a, end_of[i]) - need;
         for (int j = threadIdx.x % kWave; j < need; j += kWave) {
             const int page = found[first + j];
             row[j] = page;
@@ -501,16 +529,16 @@ int parts_of(const kunlun::KVCacheLayout &c) {
 
 } // namespace
 
-extern "C" size_t kk_kv_reserve_workspace_bytes(const kunlun::KVCacheLayout &c, int count) {
-    return ((size_t)4 * count + c.pages) * sizeof(int);
+extern "C" size_t kk_kv_reserve_workspace_bytes(const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, int count) {
+    return ((size_t)3 * count + c.pages + (p.sequences > kNearClaims ? p.sequences : 0)) * sizeof(int);
 }
 extern "C" int kk_kv_reserve(int *table, int *lengths, int *references, const int *rows, const int *added, int count,
                   const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
                   hipStream_t stream) {
-    int *need = static_cast<int *>(workspace);
+    int *need = static_cast<int *>(workspace), *found = need + 3 * (size_t)count;
     hipLaunchKernelGGL(reserve, dim3(1), dim3(kPlanThreads), 0, stream,
                        args_of(nullptr, nullptr, table, lengths, references, c, p, status), rows, added, count, need,
-                       need + count, need + 2 * (size_t)count, need + 3 * (size_t)count, need + 4 * (size_t)count);
+                       need + count, need + 2 * (size_t)count, found, found + c.pages);
     return hipGetLastError();
 }
 

@@ -163,7 +163,7 @@ int kk_kv_append(void *k_pool, void *v_pool, void *q_out, const void *q, const v
 
 // Pages taken, shared, given back, moved and copied (k200.h), each with the
 // bytes of workspace it needs.
-size_t kk_kv_reserve_workspace_bytes(const kunlun::KVCacheLayout &c, int count);
+size_t kk_kv_reserve_workspace_bytes(const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, int count);
 int kk_kv_reserve(int *table, int *lengths, int *references, const int *rows, const int *added, int count,
                   const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
                   hipStream_t stream);

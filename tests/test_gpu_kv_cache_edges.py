@@ -1,0 +1,72 @@
+"""The paged cache's and the logits step's contracts where lists, weights and infinities go to their ends:
+entries that are refused or named twice, tokens of very small weight, what is left out."""
+import numpy as np
+import pytest
+
+import kunlunk200_lib_amd as kl
+from test_gpu_kv_cache import Book, lists, upload
+
+pytestmark = pytest.mark.gpu
+
+
+# --- kv_reserve and kv_fork: lists ----------------------------------------------------------
+
+def reserve_rule(book, rows, added):
+    """In list order: an entry out of range is left out, of those that name one sequence the first counts, and
+    one that counts is granted if its pages are there. Returns the status."""
+    status, seen = 0, set()
+    free = list(np.flatnonzero(book.references == 0))
+    sequences, row_pages = book.table.shape
+    for r, a in zip(rows, added):
+        if not 0 <= r < sequences or a < 0 or book.lengths[r] + a > row_pages * book.pt and r not in seen or r in seen:
+            status |= kl.KV_BAD_INDEX
+            continue
+        seen.add(r)
+        held, need = book.held(book.lengths[r]), book.held(book.lengths[r] + a)
+        if need - held > len(free):
+            status |= kl.KV_NO_PAGE
+            continue
+        for j in range(held, need):
+            page = free.pop(0)
+            book.table[r, j], book.references[page] = page, 1
+        book.lengths[r] += a
+    return status
+
+
+def reserve(book, rows, added):
+    r, a = lists(rows, added)
+    status = reserve_rule(book, rows, added)
+    assert kl.kv_reserve(book.kernel, 0, *book.p, r.data, a.data, len(rows), book.cache.layout, book.pages)
+    book.check(status)
+    return status
+
+
+def book_of(seed, sequences, row_pages, pages, pt):
+    book = Book(np.random.default_rng(seed), sequences, row_pages, pages, pt, heads=1, width=8, layers=1)
+    book.upload()
+    return book
+
+
+def test_reserve_first_of_a_sequence_counts(gpu):
+    """The entries left out take no pages: six are free and six are asked for by those that count."""
+    book = book_of(1, 4, 5, 6, 8)
+    assert reserve(book, [1, 1, 0], [30, 25, 9]) == kl.KV_BAD_INDEX
+    assert book.lengths.tolist() == [9, 30, 0, 0] and book.table[0].tolist() == [4, 5, -1, -1, -1]
+
+
+def test_reserve_first_in_range_counts(gpu):
+    """An entry out of range is not the first of its sequence."""
+    book = book_of(2, 4, 5, 24, 8)
+    assert reserve(book, [2, 2, 9, 2], [41, 10, 3, 17]) == kl.KV_BAD_INDEX
+    assert book.lengths.tolist() == [0, 0, 10, 0]
+
+
+@pytest.mark.parametrize("sequences", [300, 3000, 6000])
+def test_reserve_named_twice_in_long_lists(gpu, sequences):
+    rng = np.random.default_rng(sequences)
+    book = book_of(3, sequences, 4, 4 * sequences, 8)
+    for _ in range(3):
+        rows = rng.integers(0, sequences, sequences)
+        added = rng.integers(0, 32, sequences)
+        assert reserve(book, rows, added) == kl.KV_BAD_INDEX
+
