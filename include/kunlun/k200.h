@@ -463,7 +463,8 @@ bool kv_reserve(Kernel &, int device, int * table, int * lengths, int * referenc
 // children[i] continues parents[i] as it stood before the call: full pages are
 // shared, a last page that is not full is copied to a page that was free before
 // the call. What a child held is released. A sequence may be parent of several
-// children, and a parent may itself be a child; of forks to one child one is made, the others are left out and reported.
+// children, and a parent may itself be a child; of forks to one
+// child the first in range is made, the others are left out and reported.
 bool kv_fork(Kernel &, int device, void * k, void * v, int * table, int * lengths, int * references,
              const int * parents, const int * children, int count, const KVCacheLayout &, const KVPagesLayout &);
 // Releases what the listed sequences hold: rows -1, lengths 0.

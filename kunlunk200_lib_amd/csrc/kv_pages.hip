@@ -221,7 +221,7 @@ struct ForkNote {
 // Workgroup 0 finds the pages; workgroup 1 + i copies the parent's row aside (a
 // parent may be a child whose row the second launch overwrites).
 __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int *parents, const int *children,
-                                                          int count, ForkNote *notes, int *found, int *rows, int *claims) {
+                                                          int count, ForkNote *notes, int *found, int *rows, int *far_claims) {
     if (blockIdx.x > 0) {
         const int i = blockIdx.x - 1, s = parents[i];
         if (static_cast<unsigned>(s) >= static_cast<unsigned>(a.sequences)) return;
@@ -230,14 +230,20 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int
             rows[(int64_t)i * a.row_pages + j] = a.table[(int64_t)s * a.row_pages + j];
         return;
     }
-    __shared__ int scratch[kPlanWaves];
+    __shared__ int scratch[kPlanWaves], near_claims[kNearClaims];
+    int *claims = cleared_claims(near_claims, far_claims, a.sequences, children, count);
     int wanted = 0;
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
         const int i = i0 + threadIdx.x;
         int length = -1;
         if (i < count && sequence_ok(a, parents[i]) && sequence_ok(a, children[i])) {
             length = length_of(a, parents[i]);
-            claims[children[i]] = i;             // of forks to one child the last store's is made
+            claim(claims, children[i], i);
+        }
+        __syncthreads();
+        if (length >= 0 && !claimed(claims, children[i], i)) {
+            kk::report(a.status, kk::kBadIndex);
+            length = -1;
         }
         const bool part = length > 0 && length % a.pool.page_tokens != 0;
         int total;
@@ -247,16 +253,10 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int
     }
     const int have = free_pages(a.references, a.pool.pages, min(wanted, a.pool.pages), found, scratch);
     for (int i = threadIdx.x; i < count; i += kPlanThreads) {
-        const ForkNote note = notes[i];
-        if (note.length < 0) continue;
-        if (claims[children[i]] != i) {
-            notes[i].length = -1;
-            kk::report(a.status, kk::kBadIndex);
-            continue;
-        }
-        const int at = note.page;
-        if (at >= 0) notes[i].page = at < have ? found[at] : -2;
-        if (at >= have && at >= 0) kk::report(a.status, kk::kNoPage);
+        const int at = notes[i].page;
+        if (at < 0) continue;
+        notes[i].page = at < have ? found[at] : -2;
+        if (at >= have) kk::report(a.status, kk::kNoPage);
     }
 }
 
@@ -544,16 +544,17 @@ extern "C" int kk_kv_reserve(int *table, int *lengths, int *references, const in
 
 extern "C" size_t kk_kv_fork_workspace_bytes(const kunlun::KVPagesLayout &p, int count) {
     return (size_t)count * (sizeof(ForkNote) + sizeof(int) + (size_t)p.row_pages * sizeof(int)) +
-           (size_t)p.sequences * sizeof(int);
+           (size_t)(p.sequences > kNearClaims ? p.sequences : 0) * sizeof(int);
 }
 extern "C" int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *references, const int *parents, const int *children,
                int count, const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
                hipStream_t stream) {
     const PagesArgs a = args_of(k, v, table, lengths, references, c, p, status);
     ForkNote *notes = static_cast<ForkNote *>(workspace);
-    int *found = reinterpret_cast<int *>(notes + count), *claims = found + count, *rows = claims + p.sequences;
+    int *found = reinterpret_cast<int *>(notes + count), *rows = found + count;
+    int *far_claims = rows + (size_t)count * p.row_pages;
     hipLaunchKernelGGL(fork_plan, dim3(1 + count), dim3(kPlanThreads), 0, stream, a, parents, children, count, notes,
-                       found, rows, claims);
+                       found, rows, far_claims);
     // at most eight (layer, pool, head) blocks of the last page per workgroup
     const int blocks = p.layers * 2 * c.heads, copiers = std::max(1, std::min(blocks, 4096 / count));
     hipLaunchKernelGGL(fork_apply, dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);

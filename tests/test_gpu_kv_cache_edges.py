@@ -70,3 +70,27 @@ def test_reserve_named_twice_in_long_lists(gpu, sequences):
         added = rng.integers(0, 32, sequences)
         assert reserve(book, rows, added) == kl.KV_BAD_INDEX
 
+
+def fork(book, parents, children):
+    p, c = lists(parents, children)
+    first = [i for i, child in enumerate(children) if child not in children[:i]]
+    book.fork(np.array(parents)[first], np.array(children)[first])
+    assert kl.kv_fork(book.kernel, 0, *book.pools, *book.p, p.data, c.data, len(parents), book.cache.layout, book.pages)
+    book.check(kl.KV_BAD_INDEX if len(first) < len(parents) else 0)
+
+
+def test_fork_first_to_a_child_counts(gpu):
+    """The forks left out take no pages: two are free and two forks that count need one each."""
+    book = book_of(6, 4, 5, 10, 8)
+    reserve(book, [0, 1], [30, 25])
+    fork(book, [0, 1, 0], [2, 2, 3])
+    assert book.lengths.tolist() == [30, 25, 30, 30] and np.all(book.references[:10] > 0)
+
+
+def test_fork_named_twice_in_long_lists(gpu):
+    rng = np.random.default_rng(61)
+    book = book_of(7, 2600, 3, 12000, 8)
+    reserve(book, np.arange(2600), rng.integers(0, 25, 2600))
+    for _ in range(3):
+        fork(book, rng.integers(0, 2600, 2500).tolist(), rng.integers(0, 2600, 2500).tolist())
+
