@@ -457,7 +457,8 @@ struct KVPagesLayout {
 };
 const char * kv_pages_reason(const KVCacheLayout &, const KVPagesLayout &);
 // Makes room for added[i] more tokens of sequence rows[i] and adds them to its length (of a sequence that is listed
-// twice, by the first entry in range; the others are left out and reported).
+// twice, by the first entry in range; the others are left out and reported). In list order: an entry whose pages are
+// not there is refused and reported, and takes none from those after it.
 bool kv_reserve(Kernel &, int device, int * table, int * lengths, int * references, const int * rows,
                 const int * added, int count, const KVCacheLayout &, const KVPagesLayout &);
 // children[i] continues parents[i] as it stood before the call: full pages are

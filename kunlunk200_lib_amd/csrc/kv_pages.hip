@@ -148,16 +148,44 @@ __device__ __forceinline__ bool claimed(const int *claims, int s, int i) {
 
 // ---- kv_reserve ----------------------------------------------------------------------------
 
+constexpr int kLeftOut = -1, kRefused = -2;
+
+// For lists that ask for more pages than there are: in list order, whatever still fits is granted; what does not
+// takes nothing from those after it. One prefix sum finds the first entry that does not fit, then every later one
+// that needs more than is left there goes with it, so the next sum grants at least one more.
+__device__ __forceinline__ void refuse_what_does_not_fit(int *need_of, int *first_of, int count, int have, long long *sums,
+                                                         int *room) {
+    int taken = 0;
+    for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
+        const int i = i0 + threadIdx.x, left = have - taken, asked = i < count ? need_of[i] : kLeftOut;
+        long long need = max(asked, 0), total;
+        if (need > left) need = 0;
+        for (;;) {
+            const long long at = prefix<long long>(need, total, sums);
+            if (total <= left) {
+                if (i < count) first_of[i] = taken + static_cast<int>(at);
+                break;
+            }
+            const bool first = at <= left && at + need > left;
+            if (first) *room = left - static_cast<int>(at);
+            __syncthreads();
+            if (first || (at > left && need > *room)) need = 0;
+        }
+        if (asked > 0 && need == 0) need_of[i] = kRefused;
+        taken += static_cast<int>(total);
+    }
+}
+
 __global__ __launch_bounds__(kPlanThreads) void reserve(PagesArgs a, const int *rows, const int *added, int count,
                                                         int *need_of, int *first_of, int *end_of, int *found,
                                                         int *far_claims) {
-    __shared__ int scratch[kPlanWaves], near_claims[kNearClaims];
+    __shared__ int scratch[kPlanWaves], near_claims[kNearClaims], room;
     __shared__ long long sums[kPlanWaves];
     int *claims = cleared_claims(near_claims, far_claims, a.sequences, rows, count);
     int64_t wanted = 0;
     for (int i0 = 0; i0 < count; i0 += kPlanThreads) {
         const int i = i0 + threadIdx.x;
-        int need = -1;                           // -1: left out
+        int need = kLeftOut;
         if (i < count && sequence_ok(a, rows[i])) {
             const int64_t len = length_of(a, rows[i]), more = added[i];
             if (more >= 0 && len + more <= (int64_t)a.row_pages * a.pool.page_tokens) {
@@ -172,29 +200,24 @@ __global__ __launch_bounds__(kPlanThreads) void reserve(PagesArgs a, const int *
         // a claim of this step never takes a sequence from an earlier one: entries come in order
         if (need >= 0 && !claimed(claims, rows[i], i)) {
             kk::report(a.status, kk::kBadIndex);
-            need = -1;
+            need = kLeftOut;
         }
         long long total;
         const int64_t at = wanted + prefix<long long>(max(need, 0), total, sums);
         if (i < count) {
             need_of[i] = need;
-            // past the pool's size no page is left for it
-            first_of[i] = static_cast<int>(min<int64_t>(at, a.pool.pages));
+            first_of[i] = static_cast<int>(min<int64_t>(at, a.pool.pages));      // as it is where all are granted
         }
         wanted += total;
     }
     const int have = free_pages(a.references, a.pool.pages, static_cast<int>(min<int64_t>(wanted, a.pool.pages)),
                                 found, scratch);
+    if (have < wanted) refuse_what_does_not_fit(need_of, first_of, count, have, sums, &room);
     // lengths first, a thread for each listed sequence: 64 sequences in turn 3.9 us the launch, one wave each 4.7
     for (int i = threadIdx.x; i < count; i += kPlanThreads) {
         const int need = need_of[i];
-        if (need < 0) continue;
-        if (need > 0 && (int64_t)first_of[i] + need > have) {
-            kk::report(a.status, kk::kNoPage);
-            need_of[i] = 0;
-            continue;
-        }
-        a.lengths[rows[i]] = end_of[i];
+        if (need == kRefused) kk::report(a.status, kk::kNoPage);
+        if (need >= 0) a.lengths[rows[i]] = end_of[i];
     }
     __syncthreads();
     // a wave for each listed sequence

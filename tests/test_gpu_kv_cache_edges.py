@@ -71,6 +71,37 @@ def test_reserve_named_twice_in_long_lists(gpu, sequences):
         assert reserve(book, rows, added) == kl.KV_BAD_INDEX
 
 
+@pytest.mark.parametrize("needs,granted", [
+    ([20, 1], [1]), ([100, 1], [1]), ([4, 7, 6, 1], [0, 2]), ([10, 1, 1], [0]), ([3, 8, 8, 7, 1], [0, 3]),
+    ([1, 10, 2, 9, 3, 8, 4, 7], [0, 2, 4, 6]), ([11, 12, 13], [])])
+def test_reserve_refused_take_no_pages(gpu, needs, granted):
+    """Ten pages are free; an entry that does not fit leaves them to those after it."""
+    book = book_of(4, len(needs) + 1, 128, 10, 4)
+    book_rows = np.arange(len(needs))
+    assert bool(reserve(book, book_rows, [4 * n for n in needs]) & kl.KV_NO_PAGE) == (len(granted) < len(needs))
+    assert np.flatnonzero(book.lengths).tolist() == granted
+
+
+@pytest.mark.parametrize("sequences,pages,most", [(70, 60, 9), (1500, 900, 2), (2500, 3000, 40), (5000, 20000, 8)])
+def test_reserve_short_of_pages(gpu, sequences, pages, most):
+    """Lists that ask for more than there is, over several steps of the plan, some of them named twice or out of range."""
+    rng = np.random.default_rng(pages)
+    book = book_of(5, sequences, 3 * most, pages, 4)
+    for turn in range(4):
+        n = int(rng.integers(sequences // 2, sequences + 1))
+        rows = rng.permutation(sequences)[:n]
+        if turn % 2:
+            rows[rng.integers(0, n, n // 10)] = rng.integers(-1, sequences + 1, n // 10)
+        added = rng.integers(0, 4 * most, n)
+        added[rng.integers(0, n, n // 20)] = 4 * 3 * most
+        reserve(book, rows, added)
+        rows = rng.permutation(sequences)[: sequences // 4]
+        book.free(rows)
+        r, = lists(rows)
+        assert kl.kv_free(book.kernel, 0, *book.p, r.data, len(rows), book.cache.layout, book.pages)
+        book.check()
+
+
 def fork(book, parents, children):
     p, c = lists(parents, children)
     first = [i for i, child in enumerate(children) if child not in children[:i]]
