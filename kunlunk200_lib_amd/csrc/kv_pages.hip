@@ -338,24 +338,30 @@ __global__ __launch_bounds__(kCopyThreads) void fork_apply(PagesArgs a, const in
 
 // ---- kv_free -------------------------------------------------------------------------------
 
-__global__ __launch_bounds__(kCopyThreads) void free_rows(PagesArgs a, const int *list) {
-    const int s = list[blockIdx.x];
-    if (static_cast<unsigned>(s) >= static_cast<unsigned>(a.sequences)) {
-        if (threadIdx.x == 0) kk::report(a.status, kk::kBadIndex);
-        return;
-    }
-    // of two entries that name one sequence only one finds its length
+constexpr int kMostFreeGroups = 65536;           // a launch has fewer than 2^32 threads
+
+__global__ __launch_bounds__(kCopyThreads) void free_rows(PagesArgs a, const int *list, int count) {
     __shared__ int length;
-    if (threadIdx.x == 0) length = atomicExch(&a.lengths[s], 0);
-    __syncthreads();
     const int64_t most = (int64_t)a.row_pages * a.pool.page_tokens;
-    if (length < 0 || length > most) {
-        if (threadIdx.x == 0) kk::report(a.status, kk::kBadIndex);
+    for (int i = blockIdx.x; i < count; i += gridDim.x) {
+        const int s = list[i];
+        if (static_cast<unsigned>(s) >= static_cast<unsigned>(a.sequences)) {
+            if (threadIdx.x == 0) kk::report(a.status, kk::kBadIndex);
+            continue;
+        }
+        // of two entries that name one sequence only one finds its length
+        if (threadIdx.x == 0) length = atomicExch(&a.lengths[s], 0);
+        __syncthreads();
+        const int len = length;
+        __syncthreads();
+        if (len < 0 || len > most) {
+            if (threadIdx.x == 0) kk::report(a.status, kk::kBadIndex);
+        }
+        const int n = pages_of(a, len < 0 ? 0 : static_cast<int>(min<int64_t>(len, most)));
+        int *row = a.table + (int64_t)s * a.row_pages;
+        release_row(a, row, n);
+        for (int j = threadIdx.x; j < n; j += kCopyThreads) row[j] = -1;
     }
-    const int n = pages_of(a, length < 0 ? 0 : static_cast<int>(min<int64_t>(length, most)));
-    int *row = a.table + (int64_t)s * a.row_pages;
-    release_row(a, row, n);
-    for (int j = threadIdx.x; j < n; j += kCopyThreads) row[j] = -1;
 }
 
 // ---- kv_compact ----------------------------------------------------------------------------
@@ -586,8 +592,8 @@ extern "C" int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *refer
 
 extern "C" int kk_kv_free(int *table, int *lengths, int *references, const int *rows, int count, const kunlun::KVCacheLayout &c,
                const kunlun::KVPagesLayout &p, int *status, hipStream_t stream) {
-    hipLaunchKernelGGL(free_rows, dim3(count), dim3(kCopyThreads), 0, stream,
-                       args_of(nullptr, nullptr, table, lengths, references, c, p, status), rows);
+    hipLaunchKernelGGL(free_rows, dim3(std::min(count, kMostFreeGroups)), dim3(kCopyThreads), 0, stream,
+                       args_of(nullptr, nullptr, table, lengths, references, c, p, status), rows, count);
     return hipGetLastError();
 }
 

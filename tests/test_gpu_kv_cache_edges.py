@@ -125,3 +125,19 @@ def test_fork_named_twice_in_long_lists(gpu):
     for _ in range(3):
         fork(book, rng.integers(0, 2600, 2500).tolist(), rng.integers(0, 2600, 2500).tolist())
 
+
+def test_free_list_past_a_grid(gpu):
+    """More sequences than one launch dimension of whole workgroups holds."""
+    sequences = (1 << 24) + 70
+    layout = kl.KVCacheLayout(8, 16, 1, 8, 128, 128, 8)
+    pages = kl.KVPagesLayout(sequences, 1, 1, 0)
+    table, lengths = np.full((sequences, 1), -1, np.int32), np.zeros(sequences, np.int32)
+    at = [0, 5, 1 << 23, sequences - 1]
+    table[at, 0], lengths[at] = [3, 1, 3, 7], 9
+    references = np.bincount([3, 1, 3, 7], minlength=8).astype(np.int32)
+    b = [upload(x) for x in (table, lengths, references, np.arange(sequences, dtype=np.int32))]
+    assert kl.kv_free(kl.Kernel(), 0, *[x.data for x in b], sequences, layout, pages)
+    assert kl.kv_cache_status(0) == 0
+    assert not b[1].download(sequences, np.int32).any() and not b[2].download(8, np.int32).any()
+    assert np.all(b[0].download(sequences, np.int32) == -1)
+
