@@ -450,7 +450,8 @@ bool kv_append(Kernel &, int device, void * k_pool, void * v_pool, void * q_out,
 // sequence's last page), lengths [sequences] in tokens, references [pages]
 // (how many rows hold a page; 0: free). `layers` pools stand layer_stride
 // elements apart and share the table. Lists are distinct sequences; entries out
-// of range are left out and reported. New pages are the lowest free ones, in list order.
+// of range are left out and reported. New pages are the lowest free ones, in list order. Up to 2^30
+// pages and sequences; kv_fork takes up to 65535 entries.
 struct KVPagesLayout {
     int sequences, row_pages, layers;
     int64_t layer_stride;

@@ -16,6 +16,7 @@ namespace {
 
 constexpr int64_t kMostStride = int64_t(1) << 40;        // elements
 constexpr int64_t kMostTokens = int64_t(1) << 27;        // of a sequence
+constexpr int kMostCounted = 1 << 30;                    // pages and sequences that 32-bit loops count in steps
 
 struct Span {
     uintptr_t at;
@@ -226,6 +227,7 @@ const char * kv_pages_reason(const KVCacheLayout & c, const KVPagesLayout & p) {
     const char * cache = kv_cache_reason(c);
     if (*cache) return cache;
     if (p.sequences <= 0 || p.row_pages <= 0 || p.layers <= 0 || p.layers > 65535) return "shape";
+    if (p.sequences > kMostCounted || c.pages > kMostCounted) return "shape";
     if ((int64_t)p.row_pages * c.page_tokens > kMostTokens) return "length";
     if (p.layers > 1 && (p.layer_stride < pool_elements(c) || p.layer_stride > (INT64_MAX / 4) / p.layers ||
                          p.layer_stride % 8))
