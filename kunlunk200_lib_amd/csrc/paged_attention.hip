@@ -63,7 +63,7 @@ constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
 constexpr int kRowSteps = 1;             // what beginning a row counts in a share
 constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even goes through
-constexpr float kWeightLog2 = 14.0f;     // weights are scaled by 2^14
+constexpr float kWeightScale = 16384.0f; // of the weights' F16 parts
 
 struct AttendArgs {
     const _Float16 *k, *v;
@@ -226,10 +226,11 @@ __device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const floa
             for (int j = 0; j < VW; ++j) acc[nt][j] *= alpha;
             m[nt] = top;
         }
-        const float shift = kWeightLog2 - (top == -INFINITY ? 0.0f : top);
+        // scaled after the exponential: an exponent of 14 and a difference holds 2^-20 of it, 3e-7 of the weight
+        const float from = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float p = __builtin_amdgcn_exp2f(sc[i] + shift);
+            const float p = __builtin_amdgcn_exp2f(sc[i] - from) * kWeightScale;
             l[nt] += p;
             const _Float16 high = static_cast<_Float16>(p);
             pf[nt][i] = static_cast<_Float16>(fmaf(low, static_cast<float>(high), p));

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from test_gpu_kv_cache import Book, lists, upload
+from test_gpu_kv_cache import F32, Book, Cache, lists, run_attention, table_of, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -140,4 +140,38 @@ def test_free_list_past_a_grid(gpu):
     assert kl.kv_cache_status(0) == 0
     assert not b[1].download(sequences, np.int32).any() and not b[2].download(8, np.int32).any()
     assert np.all(b[0].download(sequences, np.int32) == -1)
+
+
+# --- paged_attention: weights and infinities --------------------------------------------------
+
+@pytest.mark.parametrize("heads,query_heads,width,page_tokens,longest", [
+    (8, 8, 64, 16, 40), (8, 8, 128, 20, 40), (1, 16, 64, 16, 40), (8, 8, 128, 16, 2816)])
+def test_attention_weights_in_f32(gpu, heads, query_heads, width, page_tokens, longest):
+    """Weights near the row's largest are as good as an F32 exponential.
+
+    Values of +1 and -1 make every sum of products exact (parts are multiples of 2^-10 up to 2^14 each), scores below
+    2^-10 leave weights within [0.998, 1]: exponential 1 ulp, 2^-24; the weight's parts 2^-10 / 2^14 = 2^-24 of the largest.
+    Scores: a = sum |q k|, e_s = a (2^-22 + (width + 3) 2^-24) twice (subtracted from the largest). Quotient: 2^-24 |y|,
+    and |y| <= 1."""
+    rng = np.random.default_rng(81)
+    lengths = [int(n) for n in rng.integers(1, 17, 64) * 2]
+    pages = sum(-(-n // page_tokens) for n in lengths) + 1
+    cache = Cache(rng, pages, page_tokens, heads, width)
+    table = table_of(rng, lengths, page_tokens, pages, -(-longest // page_tokens))
+    for s, n in enumerate(lengths):
+        for t in range(n):
+            cache.v[0, table[s, t // page_tokens], :, t % page_tokens] = 1 - 2 * (t % 2)
+    q = (rng.standard_normal((64, query_heads, width)) * 2.0 ** -17).astype(np.float32)
+    y, _ = run_attention(cache, table, lengths, q, scale=1.0, longest=longest)
+    for s, n in enumerate(lengths):
+        t = np.arange(n)
+        for h in range(query_heads):
+            k = cache.k[0, table[s, t // page_tokens], h * heads // query_heads, t % page_tokens].astype(np.float64)
+            score = k @ q[s, h].astype(np.float64)
+            assert np.abs(score).max() < 2.0 ** -10
+            p = np.exp(score - score.max())
+            gold = (p * (1 - 2 * (t % 2))).sum() / p.sum()
+            a = np.abs(k * q[s, h]).sum(1).max()
+            tol = 2.0 ** -24 * (1 + 1 + abs(gold)) + 2 * a * (2.0 ** -22 + (width + 3) * 2.0 ** -24)
+            assert np.abs(y[s, h] - gold).max() <= tol, (s, h, np.abs(y[s, h] - gold).max(), tol)
 
