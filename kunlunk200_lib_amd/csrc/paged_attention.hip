@@ -64,6 +64,8 @@ constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
 constexpr int kRowSteps = 1;             // what beginning a row counts in a share
 constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even goes through
 constexpr float kWeightScale = 16384.0f; // of the weights' F16 parts
+constexpr float kLeastPart = 0x1p-24f;    // the least F16 above 0
+constexpr float kLeastWeight = 0x1p100f;  // p times this is above kLeastPart for every normal p
 
 struct AttendArgs {
     const _Float16 *k, *v;
@@ -192,7 +194,6 @@ __device__ __forceinline__ void split_queries(float scale_log2, int heads, int w
 template <int VW, int NT, typename There>
 __device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const float (&undo)[NT], bool masked, There there, int c,
                                       float (&m)[NT], float (&l)[NT], float4v (&acc)[NT][VW], half8 (&pf)[NT]) {
-    const float low = c < 8 ? 0.0f : -1.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         float sc[8], sum = 0.0f, top = -INFINITY;
@@ -232,8 +233,11 @@ __device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const floa
         for (int i = 0; i < 8; ++i) {
             const float p = __builtin_amdgcn_exp2f(sc[i] - from) * kWeightScale;
             l[nt] += p;
-            const _Float16 high = static_cast<_Float16>(p);
-            pf[nt][i] = static_cast<_Float16>(fmaf(low, static_cast<float>(high), p));
+            // A weight above 0 keeps a high part above 0, which takes an infinite value to its infinity (the low part
+            // takes it off again: finite values lose nothing)
+            const float part = __builtin_amdgcn_fmed3f(p, p * kLeastWeight, kLeastPart);
+            const _Float16 high = static_cast<_Float16>(part);
+            pf[nt][i] = c < 8 ? high : static_cast<_Float16>(p - static_cast<float>(high));
         }
     }
 }

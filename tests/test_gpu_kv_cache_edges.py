@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from test_gpu_kv_cache import F32, Book, Cache, lists, run_attention, table_of, upload
+from test_gpu_kv_cache import F16, F32, Book, Cache, lists, run_attention, table_of, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -174,4 +174,85 @@ def test_attention_weights_in_f32(gpu, heads, query_heads, width, page_tokens, l
             a = np.abs(k * q[s, h]).sum(1).max()
             tol = 2.0 ** -24 * (1 + 1 + abs(gold)) + 2 * a * (2.0 ** -22 + (width + 3) * 2.0 ** -24)
             assert np.abs(y[s, h] - gold).max() <= tol, (s, h, np.abs(y[s, h] - gold).max(), tol)
+
+
+# heads, query heads, width, tokens of a page, length, `longest`, order: whole rows, column tiles, split, equal shares
+ROUTES = [
+    (2, 4, 64, 16, 60, 60, "heads"),
+    (2, 4, 72, 20, 60, 60, "tokens"),
+    (1, 16, 128, 16, 60, 60, "heads"),
+    (2, 2, 256, 16, 60, 60, "heads"),
+    (1, 2, 128, 16, 3000, 3000, "heads"),
+    (8, 8, 128, 16, 700, 2816, "heads"),
+]
+
+
+def one_score_cache(rng, heads, width, page_tokens, n, order, score):
+    """A cache of one sequence (the first of eight) whose key t gives `score[t]` to the query (1, 0, ...)."""
+    cache = Cache(rng, -(-n // page_tokens) + 1, page_tokens, heads, width, order)
+    table = table_of(rng, [n], page_tokens, cache.layout.pages, -(-n // page_tokens))
+    t = np.arange(n)
+    place = (0, table[0, t // page_tokens], slice(None), t % page_tokens)
+    cache.k[place] = 0
+    cache.k[place + (0,)] = np.float16(score)[:, None]
+    return cache, table, place
+
+
+def run_one(cache, table, n, q, longest):
+    """The row of one sequence, beside seven empty ones where `longest` is more (so that it is shared out)."""
+    beside = 7 if longest > n else 0
+    row_pages = -(-longest // cache.layout.page_tokens)
+    rows = np.full((1 + beside, row_pages), -1, np.int32)
+    rows[0, :table.shape[1]] = table[0]
+    y, route = run_attention(cache, rows, [n] + [0] * beside, np.repeat(q[None], 1 + beside, 0), scale=1.0,
+                             longest=longest)
+    assert not beside or route == "paged_attention_even"
+    return y[0]
+
+
+@pytest.mark.parametrize("route", range(len(ROUTES)))
+@pytest.mark.parametrize("gap", [20, 30, 45, 60, 80])
+@pytest.mark.parametrize("first", [False, True])
+def test_attention_infinite_values_of_small_weight(gpu, route, gap, first):
+    """An infinite value whose weight is e^-gap of the row's largest, far below what its F16 parts hold, gives its
+    infinity, before and after the largest; the other columns stay what they are."""
+    heads, query_heads, width, page_tokens, n, longest, order = ROUTES[route]
+    rng = np.random.default_rng(82)
+    score = np.full(n, -float(gap))
+    heavy = n - 1 if first else 0
+    score[heavy] = 0.0
+    cache, table, place = one_score_cache(rng, heads, width, page_tokens, n, order, score)
+    for t, d, x in ((n // 2, 3, np.inf), (n // 3, 4, -np.inf), (5, 5, np.inf), (n - 7, 5, -np.inf), (17, 6, np.nan)):
+        cache.v[0, place[1][t], :, place[3][t], d] = x
+    q = np.zeros((query_heads, width), np.float32)
+    q[:, 0] = 1.0
+    y = run_one(cache, table, n, q, longest)
+    assert np.all(y[:, 3] == np.inf) and np.all(y[:, 4] == -np.inf) and np.all(np.isnan(y[:, 5:7]))
+    p = np.exp(score)
+    v = cache.v[place].astype(np.float64)                                   # [token, head, value]
+    others = [d for d in range(width) if not 3 <= d <= 6]
+    for h in range(query_heads):
+        x = v[:, h * heads // query_heads][:, others]
+        gold, size = p @ x / p.sum(), p @ np.abs(x) / p.sum()
+        # the scores are exact but for their factor (up to gap * 2^-22); parts below 2^-38 of the largest weight are lost
+        tol = size * (2 * gap * 2.0 ** -22 + 2.0 ** -20 + 2 * n * 2.0 ** -24) + 2.0 ** -38 * np.abs(x).sum(0)
+        assert np.all(np.abs(y[h, others] - gold) <= tol)
+
+
+@pytest.mark.parametrize("route", range(len(ROUTES)))
+def test_attention_infinite_values_of_no_weight(gpu, route):
+    """A weight below the smallest F32 number is 0, and 0 times infinity not a number, as products of F32 have it."""
+    heads, query_heads, width, page_tokens, n, longest, order = ROUTES[route]
+    rng = np.random.default_rng(83)
+    score = np.full(n, -120.0)
+    score[n // 4] = 0.0
+    cache, table, place = one_score_cache(rng, heads, width, page_tokens, n, order, score)
+    for t, d in ((2, 3), (n - 2, 4)):
+        cache.v[0, place[1][t], :, place[3][t], d] = np.inf
+    q = np.zeros((query_heads, width), np.float32)
+    q[:, 0] = 1.0
+    y = run_one(cache, table, n, q, longest)
+    odd = np.zeros(width, bool)
+    odd[3:5] = True
+    assert np.all(np.isnan(y[:, odd])) and np.all(np.isfinite(y[:, ~odd]))
 
