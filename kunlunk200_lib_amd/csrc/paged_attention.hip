@@ -156,36 +156,37 @@ __device__ __forceinline__ T load_row(const _Float16 *p) {
     else return *reinterpret_cast<const T *>(p);
 }
 
+// The exponent of a float's size: 128 for what is not finite, -127 for 0 and subnormal ones.
+__device__ __forceinline__ int exponent_of(float v) { return static_cast<int>((__float_as_uint(v) >> 23) & 0xff) - 127; }
+
 // q columns: column c is head c % 8 of each tile, its high (c < 8) or low part; the scores times `undo` are in base 2.
 template <int D32, int NT, bool FULL>
-__device__ __forceinline__ void split_queries(float scale_log2, int heads, int width, int c, int G, float (&q)[NT][D32][8],
+__device__ __forceinline__ void split_queries(float scale_log2, int heads, int width, int c, int G, const float (&q)[NT][D32][8],
                                               half8 (&qf)[NT][D32], float (&undo)[NT]) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const float scale = nt * 8 + (c & 7) < heads ? scale_log2 : 0.0f;
+        const bool column = nt * 8 + (c & 7) < heads;
         float top = 0.0f;
-#pragma unroll
-        for (int d = 0; d < D32; ++d) {
-            const bool in = FULL || d * 32 + G * 8 < width;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                q[nt][d][i] = in ? q[nt][d][i] * scale : 0.0f;
-                top = fmaxf(top, fabsf(q[nt][d][i]));
-            }
-        }
-        top = across_groups_max(top);
-        // 2^e with top * 2^e in [2^10, 2^11); Inf stays as it is
-        const int exponent = static_cast<int>((__float_as_uint(top) >> 23) & 0xff) - 127;
-        const int e = top == 0.0f || exponent == 128 ? 0 : min(10 - exponent, 100);
-        undo[nt] = ldexpf(1.0f, -e);
 #pragma unroll
         for (int d = 0; d < D32; ++d)
 #pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, FULL || d * 32 + G * 8 < width ? fabsf(q[nt][d][i]) : 0.0f);
+        const int size = exponent_of(across_groups_max(top));
+        // 2^e with top * |scale| * 2^e in [2^9, 2^11)
+        const int e = size == 128 ? 0 : max(-126, min(126, min(9 - size, 110) - exponent_of(scale_log2)));
+        undo[nt] = ldexpf(1.0f, -e);
+        const float factor = column ? ldexpf(scale_log2, e) : 0.0f;
+#pragma unroll
+        for (int d = 0; d < D32; ++d) {
+            const float by = FULL || d * 32 + G * 8 < width ? factor : 0.0f;
+#pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float x = ldexpf(q[nt][d][i], e);
-                const _Float16 high = static_cast<_Float16>(x);
+                const float x = q[nt][d][i] * by;
+                // a value other than 0 keeps a high part other than 0 for infinite keys, as the weights do
+                const _Float16 high = static_cast<_Float16>(__builtin_amdgcn_fmed3f(x, x * 0x1p127f, copysignf(kLeastPart, x)));
                 qf[nt][d][i] = c < 8 ? high : static_cast<_Float16>(x - static_cast<float>(high));
             }
+        }
     }
 }
 

@@ -256,3 +256,28 @@ def test_attention_infinite_values_of_no_weight(gpu, route):
     odd[3:5] = True
     assert np.all(np.isnan(y[:, odd])) and np.all(np.isfinite(y[:, ~odd]))
 
+
+@pytest.mark.parametrize("route", range(len(ROUTES)))
+@pytest.mark.parametrize("small", [1e-6, -1e-12, 1e-30])
+def test_attention_infinite_keys_under_small_queries(gpu, route, small):
+    """An infinite key gives its infinity to the score however small the query's value beside the others is."""
+    heads, query_heads, width, page_tokens, n, longest, order = ROUTES[route]
+    rng = np.random.default_rng(84)
+    score = rng.integers(-16, 17, n) / 8.0
+    cache, table, place = one_score_cache(rng, heads, width, page_tokens, n, order, score)
+    gone = [3, n // 2, n - 1]
+    for t in gone:
+        cache.k[0, place[1][t], :, place[3][t], 1] = -np.inf * np.sign(small)
+    q = np.zeros((query_heads, width), np.float32)
+    q[:, 0], q[:, 1] = 1.0, small
+    y = run_one(cache, table, n, q, longest)
+    p = np.exp(score - score.max())
+    p[gone] = 0
+    v = cache.v[place].astype(np.float64)
+    for h in range(query_heads):
+        x = v[:, h * heads // query_heads]
+        tol = (p @ np.abs(x)) / p.sum() * (2.0 ** -19 + 2 * n * 2.0 ** -24)
+        assert np.all(np.abs(y[h] - p @ x / p.sum()) <= tol)
+    cache.k[0, place[1][7], :, place[3][7], 1] = np.inf * np.sign(small)    # a score of +Inf: not a number
+    assert np.all(np.isnan(run_one(cache, table, n, q, longest)))
+
