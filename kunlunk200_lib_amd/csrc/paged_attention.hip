@@ -172,8 +172,8 @@ __device__ __forceinline__ void split_queries(float scale_log2, int heads, int w
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, FULL || d * 32 + G * 8 < width ? fabsf(q[nt][d][i]) : 0.0f);
         const int size = exponent_of(across_groups_max(top));
-        // 2^e with top * |scale| * 2^e in [2^9, 2^11)
-        const int e = size == 128 ? 0 : max(-126, min(126, min(9 - size, 110) - exponent_of(scale_log2)));
+        // 2^e with top * |scale| * 2^e in [2^9, 2^11); beside an infinite value every finite one stays finite
+        const int e = max(-126, min(126, min(9 - size, 110) - exponent_of(scale_log2)));
         undo[nt] = ldexpf(1.0f, -e);
         const float factor = column ? ldexpf(scale_log2, e) : 0.0f;
 #pragma unroll

@@ -281,3 +281,21 @@ def test_attention_infinite_keys_under_small_queries(gpu, route, small):
     cache.k[0, place[1][7], :, place[3][7], 1] = np.inf * np.sign(small)    # a score of +Inf: not a number
     assert np.all(np.isnan(run_one(cache, table, n, q, longest)))
 
+
+@pytest.mark.parametrize("route", range(len(ROUTES)))
+def test_attention_infinite_queries(gpu, route):
+    """An infinite query value beside large finite ones: its infinity alone decides the scores."""
+    heads, query_heads, width, page_tokens, n, longest, order = ROUTES[route]
+    rng = np.random.default_rng(85)
+    score = np.where(np.arange(n) % 3, -1.0, -2.0)
+    cache, table, place = one_score_cache(rng, heads, width, page_tokens, n, order, score)
+    cache.k[place + (1,)] = 1.0
+    q = np.zeros((query_heads, width), np.float32)
+    q[:, 0], q[:, 1] = np.inf, 1e30
+    q[:, 2:] = 0.0
+    cache.k[place + (slice(2, None),)] = 0
+    y = run_one(cache, table, n, q, longest)
+    assert np.all(y == 0)                                                  # every score -Inf
+    cache.k[place + (0,)] = 1.0
+    assert np.all(np.isnan(run_one(cache, table, n, q, longest)))          # every score +Inf
+
