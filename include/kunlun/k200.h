@@ -428,7 +428,7 @@ bool paged_attention(Kernel &, int device, void * y, const void * q, const void 
 // values (2j, 2j + 1) (adjacent) or (j, j + rotary / 2) (halves). k, v rows of
 // [heads][width] and q rows of [query_heads][width] values of `type` are
 // *_stride elements apart, so that they may lie in one product's rows. Turned q
-// goes to q_out (q may be null, then query_heads is ignored; q_out may be q with
+// goes to q_out (q may be null, then query_heads and the strides of q are ignored; q_out may be q with
 // equal strides). k and v are rounded to F16 once. position null: token i is the
 // newest, lengths[i] - 1, of sequence i (sequence null too, tokens <= sequences). A
 // negative position or sequence marks a token that is left out; one out of range is left out and reported. Two tokens of one

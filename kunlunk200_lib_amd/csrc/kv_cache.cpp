@@ -174,8 +174,10 @@ const char * kv_append_reason(const KVCacheLayout & c, const KVAppendLayout & p)
 
 bool kv_append(Kernel & kernel, int id, void * k_pool, void * v_pool, void * q_out, const void * q, const void * k,
                const void * v, const int * sequence, const int * position, const int * lengths, const int * table,
-               const float * cosine, const float * sine, const KVCacheLayout & c, const KVAppendLayout & p) {
+               const float * cosine, const float * sine, const KVCacheLayout & c, const KVAppendLayout & given) {
     std::lock_guard<std::recursive_mutex> lock(detail::mutex());
+    KVAppendLayout p = given;
+    if (!q) p.query_heads = 0;          // without queries their layout is ignored
     if (*kv_append_reason(c, p) || !k_pool || !v_pool || !k || !v || !table) return false;
     const bool queries = q != nullptr;
     if (queries != (q_out != nullptr) || (queries && p.query_heads == 0)) return false;

@@ -299,3 +299,23 @@ def test_attention_infinite_queries(gpu, route):
     cache.k[place + (0,)] = 1.0
     assert np.all(np.isnan(run_one(cache, table, n, q, longest)))          # every score +Inf
 
+
+# --- kv_append ------------------------------------------------------------------------------
+
+def test_append_without_queries_ignores_their_layout(gpu):
+    rng = np.random.default_rng(91)
+    cache = Cache(rng, 4, 16, 2, 64)
+    rows = rng.standard_normal((3, 256)).astype(np.float32)
+    k_pool, v_pool = cache.upload()
+    r, s, p, t = upload(rows), *lists([0, 0, 0], [0, 5, 17], [[2, 1]])
+    kernel = kl.Kernel()
+    for query_heads, stride in ((4, 0), (5000, 0), (-1, -7), (4, 1 << 50)):
+        call = kl.KVAppendLayout(3, 1, 2, query_heads, stride, 256, 256, stride, 0, 0, kl.RotaryPairs.adjacent, F32)
+        assert kl.kv_append(kernel, 0, k_pool, v_pool, None, None, r.data, r.data + 512, s.data, p.data, None, t.data,
+                            None, None, cache.layout, call), (query_heads, stride)
+        assert kl.kv_cache_status(0) == 0
+    _, (k, v) = cache.download()
+    for i, (page, at) in enumerate(((2, 0), (2, 5), (1, 1))):
+        assert np.array_equal(k[0, page, :, at], rows[i, :128].reshape(2, 64).astype(np.float16))
+        assert np.array_equal(v[0, page, :, at], rows[i, 128:].reshape(2, 64).astype(np.float16))
+
