@@ -431,8 +431,9 @@ bool paged_attention(Kernel &, int device, void * y, const void * q, const void 
 // goes to q_out (q may be null, then query_heads and the strides of q are ignored; q_out may be q with
 // equal strides). k and v are rounded to F16 once. position null: token i is the
 // newest, lengths[i] - 1, of sequence i (sequence null too, tokens <= sequences). A
-// negative position or sequence marks a token that is left out; one out of range is left out and reported. Two tokens of one
-// call must not name one place.
+// negative position or sequence marks a token that is left out; one out of range, or without a page
+// in the pool, is left out whole and reported: nothing is stored and its row of q_out stays as it was. Two tokens of
+// one call must not name one place.
 enum class RotaryPairs { adjacent, halves };
 struct KVAppendLayout {
     int tokens, sequences, row_pages, query_heads;

@@ -79,16 +79,14 @@ __global__ __launch_bounds__(kThreads) void append(AppendArgs a) {
     const T *from = (is_q ? static_cast<const T *>(a.q) + token * a.q_stride
                           : is_k ? static_cast<const T *>(a.k) + token * a.k_stride
                                  : static_cast<const T *>(a.v) + token * a.v_stride) + h * a.pool.width;
-    _Float16 *to = nullptr;
-    if (!is_q) {
-        const int page = a.table[(int64_t)s * a.row_pages + page_at];
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.pages)) {
-            kk::report(a.status, kk::kBadPage);
-            return;
-        }
-        to = (is_k ? a.k_pool : a.v_pool) + page * a.pool.page_stride + h * a.pool.head_stride +
-             (pos - page_at * a.pool.page_tokens) * a.pool.token_stride;
+    // a token without a page is left out whole, its query too
+    const int page = a.table[(int64_t)s * a.row_pages + page_at];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.pages)) {
+        if (in_token == 0) kk::report(a.status, kk::kBadPage);
+        return;
     }
+    _Float16 *to = (is_k ? a.k_pool : a.v_pool) + page * a.pool.page_stride + h * a.pool.head_stride +
+                   (pos - page_at * a.pool.page_tokens) * a.pool.token_stride;       // of a key or a value
     T *q_to = is_q ? static_cast<T *>(a.q_out) + token * a.q_out_stride + h * a.pool.width : nullptr;
 
     const int half = a.rotary / 2;

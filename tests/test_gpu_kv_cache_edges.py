@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from test_gpu_kv_cache import F16, F32, Book, Cache, lists, run_attention, table_of, upload
+from test_gpu_kv_cache import F16, F32, GUARD, Book, Cache, lists, run_attention, table_of, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -318,4 +318,39 @@ def test_append_without_queries_ignores_their_layout(gpu):
     for i, (page, at) in enumerate(((2, 0), (2, 5), (1, 1))):
         assert np.array_equal(k[0, page, :, at], rows[i, :128].reshape(2, 64).astype(np.float16))
         assert np.array_equal(v[0, page, :, at], rows[i, 128:].reshape(2, 64).astype(np.float16))
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rotary,pairs", [(64, 0), (64, 1), (6, 0), (0, 0)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_leaves_the_whole_token_out(gpu, half, rotary, pairs, in_place):
+    """A token without a page is left out with its query, as one out of range is."""
+    rng = np.random.default_rng(92)
+    dtype = np.float16 if half else np.float32
+    cache = Cache(rng, 4, 16, 2, 64)
+    rows = rng.standard_normal((5, 512)).astype(dtype)                     # 4 query heads, 2 + 2
+    k_pool, v_pool = cache.upload()
+    r, out = upload(rows), upload(np.full((5, 256), GUARD, dtype))
+    s, p, t = lists([0, 1, 0, 1, -1], [3, 20, 16, 2, 0], [[2, -1], [1, 4]])
+    angle = rng.standard_normal((32, max(1, rotary // 2)))
+    cosine, sine = upload(np.cos(angle).astype(np.float32)), upload(np.sin(angle).astype(np.float32))
+    size = rows.itemsize
+    call = kl.KVAppendLayout(5, 2, 2, 4, 512, 512, 512, 512 if in_place else 256, rotary, 32, kl.RotaryPairs(pairs),
+                             F16 if half else F32)
+    assert kl.kv_append(kl.Kernel(), 0, k_pool, v_pool, r.data if in_place else out.data, r.data, r.data + 256 * size,
+                        r.data + 384 * size, s.data, p.data, None, t.data, cosine.data, sine.data, cache.layout, call)
+    assert kl.kv_cache_status(0) == kl.KV_BAD_PAGE
+    q = (r.download(rows.shape, dtype)[:, :256] if in_place else out.download((5, 256), dtype))
+    before = rows[:, :256] if in_place else np.full((5, 256), GUARD, dtype)
+    for i, there in enumerate((True, False, False, True, False)):
+        if not there:
+            assert np.array_equal(q[i], before[i]), f"token {i} wrote its query"
+        else:
+            assert not np.any(q[i] == np.array(GUARD, dtype))
+            assert np.array_equal(q[i].reshape(4, 64)[:, rotary:], rows[i, :256].reshape(4, 64)[:, rotary:])
+    _, (k, _) = cache.download()
+    want = cache.k.copy()
+    for page, at in ((2, 3), (1, 2)):
+        want[0, page, :, at] = k[0, page, :, at]
+    assert np.array_equal(k, want)
 
