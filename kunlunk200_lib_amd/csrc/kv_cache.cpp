@@ -394,8 +394,9 @@ bool process_logits(Kernel & kernel, int id, void * y, const void * logits, cons
                     const LogitsLayout & p) {
     std::lock_guard<std::recursive_mutex> lock(detail::mutex());
     if (*logits_reason(p) || !y || !logits) return false;
-    if (history && (!history_lengths || !penalties)) return false;
-    if (bias_ids && (!bias_values || !bias_lengths)) return false;
+    // a stride is a list's room too: 0 would pass over a list that is given
+    if (history && (!history_lengths || !penalties || p.history_stride == 0)) return false;
+    if (bias_ids && (!bias_values || !bias_lengths || p.bias_stride == 0)) return false;
     if (!aligned_to(4, {y, logits, penalties, history, history_lengths, bias_ids, bias_values, bias_lengths, mask}))
         return false;
     const Span out = rows_span(y, p.rows, p.y_stride, p.vocabulary, 4);

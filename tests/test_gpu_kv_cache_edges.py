@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from test_gpu_kv_cache import F16, F32, GUARD, Book, Cache, lists, run_attention, table_of, upload
+from test_gpu_kv_cache import F16, F32, GUARD, Book, Cache, finish, lists, run_attention, table_of, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -353,4 +353,37 @@ def test_append_leaves_the_whole_token_out(gpu, half, rotary, pairs, in_place):
     for page, at in ((2, 3), (1, 2)):
         want[0, page, :, at] = k[0, page, :, at]
     assert np.array_equal(k, want)
+
+
+# --- process_logits -------------------------------------------------------------------------
+
+def logits_call(rows, vocabulary, past, biases, history_stride, bias_stride, history_lengths, bias_lengths):
+    rng = np.random.default_rng(95)
+    z = rng.standard_normal((rows, vocabulary)).astype(np.float32)
+    history = rng.integers(0, vocabulary, (rows, past)).astype(np.int32)
+    ids = rng.integers(0, vocabulary, (rows, biases)).astype(np.int32)
+    values = rng.standard_normal((rows, biases)).astype(np.float32)
+    penalties = np.tile(np.float32([1.5, 0.25, 0.5]), (rows, 1))
+    y = upload(np.full((rows, vocabulary), GUARD, np.float32))
+    b = [upload(z), upload(penalties), upload(history), upload(np.int32(history_lengths)), upload(ids), upload(values),
+         upload(np.int32(bias_lengths))]
+    call = kl.LogitsLayout(rows, vocabulary, vocabulary, vocabulary, history_stride, bias_stride, 0)
+    done = kl.process_logits(kl.Kernel(), 0, y.data, *[x.data for x in b], None, call)
+    finish()
+    gold = z.astype(np.float64)
+    for i in range(rows):
+        h = history[i, :max(0, history_lengths[i])]
+        n = np.bincount(h, minlength=vocabulary)
+        gold[i] = np.where(n > 0, np.where(gold[i] > 0, gold[i] / 1.5, gold[i] * 1.5) - n * 0.25 - 0.5, gold[i])
+        last = dict(zip(ids[i, :max(0, bias_lengths[i])], values[i]))
+        for t, x in last.items():
+            gold[i, t] += np.float64(x)
+    return done, y.download((rows, vocabulary), np.float32), gold, past
+
+
+@pytest.mark.parametrize("history_stride,bias_stride", [(0, 3), (7, 0), (0, 0)])
+def test_logits_refuses_lists_without_room(gpu, history_stride, bias_stride):
+    """A stride of 0 leaves a given list no room: refused, not passed over."""
+    done, y, _, _ = logits_call(1, 50, 7, 3, history_stride, bias_stride, [7], [3])
+    assert done is False and np.all(y == GUARD)
 
