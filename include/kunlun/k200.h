@@ -490,7 +490,8 @@ bool kv_copy_pages(Kernel &, int device, void * k, void * v, const int * sources
 // -= n f + (n > 0) p; z += the value of the row's last bias entry for t; then
 // -inf where bit t % 32 of mask word t / 32 is 0. penalties, history, bias_ids
 // and mask may be null (nothing of the kind; the bias arrays go together, history
-// needs penalties). history_stride and bias_stride are the lists' room as well: above 0 for a list that is given.
+// needs penalties). history_stride and bias_stride are the lists' room as well: above 0 for a list that is given; a length
+// out of it is cut and reported by kv_cache_status.
 // mask_stride 0: one mask for all rows. Entries outside the vocabulary are left out. y may be logits
 // (equal strides). Strides are elements between rows.
 struct LogitsLayout {

@@ -417,7 +417,7 @@ bool process_logits(Kernel & kernel, int id, void * y, const void * logits, cons
     detail::DeviceContext & ctx = detail::context(id);
     detail::check_hip((hipError_t)kk_process_logits(static_cast<float *>(y), static_cast<const float *>(logits), penalties,
                                                     history, history_lengths, bias_ids, bias_values, bias_lengths, mask, p,
-                                                    ctx.cus, ctx.stream),
+                                                    ctx.status + 1, ctx.cus, ctx.stream),
                       "kk_process_logits");
     note(impl, id, "process_logits");
     return true;

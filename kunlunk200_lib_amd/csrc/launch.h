@@ -185,6 +185,6 @@ int kk_kv_copy_pages(void *k, void *v, const int *sources, const int *destinatio
 int kk_process_logits(float *y, const float *logits, const float *penalties, const int *history,
                       const int *history_lengths, const int *bias_ids, const float *bias_values,
                       const int *bias_lengths, const uint32_t *mask, const kunlun::LogitsLayout &p,
-                      int cus, hipStream_t stream);
+                      int *status, int cus, hipStream_t stream);
 
 }

@@ -8,6 +8,7 @@
 // does not matter. Each slice reads the row's lists (from the L2 after the first).
 #include "device_common.h"
 #include "launch.h"
+#include "paged.h"
 
 #include <kunlun/k200.h>
 
@@ -24,6 +25,7 @@ struct LogitsArgs {
     const int *bias_lengths;
     const uint32_t *mask;
     int64_t logits_stride, y_stride, history_stride, bias_stride, mask_stride;
+    int *status;
     int vocabulary;
 };
 
@@ -65,8 +67,14 @@ __global__ __launch_bounds__(kThreads) void process(LogitsArgs a) {
         const int at = min(i, n - 1);
         bits[u] = a.mask ? a.mask[row * a.mask_stride + (first + at) / 32] >> (at & 28) : ~0u;
     }
-    const int past = counted ? static_cast<int>(min<int64_t>(scalar_load(a.history_lengths + row), a.history_stride)) : 0;
-    const int given = biased ? static_cast<int>(min<int64_t>(scalar_load(a.bias_lengths + row), a.bias_stride)) : 0;
+    // a list's length, cut to its room and reported where that is less
+    auto length = [&](const int *lengths, int64_t room) {
+        const int n = scalar_load(lengths + row);
+        if ((n < 0 || n > room) && first == 0 && tid == 0) kk::report(a.status, kk::kBadIndex);
+        return static_cast<int>(min<int64_t>(max(n, 0), room));
+    };
+    const int past = counted ? length(a.history_lengths, a.history_stride) : 0;
+    const int given = biased ? length(a.bias_lengths, a.bias_stride) : 0;
     int seen[kAhead], id[2];
     float value[2];
 #pragma unroll
@@ -157,10 +165,10 @@ void launch(const LogitsArgs &a, int rows, bool vec, hipStream_t stream) {
 extern "C" int kk_process_logits(float *y, const float *logits, const float *penalties, const int *history,
                       const int *history_lengths, const int *bias_ids, const float *bias_values,
                       const int *bias_lengths, const uint32_t *mask, const kunlun::LogitsLayout &p,
-                      int cus, hipStream_t stream) {
+                      int *status, int cus, hipStream_t stream) {
     if (p.rows <= 0 || p.rows > 65535 || p.vocabulary <= 0) return hipErrorInvalidValue;
     const LogitsArgs a{y, logits, penalties, history, history_lengths, bias_ids, bias_values, bias_lengths, mask,
-                       p.logits_stride, p.y_stride, p.history_stride, p.bias_stride, p.mask_stride, p.vocabulary};
+                       p.logits_stride, p.y_stride, p.history_stride, p.bias_stride, p.mask_stride, status, p.vocabulary};
     const bool vec = ((uintptr_t)y | (uintptr_t)logits) % 16 == 0 && (p.logits_stride | p.y_stride) % 4 == 0;
     // larger slices read the lists less often, smaller ones leave no CU idle: 200 rows x 32000, history 3000: slices of
     // 4096 logits 20.1 us, 2048 16.5, 1024 16.7; up to 64 rows they are equal

@@ -1,5 +1,5 @@
 // What the kernels of the paged key-value cache share: addresses in a pool and
-// the status word they report to.
+// the status word that they and the logits step report to.
 #pragma once
 
 #include <hip/hip_runtime.h>

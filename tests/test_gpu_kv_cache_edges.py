@@ -387,3 +387,15 @@ def test_logits_refuses_lists_without_room(gpu, history_stride, bias_stride):
     done, y, _, _ = logits_call(1, 50, 7, 3, history_stride, bias_stride, [7], [3])
     assert done is False and np.all(y == GUARD)
 
+
+@pytest.mark.parametrize("history_lengths,bias_lengths,status", [
+    ([7, 0, 3], [3, 0, 1], 0), ([8, 0, 3], [3, 0, 1], 2), ([7, -1, 3], [3, 0, 1], 2), ([7, 0, 3], [3, 0, 2 ** 31 - 1], 2),
+    ([7, 0, 3], [-5, 0, 1], 2)])
+@pytest.mark.parametrize("vocabulary", [50, 3000])
+def test_logits_reports_lengths_out_of_range(gpu, history_lengths, bias_lengths, status, vocabulary):
+    """A list's length is cut to its row, and reported as the cache's lengths are."""
+    assert gpu.kv_cache_status(0) == 0
+    done, y, gold, past = logits_call(3, vocabulary, 7, 3, 7, 3, history_lengths, bias_lengths)
+    assert done is True and gpu.kv_cache_status(0) == status
+    assert np.all(np.abs(y - gold) <= 4 * 2.0 ** -24 * (2 * np.abs(gold) + 2 + past + 5))
+
