@@ -407,8 +407,11 @@ int kv_cache_status(int device);
 // (window 0: all); a sequence of length 0, and a row of which every weight is 0, give zeros. Pages before
 // the window and past the length are not read. `longest` bounds the lengths
 // (up to row_pages * page_tokens). q and y have rows of [query_heads][width] values of
-// `type`, q_stride and y_stride elements apart. F32 q and y get F32 arithmetic
-// (products of keys and weights split in two F16 parts, F32 sums and statistics).
+// `type`, q_stride and y_stride elements apart. F32 q and y get sums and
+// statistics in F32; queries and weights are factors of two F16 parts, which hold a query value to 2^-22 of itself or
+// 2^-34 of its row's largest and a weight to 2^-22 of itself or 2^-39 of the largest, whichever is more. Infinities
+// and what is not a number follow F32 products: an infinite value gives its infinity wherever its weight is above
+// 2^-126 of the largest, an infinite key wherever the query's value is not 0. scale * log2(e) has to be finite.
 struct PagedAttentionLayout {
     int sequences, query_heads, longest, window, row_pages;
     int64_t q_stride, y_stride;

@@ -121,7 +121,7 @@ const char * paged_attention_reason(const KVCacheLayout & c, const PagedAttentio
     if (p.query_heads <= 0 || p.query_heads > 1024 || p.query_heads % c.heads) return "heads";
     if (p.longest <= 0 || p.longest > kMostTokens - 4096 || p.longest > (int64_t)p.row_pages * c.page_tokens)
         return "length";
-    if (!std::isfinite(p.scale)) return "scale";
+    if (!std::isfinite(p.scale * kLog2E)) return "scale";
     for (const int64_t s : {p.q_stride, p.y_stride})
         if (s < (int64_t)p.query_heads * c.width || s > kMostStride) return "stride";
     return "";

@@ -145,6 +145,8 @@ int kk_i8_quantize(const float *x, int k, int batch, void *workspace, int *statu
 int kk_i8_matmul(const void *workspace, const int8_t *w, const float *scales, const float *maxima,
                  float *y, int k, int n, int batch, hipStream_t stream, const char **route);
 
+// log2(e): the attention's scores are kept in base 2.
+constexpr float kLog2E = 1.44269504088896340736f;
 // Attention of one new token per sequence over a paged cache (k200.h). The
 // workspace (kk_paged_attention_workspace_bytes, may be 0) holds the sums of
 // sequences split over several workgroups.

@@ -1085,7 +1085,7 @@ extern "C" int kk_paged_attention(void *y, const void *q, const void *k, const v
     a.chunks = r.chunks;
     a.f16 = p.type == kunlun::InputType::f16;
     a.q_wide = (uintptr_t)q % 16 == 0 && p.q_stride % (a.f16 ? 8 : 4) == 0;
-    a.scale_log2 = p.scale * 1.44269504088896340736f;
+    a.scale_log2 = p.scale * kLog2E;
     hipError_t rc;
     if (c.width <= 64) rc = launch_width<2, 4>(a, r, p.sequences, c.heads, stream);
     else if (c.width <= 96) rc = launch_width<3, 8>(a, r, p.sequences, c.heads, stream);
