@@ -396,7 +396,7 @@ const char * kv_cache_reason(const KVCacheLayout &);
 
 // What the kernels met on `device` since the last call, completing its work
 // first: 0, or a sum of 1 (a page id outside the pool; its tokens were left out),
-// 2 (a sequence, position or length out of range; left out or cut) and 4 (no
+// 2 (a sequence, position or length out of range, or a second entry for one sequence; left out or cut) and 4 (no
 // free page: the sequence kept its length, a fork's child is empty). -1: no such device.
 int kv_cache_status(int device);
 

@@ -2,11 +2,11 @@
 // by reference counts.
 //
 // What has to be decided in order (which free page goes to which sequence, which page
-// moves where) is decided by one workgroup with prefix sums over the reference
-// counts, in the order of page numbers and of the caller's list, so that the
-// same calls give the same tables every time; counts themselves change by
-// integer atomics. What moves data (rows, pages) follows in a second launch over the
-// whole card and is bound by the bytes it copies.
+// moves where, which of two entries that name one sequence counts) is decided by prefix sums over the reference
+// counts and by the lowest place in the caller's list, in the order of page numbers and of that list, so that the
+// same calls give the same tables every time: one workgroup for reservations and forks, one a tile of pages for the
+// compaction. Counts themselves change by integer atomics. What moves data (rows, pages) follows in a second launch over
+// the whole card and is bound by the bytes it copies.
 #include "device_common.h"
 #include "launch.h"
 #include "paged.h"
@@ -127,7 +127,7 @@ __device__ __forceinline__ void release_row(const PagesArgs &a, const int *row, 
 }
 
 // Which entry of a list counts for the sequence it names: the first of those that claim it. Claims stand in LDS
-// where the table has few sequences, else in the workspace.
+// where the table has few sequences, else in the workspace (by LDS instructions instead of flat ones they take as long).
 constexpr int kNearClaims = 4096;
 
 __device__ __forceinline__ int *cleared_claims(int *near, int *far, int sequences, const int *list, int count) {

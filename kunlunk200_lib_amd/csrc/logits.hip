@@ -5,7 +5,8 @@
 // A workgroup takes a slice of one row, 4 * VPT logits a thread, which are on their
 // way first. Meanwhile it counts the row's history and finds the last bias entry
 // of each token in LDS words of its own slice, by integer atomics, whose order
-// does not matter. Each slice reads the row's lists (from the L2 after the first).
+// does not matter. Each slice reads the row's lists (from the L2 after the first)
+// and tests every entry: of 200 rows x 32000 with 3000 history entries and 300 biases, 15.9 us, that is 2.7.
 #include "device_common.h"
 #include "launch.h"
 #include "paged.h"
@@ -171,7 +172,7 @@ extern "C" int kk_process_logits(float *y, const float *logits, const float *pen
                        p.logits_stride, p.y_stride, p.history_stride, p.bias_stride, p.mask_stride, status, p.vocabulary};
     const bool vec = ((uintptr_t)y | (uintptr_t)logits) % 16 == 0 && (p.logits_stride | p.y_stride) % 4 == 0;
     // larger slices read the lists less often, smaller ones leave no CU idle: 200 rows x 32000, history 3000: slices of
-    // 4096 logits 20.1 us, 2048 16.5, 1024 16.7; up to 64 rows they are equal
+    // 4096 logits 20.3 us, 2048 15.9, 1024 16.6; up to 64 rows they are equal
     const int64_t logits_of_call = (int64_t)p.rows * p.vocabulary;
     if (logits_of_call >= (int64_t)slice_of(2) * 4 * cus) launch<2>(a, p.rows, vec, stream);
     else launch<1>(a, p.rows, vec, stream);

@@ -21,18 +21,19 @@
 // into fp16 parts x = hi + lo (hi 11 bits, lo the next 11), hi in column c and lo in
 // column c + 8 of one tile; the two columns' sums are added at the end. So F32
 // queries and weights cost no instruction more than F16 ones with 8 query heads
-// or fewer, and errors stay at 2^-22 (against 64 bits 1.4e-7 relative over 4096 tokens, where
-// products in F32 one by one leave 2.4e-7). q is scaled by a power of two
-// (max |q| in [2^10, 2^11)) and the weights by 2^14, so that what the low
-// parts lose below 2^-24 stays far below that.
+// or fewer, and errors stay at 2^-22 (against 64 bits 1.0e-7 relative over 4096 tokens, where
+// products in F32 one by one leave 2.0e-7). q is scaled by a power of two
+// (max |scale q| in [2^9, 2^11)) and the weights by 2^14, so that what the low
+// parts lose below 2^-24 stays far below that. Where a factor is not 0 its high part is not either, so that infinite
+// keys and values meet it as they would an F32 number.
 //
 // What bounds it: reading the cache (4 * width bytes per token and head). A step's K rows
 // are reloaded behind its scores and its V rows behind its second product, so a wave has 8
 // to 16 KiB on their way at any time, three workgroups to a CU; one sequence of 32768 tokens x 8 heads takes
-// 24.5 us (5.5 TB/s) and 4.5 for the join. Long ragged rows go to attend_even, below: 32 sequences of up to
-// 4096 tokens x 32 heads of 128 (1.2 GB) 180..185 us, 6.6 TB/s, what a kernel that only reads reaches. Below some
+// 24.6 us (5.5 TB/s) and 4.6 for the join. Long ragged rows go to attend_even, below: 32 sequences of up to
+// 4096 tokens x 32 heads of 128 (1.2 GB) 183 us, 6.6 TB/s, what a kernel that only reads reaches. Below some
 // ten MB it is the chain of latencies (length and pages, rows, two products, the waves' sums): 33 tokens x 32 heads
-// 5.6 us of kernel.
+// 5.9 us of kernel.
 //
 // Sequences of more than one chunk leave (sum w v, m, sum w) per chunk in the
 // workspace; a second launch joins them in order, so results do not
@@ -291,8 +292,9 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
     }
     // Workgroups also go round the CUs, wherever one has room: parts that are there first (part number slowest: those
     // past a sequence's end come last and at once), and sequences turned within each eight, so that long and
-    // short ones that take turns do not meet on the same CUs (sequences of 1000 tokens where `longest` is 32768: 121 us in
-    // order of sequences, 48 so; 64 x 8 heads ragged to 2048, every other one long: 70, in order 83, turned 63)
+    // short ones that take turns do not meet on the same CUs (64 sequences of 1000 tokens x 6 heads where
+    // `longest` is 32768: 41 us, in order of sequences and their parts 54; 96 x 8 heads of 80, every other one of 2048 tokens,
+    // the rest of half as many at most: 70, in that order 72, not turned 83)
     const int eight = s / 8, first_of = eight * 8, size = min(8, static_cast<int>(gridDim.y) - first_of);
     s = first_of + (s - first_of + eight + eight / 4 + chunk) % size;
     const int head0 = kvh * a.group + tile * 8 * NT;                        // first query head
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
 #pragma unroll
             for (int part = 0; part < VW / VP; ++part) {
                 // a column past the width gives values past it, which are not stored: any part of the row will do (zeros
-                // in its place make the wave wait for the row here: 64 x 1024 tokens x 8 heads of 80 36.4 us, with them 38.4)
+                // in its place make the wave wait for the row here: 64 x 1024 tokens x 8 heads of 80 34.6 us, with them 2 more)
                 const int col = part * 128 + c * VP;
                 const bool in = (FULL && 16 * VW == 32 * D32) || col < width;
                 const _Float16 *p = UNI ? v_head + w.at[i / 4] + (i & 3) * a.pool.token_stride + (v_lane + (in ? col : 0))
@@ -622,11 +624,11 @@ __device__ __forceinline__ Share share_of(const AttendArgs &a, int number, int f
 
 // The same sums by one workgroup to a CU (width 64: two), each an equal share of the steps of all rows. Its waves take four
 // neighbouring key-value heads, so that what it reads lies together in either order within a page (64 x 4096 tokens x 8
-// heads, token by token: 200 us by `attend`, 5.4 TB/s; 174 so, 6.2), and a wave's sums are its head's: no barrier, no LDS.
-// Four waves with a step on its way each keep up with the memory (two workgroups to a CU: 172 for 169 with 64 x 4096 head by
-// head; width 64: 92 for 98). A new row costs a chain of latencies - length, page, rows - of some 4 us: the next row is
+// heads, token by token: 195 us by `attend`, 5.5 TB/s; 168 so, 6.4), and a wave's sums are its head's: no barrier, no LDS.
+// Four waves with a step on its way each keep up with the memory (two workgroups to a CU: 172 for 165 with 64 x 4096 head by
+// head; width 64: 91 for 95). A new row costs a chain of latencies - length, page, rows - of some 4 us: the next row is
 // looked up while this one's first rows are on their way, its first rows are asked for behind this one's last scores, and
-// beginning it counts as a step of a share (64 sequences ragged to 2048 x 8 heads: 63 us without all that, 58 with; `attend` 66).
+// beginning it counts as a step of a share (64 sequences ragged to 2048 x 8 heads: 63 us without all that, 58 with).
 template <int D32, int VW>
 __global__ __launch_bounds__(kThreads, 1) void attend_even(AttendArgs a) {
     constexpr int VP = VW < 8 ? VW : 8, VR = VW / 2, width = 32 * D32;
@@ -939,20 +941,20 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
     // No split, so no second launch: eight waves to a workgroup for rows of up to 512 tokens, or 1024 where they
-    // leave few CUs idle, four for more rows of up to 512 (us, against the split: 4 x 160 / 320 / 512 tokens x 8 heads
-    // 7.2 / 8.0 / 9.1, split 10.3 / 10.5 / 10.6; eight waves at 768 12.3, split 11.8; 32 x 512 / 1024 x 8 heads
-    // 14.2 / 28.3, split 18.7 / 29.9).
+    // leave few CUs idle, four for more rows of up to 512 (us, against the split or shares: 4 x 160 / 320 / 512 tokens x 8
+    // heads 7.8 / 8.6 / 9.6, split 11.1 / 11.2 / 11.5; eight waves at 768 12.6, split 11.5; 32 x 512 / 1024 x 8 heads
+    // 13.8 / 26.8, split 18.4, shares 30.8).
     const int whole = kMaxChunk + kStep;             // a window starts up to kStep - 1 tokens early
     r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
              longest <= (rows > cus / 2 ? 2 * whole : whole);
     const int64_t least = r.wide ? longest : rows > cus && longest <= whole ? longest : kMinChunk;
-    // (The figures of parts of rows that attend_even takes now, below, are `attend`'s.)
     // Otherwise two workgroups' tokens to a CU, in parts of one size: of up to 512 tokens (1 x 32768 tokens x 8 heads
-    // 29.1 us, of 256 32.0); with two rows and more to a CU whole rows of up to 1024 (64 x 640 / 1024 tokens x 8 heads
-    // 30 / 46, in parts of 512 40 / 54) and, above, at least three parts of up to 1024 (64 x 8 heads ragged to 2048: two
-    // parts 64.7, three 61.9, four 61.1; all of 2048: 92.9, 94.0, 95.7); of workgroups that a CU holds one or two of
-    // instead of three, twice as many tokens (64 x 2048 x 8 heads of 256 175 whole, 204 in three parts; groups of 16 query
-    // heads 92 / 117).
+    // 29.3 us, of 256 32.2); with two rows and more to a CU whole rows of up to 1024 (64 x 640 / 1024 tokens x 8 heads
+    // 29.6 / 44, in shares 36 / 50) and, above, at least three parts of up to 1024, where shares do not take them (two parts,
+    // three, four: 64 x 2048 x 8 heads of 80 uniform 46.7, 44.6, 45.7, full 75.0, 70.7, 74.0; pages of 24 tokens 64.3,
+    // 61.4, 62.9 and 106.6, 107.7, 108.9; 96 x 2048 x 6 heads of 128 70.0, 67.9, 64.6 and 109.9, 107.7, 108.6); of
+    // workgroups that a CU holds one or two of instead of three, twice as many tokens (64 x 2048 x 8 heads of 160 143
+    // whole, 168 in three parts, uniform 114 and 104; groups of 16 query heads 94 and 119, 68 and 72).
     const int many = c.width > 128 || r.nt == 2 ? 2 * kMaxChunkMany : kMaxChunkMany;
     const int64_t most = rows >= 2 * cus ? many : kMaxChunk;
     const int64_t wanted = std::min<int64_t>((longest * rows + 2 * cus - 1) / (2 * cus), most);
@@ -966,24 +968,24 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int64_t parts = std::max(std::min(asked, most_parts), id_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
-    // One wave to a workgroup for many rows of up to four steps (512 sequences x 8 heads: 2 / 64 / 128 tokens 32 / 41 / 59 us
-    // on four waves, 17 / 32 / 55 on one, 256 tokens 97 / 102; 64 x 8: 128 tokens 10.6 / 11.2; width 256, 60 x 64 tokens x 32
-    // heads 61 / 35)
+    // One wave to a workgroup for many rows of up to four steps (512 sequences x 8 heads: 2 / 64 / 128 tokens 31 / 40 / 55 us
+    // on four waves, 17 / 33 / 54 on one, 256 tokens 97 / 100; 64 x 8: 128 tokens 10.4 / 11.3; width 256, 60 x 64 tokens x 32
+    // heads 60 / 32)
     r.narrow = r.nt == 1 && rows > 2 * cus && longest <= 4 * kStep;
     // The non-temporal hint, for reads of whole cache lines that fill more than a quarter of the 256 MiB cache with
-    // nothing that is read again (us by `attend`, with the hint and without: 32 x 4096 tokens x 32 heads 196 / 218; 64 x 4096 x 8 in
-    // token order 198 / 207; 64 x 1024 x 8 of 64 25.4 / 28.3; 16 x 1024 x 8, 67 MB, 20.1 / 18.9; tiles that read the same
-    // rows, 32 query heads on one, 107 / 96; rows that share lines, 64 x 1024 x 8 of 80, 40.5 / 38.4).
+    // nothing that is read again (us by `attend`, with the hint and without: 64 x 1024 x 8 heads 44 / 50; 96 x 2048 x 6 104 /
+    // 117, in token order 111 / 119; 64 x 1024 x 8 of 64 24.7 / 27.1; 16 x 1024 x 8, 67 MB, 20.0 / 18.4; tiles that read the
+    // same rows, 256 x 2048 with 32 query heads on one, 79 / 65; rows that share lines, 64 x 1024 x 8 of 80, 38.7 / 34.6).
     r.once = r.tiles == 1 && (int64_t)p.sequences * longest * c.heads * c.width * 4 > (64 << 20);
     // Equal shares where rows would be split and there is enough to read (us, by `attend` and in shares, 8 heads of 128, head by
-    // head / token by token: 64 sequences uniform to 1536 48 and 45 / 53 and 45, to 4096 110 and 97 / 121 and 99; 16 to
-    // 2048 25.4 and 20.9 / 27.8 and 21.3, all 2048 29.9 and 32.0 / 32.7 and 31.9; width 256, 16 to 16384 201 and 157; 1 x
-    // 131072 98 and 92). One sequence is even by itself, until the last round of its parts counts little (1 x 32768
-    // 30.5 and 31.8). Where `longest` is ten times the lengths the shares lose 2 to 5 us (64 to 153 of 1536: 12.7 and 17.3).
-    // Rows that one workgroup takes whole stay with it (64 x 1024 47 and 52, uniform to 1024 35 and 37), unless they lie
-    // token by token (256 x 1024 190 and 177, uniform 119 and 109; to 768 even) or few workgroups fit on a CU (width
-    // 256, 64 uniform to 768 / 2048 55 and 49 / 129 and 103; width 192 44 and 43 / 105 and 87, all 2048 138 and 141; 256
-    // uniform to 512 99 and 102).
+    // head / token by token: 64 sequences uniform to 1536 48 and 43 / 52 and 43, to 4096 98 and 88 / 115 and 91; 16 to
+    // 2048 24.6 and 21.1 / 26.6 and 20.8, all 2048 29.7 and 31.9 / 32.2 and 32.1; width 256, 16 to 16384 202 and 150; 1 x
+    // 131072 94 and 88). One sequence is even by itself, until the last round of its parts counts little (1 x 32768
+    // 29.2 and 31.1). Where `longest` is far above the lengths the shares lose 3 to 4 us (64 to 153 of 1536: 13.0 and 16.4;
+    // 64 of 1000, of 32768: 48 and 52). Rows that one workgroup takes whole stay with it (64 x 1024 44 and 50, uniform to
+    // 1024 33 and 35), unless they lie token by token (256 x 1024 190 and 170, uniform 118 and 107, 64 x 1024 50 and 51, 37
+    // and 35) or few workgroups fit on a CU (width 256, 64 uniform to 768 / 2048 56 and 50 / 126 and 94; width 192 43 and 45
+    // / 97 and 83, all 2048 132 and 138).
     const bool together = c.head_stride < c.token_stride;
     const bool share_whole = !r.wide && (c.width > 128 ? longest > kMaxChunk : together && longest > 6 * kMinChunk);
     r.shares = 0;
