@@ -674,7 +674,8 @@ class KVPagesLayout(ctypes.Structure):
 
 
 class LogitsLayout(ctypes.Structure):
-    """One process_logits call; strides are elements between rows (mask_stride 0: one mask for all rows)."""
+    """One process_logits call; strides are elements between rows (mask_stride 0: one mask for all rows;
+    history_stride and bias_stride are the given lists' room, above 0)."""
     _fields_ = _fields("rows", "vocabulary", "logits_stride", "y_stride", "history_stride", "bias_stride",
                        "mask_stride", logits_stride=ctypes.c_int64, y_stride=ctypes.c_int64,
                        history_stride=ctypes.c_int64, bias_stride=ctypes.c_int64, mask_stride=ctypes.c_int64)
@@ -728,7 +729,8 @@ def kv_append(kernel: Kernel, device: int, k_pool, v_pool, q_out, q, k, v, seque
 
 def kv_reserve(kernel: Kernel, device: int, table, lengths, references, rows, added, count: int,
                cache: KVCacheLayout, pages: KVPagesLayout) -> bool:
-    """Submit: room for added[i] more tokens of sequence rows[i], on the lowest free pages."""
+    """Submit: room for added[i] more tokens of sequence rows[i], on the lowest free pages, in list order
+    (an entry whose pages are not there takes none from those after it)."""
     return bool(load().kunlun_kv_reserve(kernel.handle, int(device), _ptr(table), _ptr(lengths), _ptr(references),
                                          _ptr(rows), _ptr(added), int(count), ctypes.byref(cache),
                                          ctypes.byref(pages)))
