@@ -74,6 +74,8 @@ struct KVPagesLayout;
 struct KVAppendLayout;
 struct PagedAttentionLayout;
 struct LogitsLayout;
+struct KVCacheF8Layout;
+struct KVReadLayout;
 
 // Per-call state owner: binds to the first device it is used on and owns
 // lazily grown device workspaces (reference k200.h:62-88).
@@ -109,6 +111,21 @@ private:
                            const int *, const KVCacheLayout &, const KVPagesLayout &);
     friend bool kv_copy_pages(Kernel &, int, void *, void *, const int *, const int *, int, const KVCacheLayout &,
                               const KVPagesLayout &);
+    friend bool paged_attention_f8(Kernel &, int, void *, const void *, const void *, const void *, const float *,
+                                   const float *, const int *, const int *, const KVCacheF8Layout &,
+                                   const PagedAttentionLayout &);
+    friend bool kv_append_f8(Kernel &, int, void *, void *, float *, float *, void *, const void *, const void *,
+                             const void *, const int *, const int *, const int *, const int *, const float *,
+                             const float *, const KVCacheF8Layout &, const KVAppendLayout &);
+    friend bool kv_read_f8(Kernel &, int, void *, void *, const void *, const void *, const float *, const float *,
+                           const int *, const int *, const int *, const int *, const KVCacheF8Layout &,
+                           const KVReadLayout &);
+    friend bool kv_fork_f8(Kernel &, int, void *, void *, float *, float *, int *, int *, int *, const int *, const int *,
+                           int, const KVCacheF8Layout &, const KVPagesLayout &);
+    friend bool kv_compact_f8(Kernel &, int, void *, void *, float *, float *, int *, int *, int *, const int *,
+                              const int *, const int *, const KVCacheF8Layout &, const KVPagesLayout &);
+    friend bool kv_copy_pages_f8(Kernel &, int, void *, void *, float *, float *, const int *, const int *, int,
+                                 const KVCacheF8Layout &, const KVPagesLayout &);
     friend bool process_logits(Kernel &, int, void *, const void *, const float *, const int *, const int *,
                                const int *, const float *, const int *, const uint32_t *, const LogitsLayout &);
 };
@@ -486,6 +503,67 @@ bool kv_compact(Kernel &, int device, void * k, void * v, int * table_out, int *
 // entry are left out). No destination may be named twice or be a source.
 bool kv_copy_pages(Kernel &, int device, void * k, void * v, const int * sources, const int * destinations,
                    int count, const KVCacheLayout &, const KVPagesLayout &);
+
+// The same cache in 8 bits. A pool holds e4m3 codes (4 exponent and 3 mantissa bits, largest 448), a byte each, at the
+// places that `cache` names for values. Beside it stands an F32 scale for every block_tokens tokens of a head:
+// token t of head h of page p has scale [(p * heads + h) * (page_tokens / block_tokens) + t / block_tokens], and a value is its
+// code times its scale. block_tokens is a power of two up to 64 that divides page_tokens. Pools are 16-byte, scales
+// 4-byte aligned. Tables, lengths and counts are those of the F16 cache, with kv_reserve(cache) and kv_free(cache).
+struct KVCacheF8Layout {
+    KVCacheLayout cache;
+    int block_tokens;
+};
+// "" or the first rule broken: those of kv_cache_reason, "block".
+const char * kv_cache_f8_reason(const KVCacheF8Layout &);
+
+// paged_attention over such a cache, with its rules and numerics: products run on the codes, which F16 holds exactly; a
+// token's key scale multiplies its score, its value scale its weight, in F32, and the product of weight and value
+// scale is held to 2^-22 of itself or 2^-39 of the largest one. Any finite F32 scales will do. A scale or a code that is not
+// a number makes the rows that read it not a number. What stands past a row's length or before its window may be anything.
+const char * paged_attention_f8_reason(const KVCacheF8Layout &, const PagedAttentionLayout &);
+bool paged_attention_f8(Kernel &, int device, void * y, const void * q, const void * k, const void * v,
+                        const float * k_scales, const float * v_scales, const int * table, const int * lengths,
+                        const KVCacheF8Layout &, const PagedAttentionLayout &);
+
+// kv_append into such a cache: the same arguments, rules and rows of q. A block's scale becomes the least power of
+// two, 2^-64 or more, that takes the largest of its new tokens' values to at most 448, or what it was where the block
+// holds earlier tokens and their scale is larger; where it grows, the earlier tokens' codes are rounded to the new one.
+// A new value is rounded once, to the nearest code of its F64 rotation (ties to the even code). A value that is not finite
+// makes its block's scale, so all of the block, not a number, until the block is begun again. Tokens of one block must
+// be consecutive entries of rising positions; what the block held from the first of them on is forgotten.
+// Up to 2^31 threads: (query_heads * width / 8 + 512 * heads) * tokens.
+const char * kv_append_f8_reason(const KVCacheF8Layout &, const KVAppendLayout &);
+bool kv_append_f8(Kernel &, int device, void * k_pool, void * v_pool, float * k_scales, float * v_scales, void * q_out,
+                  const void * q, const void * k, const void * v, const int * sequence, const int * position,
+                  const int * lengths, const int * table, const float * cosine, const float * sine,
+                  const KVCacheF8Layout &, const KVAppendLayout &);
+
+// Reads tokens back: row i of k and v (rows of [heads][width] values of `type`, *_stride elements apart, of their own or
+// side by side in common rows) becomes token position[i] of sequence[i], code times scale, rounded once where `type` is F16.
+// Tokens are named as for kv_append (position null: the newest of each sequence), in any order; those left out, out of
+// range or without a page leave their rows as they were, the latter two reported.
+struct KVReadLayout {
+    int tokens, sequences, row_pages;
+    int64_t k_stride, v_stride;
+    InputType type;
+};
+const char * kv_read_f8_reason(const KVCacheF8Layout &, const KVReadLayout &);
+bool kv_read_f8(Kernel &, int device, void * k, void * v, const void * k_pool, const void * v_pool,
+                const float * k_scales, const float * v_scales, const int * sequence, const int * position,
+                const int * lengths, const int * table, const KVCacheF8Layout &, const KVReadLayout &);
+
+// kv_fork, kv_compact and kv_copy_pages for such a cache: pages move with their scales. layer_stride counts codes; the
+// layers' scales follow one another, pages * heads * (page_tokens / block_tokens) each. The first rule broken is one of
+// kv_cache_f8_reason or kv_pages_reason.
+const char * kv_pages_f8_reason(const KVCacheF8Layout &, const KVPagesLayout &);
+bool kv_fork_f8(Kernel &, int device, void * k, void * v, float * k_scales, float * v_scales, int * table, int * lengths,
+                int * references, const int * parents, const int * children, int count, const KVCacheF8Layout &,
+                const KVPagesLayout &);
+bool kv_compact_f8(Kernel &, int device, void * k, void * v, float * k_scales, float * v_scales, int * table_out,
+                   int * references_out, int * used, const int * table, const int * lengths, const int * references,
+                   const KVCacheF8Layout &, const KVPagesLayout &);
+bool kv_copy_pages_f8(Kernel &, int device, void * k, void * v, float * k_scales, float * v_scales, const int * sources,
+                      const int * destinations, int count, const KVCacheF8Layout &, const KVPagesLayout &);
 
 // Logits before a token is chosen, F32, row by row: with n the times that token t
 // stands among the row's first history_lengths[row] history entries and

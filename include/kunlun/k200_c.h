@@ -308,6 +308,44 @@ int kunlun_process_logits(kunlun_kernel *kernel, int device, void *y, const void
                           const float *bias_values, const int *bias_lengths, const uint32_t *mask,
                           const kunlun_logits_layout *call);
 
+/* The cache in 8 bits (kunlun::KVCacheF8Layout, KVReadLayout and the functions of the same names). */
+typedef struct {
+    kunlun_kv_cache_layout cache;
+    int block_tokens;
+} kunlun_kv_cache_f8_layout;
+typedef struct {
+    int tokens, sequences, row_pages;
+    int64_t k_stride, v_stride;
+    int type;
+} kunlun_kv_read_layout;
+const char *kunlun_kv_cache_f8_reason(const kunlun_kv_cache_f8_layout *cache);
+const char *kunlun_paged_attention_f8_reason(const kunlun_kv_cache_f8_layout *cache,
+                                             const kunlun_paged_attention_layout *call);
+const char *kunlun_kv_append_f8_reason(const kunlun_kv_cache_f8_layout *cache, const kunlun_kv_append_layout *call);
+const char *kunlun_kv_read_f8_reason(const kunlun_kv_cache_f8_layout *cache, const kunlun_kv_read_layout *call);
+const char *kunlun_kv_pages_f8_reason(const kunlun_kv_cache_f8_layout *cache, const kunlun_kv_pages_layout *pages);
+int kunlun_paged_attention_f8(kunlun_kernel *kernel, int device, void *y, const void *q, const void *k, const void *v,
+                              const float *k_scales, const float *v_scales, const int *table, const int *lengths,
+                              const kunlun_kv_cache_f8_layout *cache, const kunlun_paged_attention_layout *call);
+int kunlun_kv_append_f8(kunlun_kernel *kernel, int device, void *k_pool, void *v_pool, float *k_scales, float *v_scales,
+                        void *q_out, const void *q, const void *k, const void *v, const int *sequence,
+                        const int *position, const int *lengths, const int *table, const float *cosine,
+                        const float *sine, const kunlun_kv_cache_f8_layout *cache, const kunlun_kv_append_layout *call);
+int kunlun_kv_read_f8(kunlun_kernel *kernel, int device, void *k, void *v, const void *k_pool, const void *v_pool,
+                      const float *k_scales, const float *v_scales, const int *sequence, const int *position,
+                      const int *lengths, const int *table, const kunlun_kv_cache_f8_layout *cache,
+                      const kunlun_kv_read_layout *call);
+int kunlun_kv_fork_f8(kunlun_kernel *kernel, int device, void *k, void *v, float *k_scales, float *v_scales, int *table,
+                      int *lengths, int *references, const int *parents, const int *children, int count,
+                      const kunlun_kv_cache_f8_layout *cache, const kunlun_kv_pages_layout *pages);
+int kunlun_kv_compact_f8(kunlun_kernel *kernel, int device, void *k, void *v, float *k_scales, float *v_scales,
+                         int *table_out, int *references_out, int *used, const int *table, const int *lengths,
+                         const int *references, const kunlun_kv_cache_f8_layout *cache,
+                         const kunlun_kv_pages_layout *pages);
+int kunlun_kv_copy_pages_f8(kunlun_kernel *kernel, int device, void *k, void *v, float *k_scales, float *v_scales,
+                            const int *sources, const int *destinations, int count,
+                            const kunlun_kv_cache_f8_layout *cache, const kunlun_kv_pages_layout *pages);
+
 #ifdef __cplusplus
 }
 #endif

@@ -128,6 +128,17 @@ C_FUNCTIONS = [
     ("kunlun_kv_compact", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 10),
     ("kunlun_kv_copy_pages", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] + [_c_void_p] * 2),
     ("kunlun_process_logits", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 10),
+    ("kunlun_kv_cache_f8_reason", ctypes.c_char_p, [_c_void_p]),
+    ("kunlun_paged_attention_f8_reason", ctypes.c_char_p, [_c_void_p, _c_void_p]),
+    ("kunlun_kv_append_f8_reason", ctypes.c_char_p, [_c_void_p, _c_void_p]),
+    ("kunlun_kv_read_f8_reason", ctypes.c_char_p, [_c_void_p, _c_void_p]),
+    ("kunlun_kv_pages_f8_reason", ctypes.c_char_p, [_c_void_p, _c_void_p]),
+    ("kunlun_paged_attention_f8", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 10),
+    ("kunlun_kv_append_f8", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 16),
+    ("kunlun_kv_read_f8", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 12),
+    ("kunlun_kv_fork_f8", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 9 + [_c_int] + [_c_void_p] * 2),
+    ("kunlun_kv_compact_f8", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 12),
+    ("kunlun_kv_copy_pages_f8", _c_int, [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] + [_c_void_p] * 2),
 ]
 
 
@@ -681,6 +692,18 @@ class LogitsLayout(ctypes.Structure):
                        history_stride=ctypes.c_int64, bias_stride=ctypes.c_int64, mask_stride=ctypes.c_int64)
 
 
+class KVCacheF8Layout(ctypes.Structure):
+    """8-bit pools: e4m3 codes at the places that `cache` names for values, a byte each, and F32 scales
+    [pages][heads][page_tokens / block_tokens] beside them (include/kunlun/k200.h)."""
+    _fields_ = _fields("cache", "block_tokens", cache=KVCacheLayout)
+
+
+class KVReadLayout(ctypes.Structure):
+    """One kv_read_f8 call; strides are elements between tokens, type an InputType."""
+    _fields_ = _fields("tokens", "sequences", "row_pages", "k_stride", "v_stride", "type", k_stride=ctypes.c_int64,
+                       v_stride=ctypes.c_int64)
+
+
 KV_BAD_PAGE, KV_BAD_INDEX, KV_NO_PAGE = 1, 2, 4
 
 
@@ -765,6 +788,78 @@ def kv_copy_pages(kernel: Kernel, device: int, k, v, sources, destinations, coun
     return bool(load().kunlun_kv_copy_pages(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(sources),
                                             _ptr(destinations), int(count), ctypes.byref(cache),
                                             ctypes.byref(pages)))
+
+
+def kv_cache_f8_reason(cache: KVCacheF8Layout) -> str:
+    return load().kunlun_kv_cache_f8_reason(ctypes.byref(cache)).decode()
+
+
+def paged_attention_f8_reason(cache: KVCacheF8Layout, call: PagedAttentionLayout) -> str:
+    return load().kunlun_paged_attention_f8_reason(ctypes.byref(cache), ctypes.byref(call)).decode()
+
+
+def kv_append_f8_reason(cache: KVCacheF8Layout, call: KVAppendLayout) -> str:
+    return load().kunlun_kv_append_f8_reason(ctypes.byref(cache), ctypes.byref(call)).decode()
+
+
+def kv_read_f8_reason(cache: KVCacheF8Layout, call: KVReadLayout) -> str:
+    return load().kunlun_kv_read_f8_reason(ctypes.byref(cache), ctypes.byref(call)).decode()
+
+
+def kv_pages_f8_reason(cache: KVCacheF8Layout, pages: KVPagesLayout) -> str:
+    return load().kunlun_kv_pages_f8_reason(ctypes.byref(cache), ctypes.byref(pages)).decode()
+
+
+def paged_attention_f8(kernel: Kernel, device: int, y, q, k, v, k_scales, v_scales, table, lengths,
+                       cache: KVCacheF8Layout, call: PagedAttentionLayout) -> bool:
+    """Submit the attention of one new token per sequence over its pages of an 8-bit cache; False when
+    the arguments break a rule (paged_attention_f8_reason names the layouts')."""
+    return bool(load().kunlun_paged_attention_f8(kernel.handle, int(device), _ptr(y), _ptr(q), _ptr(k), _ptr(v),
+                                                 _ptr(k_scales), _ptr(v_scales), _ptr(table), _ptr(lengths),
+                                                 ctypes.byref(cache), ctypes.byref(call)))
+
+
+def kv_append_f8(kernel: Kernel, device: int, k_pool, v_pool, k_scales, v_scales, q_out, q, k, v, sequence, position,
+                 lengths, table, cosine, sine, cache: KVCacheF8Layout, call: KVAppendLayout) -> bool:
+    """Submit new tokens: q and k turned by their positions' angles, k and v quantised into their pages
+    (tokens of one block in consecutive entries of rising positions)."""
+    return bool(load().kunlun_kv_append_f8(kernel.handle, int(device), _ptr(k_pool), _ptr(v_pool), _ptr(k_scales),
+                                           _ptr(v_scales), _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(sequence),
+                                           _ptr(position), _ptr(lengths), _ptr(table), _ptr(cosine), _ptr(sine),
+                                           ctypes.byref(cache), ctypes.byref(call)))
+
+
+def kv_read_f8(kernel: Kernel, device: int, k, v, k_pool, v_pool, k_scales, v_scales, sequence, position, lengths,
+               table, cache: KVCacheF8Layout, call: KVReadLayout) -> bool:
+    """Submit: rows i of k and v become token position[i] of sequence[i], code times scale."""
+    return bool(load().kunlun_kv_read_f8(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(k_pool), _ptr(v_pool),
+                                         _ptr(k_scales), _ptr(v_scales), _ptr(sequence), _ptr(position),
+                                         _ptr(lengths), _ptr(table), ctypes.byref(cache), ctypes.byref(call)))
+
+
+def kv_fork_f8(kernel: Kernel, device: int, k, v, k_scales, v_scales, table, lengths, references, parents, children,
+               count: int, cache: KVCacheF8Layout, pages: KVPagesLayout) -> bool:
+    """kv_fork over 8-bit pools: the last page is copied with its scales."""
+    return bool(load().kunlun_kv_fork_f8(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(k_scales), _ptr(v_scales),
+                                         _ptr(table), _ptr(lengths), _ptr(references), _ptr(parents), _ptr(children),
+                                         int(count), ctypes.byref(cache), ctypes.byref(pages)))
+
+
+def kv_compact_f8(kernel: Kernel, device: int, k, v, k_scales, v_scales, table_out, references_out, used, table,
+                  lengths, references, cache: KVCacheF8Layout, pages: KVPagesLayout) -> bool:
+    """kv_compact over 8-bit pools: pages move with their scales."""
+    return bool(load().kunlun_kv_compact_f8(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(k_scales),
+                                            _ptr(v_scales), _ptr(table_out), _ptr(references_out), _ptr(used),
+                                            _ptr(table), _ptr(lengths), _ptr(references), ctypes.byref(cache),
+                                            ctypes.byref(pages)))
+
+
+def kv_copy_pages_f8(kernel: Kernel, device: int, k, v, k_scales, v_scales, sources, destinations, count: int,
+                     cache: KVCacheF8Layout, pages: KVPagesLayout) -> bool:
+    """kv_copy_pages over 8-bit pools: pages are copied with their scales."""
+    return bool(load().kunlun_kv_copy_pages_f8(kernel.handle, int(device), _ptr(k), _ptr(v), _ptr(k_scales),
+                                               _ptr(v_scales), _ptr(sources), _ptr(destinations), int(count),
+                                               ctypes.byref(cache), ctypes.byref(pages)))
 
 
 def process_logits(kernel: Kernel, device: int, y, logits, penalties, history, history_lengths, bias_ids,

@@ -46,6 +46,10 @@ kunlun::KVAppendLayout layout(const kunlun_kv_append_layout & p) {
 kunlun::KVPagesLayout layout(const kunlun_kv_pages_layout & p) {
     return {p.sequences, p.row_pages, p.layers, p.layer_stride};
 }
+kunlun::KVCacheF8Layout layout(const kunlun_kv_cache_f8_layout & c) { return {layout(c.cache), c.block_tokens}; }
+kunlun::KVReadLayout layout(const kunlun_kv_read_layout & p) {
+    return {p.tokens, p.sequences, p.row_pages, p.k_stride, p.v_stride, static_cast<kunlun::InputType>(p.type)};
+}
 kunlun::LogitsLayout layout(const kunlun_logits_layout & p) {
     return {p.rows, p.vocabulary, p.logits_stride, p.y_stride, p.history_stride, p.bias_stride, p.mask_stride};
 }
@@ -391,6 +395,71 @@ int kunlun_process_logits(kunlun_kernel * kernel, int device, void * y, const vo
     return kernel && call &&
            done(kernel, kunlun::process_logits(kernel->kernel, device, y, logits, penalties, history, history_lengths,
                                                bias_ids, bias_values, bias_lengths, mask, layout(*call)));
+}
+
+const char * kunlun_kv_cache_f8_reason(const kunlun_kv_cache_f8_layout * cache) {
+    return cache ? kunlun::kv_cache_f8_reason(layout(*cache)) : "shape";
+}
+const char * kunlun_paged_attention_f8_reason(const kunlun_kv_cache_f8_layout * cache,
+                                              const kunlun_paged_attention_layout * call) {
+    return cache && call ? kunlun::paged_attention_f8_reason(layout(*cache), layout(*call)) : "shape";
+}
+const char * kunlun_kv_append_f8_reason(const kunlun_kv_cache_f8_layout * cache, const kunlun_kv_append_layout * call) {
+    return cache && call ? kunlun::kv_append_f8_reason(layout(*cache), layout(*call)) : "shape";
+}
+const char * kunlun_kv_read_f8_reason(const kunlun_kv_cache_f8_layout * cache, const kunlun_kv_read_layout * call) {
+    return cache && call ? kunlun::kv_read_f8_reason(layout(*cache), layout(*call)) : "shape";
+}
+const char * kunlun_kv_pages_f8_reason(const kunlun_kv_cache_f8_layout * cache, const kunlun_kv_pages_layout * pages) {
+    return cache && pages ? kunlun::kv_pages_f8_reason(layout(*cache), layout(*pages)) : "shape";
+}
+int kunlun_paged_attention_f8(kunlun_kernel * kernel, int device, void * y, const void * q, const void * k,
+                              const void * v, const float * k_scales, const float * v_scales, const int * table,
+                              const int * lengths, const kunlun_kv_cache_f8_layout * cache,
+                              const kunlun_paged_attention_layout * call) {
+    return kernel && cache && call &&
+           done(kernel, kunlun::paged_attention_f8(kernel->kernel, device, y, q, k, v, k_scales, v_scales, table, lengths,
+                                                   layout(*cache), layout(*call)));
+}
+int kunlun_kv_append_f8(kunlun_kernel * kernel, int device, void * k_pool, void * v_pool, float * k_scales,
+                        float * v_scales, void * q_out, const void * q, const void * k, const void * v,
+                        const int * sequence, const int * position, const int * lengths, const int * table,
+                        const float * cosine, const float * sine, const kunlun_kv_cache_f8_layout * cache,
+                        const kunlun_kv_append_layout * call) {
+    return kernel && cache && call &&
+           done(kernel, kunlun::kv_append_f8(kernel->kernel, device, k_pool, v_pool, k_scales, v_scales, q_out, q, k, v,
+                                             sequence, position, lengths, table, cosine, sine, layout(*cache),
+                                             layout(*call)));
+}
+int kunlun_kv_read_f8(kunlun_kernel * kernel, int device, void * k, void * v, const void * k_pool, const void * v_pool,
+                      const float * k_scales, const float * v_scales, const int * sequence, const int * position,
+                      const int * lengths, const int * table, const kunlun_kv_cache_f8_layout * cache,
+                      const kunlun_kv_read_layout * call) {
+    return kernel && cache && call &&
+           done(kernel, kunlun::kv_read_f8(kernel->kernel, device, k, v, k_pool, v_pool, k_scales, v_scales, sequence,
+                                           position, lengths, table, layout(*cache), layout(*call)));
+}
+int kunlun_kv_fork_f8(kunlun_kernel * kernel, int device, void * k, void * v, float * k_scales, float * v_scales,
+                      int * table, int * lengths, int * references, const int * parents, const int * children, int count,
+                      const kunlun_kv_cache_f8_layout * cache, const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_fork_f8(kernel->kernel, device, k, v, k_scales, v_scales, table, lengths, references,
+                                           parents, children, count, layout(*cache), layout(*pages)));
+}
+int kunlun_kv_compact_f8(kunlun_kernel * kernel, int device, void * k, void * v, float * k_scales, float * v_scales,
+                         int * table_out, int * references_out, int * used, const int * table, const int * lengths,
+                         const int * references, const kunlun_kv_cache_f8_layout * cache,
+                         const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_compact_f8(kernel->kernel, device, k, v, k_scales, v_scales, table_out, references_out,
+                                              used, table, lengths, references, layout(*cache), layout(*pages)));
+}
+int kunlun_kv_copy_pages_f8(kunlun_kernel * kernel, int device, void * k, void * v, float * k_scales, float * v_scales,
+                            const int * sources, const int * destinations, int count,
+                            const kunlun_kv_cache_f8_layout * cache, const kunlun_kv_pages_layout * pages) {
+    return kernel && cache && pages &&
+           done(kernel, kunlun::kv_copy_pages_f8(kernel->kernel, device, k, v, k_scales, v_scales, sources, destinations,
+                                                 count, layout(*cache), layout(*pages)));
 }
 
 }

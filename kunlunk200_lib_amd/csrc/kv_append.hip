@@ -9,6 +9,7 @@
 // head rotated in halves, 4 of the first half and their 4 partners. Where rows,
 // strides or the tables' halves are off 4 values, every value is taken by itself.
 #include "device_common.h"
+#include "kv_rows.h"
 #include "launch.h"
 #include "paged.h"
 
@@ -32,24 +33,8 @@ struct AppendArgs {
     uint32_t units;                              // tokens x units of a token
 };
 
-template <typename T, int N>
-struct alignas(N * sizeof(T)) Pack {
-    T v[N];
-};
-
-template <typename T, int N>
-__device__ __forceinline__ void load_values(const T *from, float (&out)[8], int at) {
-    const Pack<T, N> p = *reinterpret_cast<const Pack<T, N> *>(from);
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[at + i] = static_cast<float>(p.v[i]);
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_values(T *to, const float (&x)[8], int at) {
-    Pack<T, N> p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) p.v[i] = static_cast<T>(x[at + i]);
-    *reinterpret_cast<Pack<T, N> *>(to) = p;
-}
+using kk::load_values;
+using kk::store_values;
 
 template <typename T, bool HALVES, bool VEC>
 __global__ __launch_bounds__(kThreads) void append(AppendArgs a) {

@@ -2,98 +2,14 @@
 // submission. None of them has a counterpart in the part of the reference's
 // header that this library keeps; they follow matmul in submitting without
 // waiting and swiglu in refusing arguments by their return value.
+#include "kv_rules.h"
 #include "launch.h"
-#include "runtime_internal.h"
 
-#include <algorithm>
 #include <cmath>
-#include <cstdint>
-#include <initializer_list>
 
 namespace kunlun {
 
-namespace {
-
-constexpr int64_t kMostStride = int64_t(1) << 40;        // elements
-constexpr int64_t kMostTokens = int64_t(1) << 27;        // of a sequence
-constexpr int kMostCounted = 1 << 30;                    // pages and sequences that 32-bit loops count in steps
-
-struct Span {
-    uintptr_t at;
-    size_t bytes;
-    Span(const void * p, size_t n) : at((uintptr_t)p), bytes(p ? n : 0) {}
-};
-
-bool clash(const Span & a, const Span & b) {
-    return a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes;
-}
-// Whether an output meets any of the others, or the others' list itself is out of range.
-bool clash(const Span & out, std::initializer_list<Span> others) {
-    for (const Span & s : others)
-        if (clash(out, s)) return true;
-    return false;
-}
-bool wraps(std::initializer_list<Span> spans) {
-    for (const Span & s : spans)
-        if (s.at + s.bytes < s.at) return true;
-    return false;
-}
-bool aligned_to(size_t bytes, std::initializer_list<const void *> pointers) {
-    for (const void * p : pointers)
-        if ((uintptr_t)p % bytes) return false;
-    return true;
-}
-
-int element_bytes(InputType type) { return type == InputType::f32 ? 4 : 2; }
-bool known(InputType type) { return type == InputType::f32 || type == InputType::f16; }
-
-// Elements from a pool's first value to its last, both included.
-int64_t pool_elements(const KVCacheLayout & c) {
-    return (c.pages - 1) * c.page_stride + (c.heads - 1) * c.head_stride + (c.page_tokens - 1) * c.token_stride + c.width;
-}
-Span pool_span(const void * pool, const KVCacheLayout & c) { return Span(pool, (size_t)pool_elements(c) * 2); }
-Span pool_span(const void * pool, const KVCacheLayout & c, const KVPagesLayout & p) {
-    return Span(pool, ((size_t)(p.layers - 1) * p.layer_stride + pool_elements(c)) * 2);
-}
-// Rows of `width` values of `bytes` each.
-Span rows_span(const void * first, int64_t rows, int64_t stride, int64_t width, int bytes) {
-    return Span(first, (size_t)((rows - 1) * stride + width) * bytes);
-}
-Span ints(const void * p, int64_t n) { return Span(p, (size_t)n * 4); }
-
-// The Kernel's device, or a visible one that the Kernel may be bound to.
-template <typename Impl>
-bool usable(const Impl & impl, int device) {
-    return detail::device_visible(device) && (impl.id == -1 || impl.id == device);
-}
-
-// The Kernel's workspace of the cache operators; nullptr when there is no memory for it.
-template <typename Impl>
-void * workspace(Impl & impl, int device, detail::DeviceContext & ctx, size_t need) {
-    if (impl.kv_workspace_size < need) {
-        if (impl.kv_workspace) {
-            detail::check_hip(hipStreamSynchronize(ctx.stream), "hipStreamSynchronize");
-            release(device, impl.kv_workspace, impl.kv_workspace_size);
-            impl.kv_workspace = nullptr;
-            impl.kv_workspace_size = 0;
-        }
-        // at least 1 MiB, so that a decode loop's growing lengths seldom get here
-        const size_t size = std::max<size_t>(need, size_t(1) << 20);
-        impl.kv_workspace = allocate(device, size);
-        if (!impl.kv_workspace) return nullptr;
-        impl.kv_workspace_size = size;
-    }
-    return impl.kv_workspace;
-}
-
-template <typename Impl>
-void note(Impl & impl, int device, const char * route) {
-    impl.id = device;
-    impl.route = route;
-    detail::note_route(route);
-}
-
-} // namespace
+using namespace rules;
 
 const char * kv_cache_reason(const KVCacheLayout & c) {
     if (c.pages <= 0 || c.page_tokens <= 0 || c.page_tokens > 65536 || c.heads <= 0 || c.heads > 1024 ||
@@ -127,19 +43,23 @@ const char * paged_attention_reason(const KVCacheLayout & c, const PagedAttentio
     return "";
 }
 
-bool paged_attention(Kernel & kernel, int id, void * y, const void * q, const void * k, const void * v,
-                     const int * table, const int * lengths, const KVCacheLayout & c,
-                     const PagedAttentionLayout & p) {
-    std::lock_guard<std::recursive_mutex> lock(detail::mutex());
-    if (*paged_attention_reason(c, p) || !y || !q || !k || !v || !table || !lengths) return false;
+bool rules::attention_ok(const void * y, const void * q, const Pools & pools, const int * table, const int * lengths,
+                         const KVCacheLayout & c, const PagedAttentionLayout & p) {
+    if (*paged_attention_reason(c, p) || !y || !q || !pools.given() || !table || !lengths) return false;
     const int bytes = element_bytes(p.type);
-    if (!aligned_to(bytes, {y, q}) || !aligned_to(16, {k, v}) || !aligned_to(4, {table, lengths})) return false;
+    if (!aligned_to(bytes, {y, q}) || !pools.aligned() || !aligned_to(4, {table, lengths})) return false;
     const int64_t row = (int64_t)p.query_heads * c.width;
     const Span out = rows_span(y, p.sequences, p.y_stride, row, bytes);
     const Span in = rows_span(q, p.sequences, p.q_stride, row, bytes);
     const Span rows = ints(table, (int64_t)p.sequences * p.row_pages), counts = ints(lengths, p.sequences);
-    const Span keys = pool_span(k, c), values = pool_span(v, c);
-    if (wraps({out, in, rows, counts, keys, values}) || clash(out, {in, rows, counts, keys, values})) return false;
+    return !wraps({out, in, rows, counts}) && !pools.wrap() && !clash(out, {in, rows, counts}) && !pools.meet(out);
+}
+
+bool paged_attention(Kernel & kernel, int id, void * y, const void * q, const void * k, const void * v,
+                     const int * table, const int * lengths, const KVCacheLayout & c,
+                     const PagedAttentionLayout & p) {
+    std::lock_guard<std::recursive_mutex> lock(detail::mutex());
+    if (*kv_cache_reason(c) || !attention_ok(y, q, Pools(k, v, c), table, lengths, c, p)) return false;
     Kernel::Impl & impl = *kernel.impl_;
     if (!usable(impl, id)) return false;
     detail::DeviceContext & ctx = detail::context(id);
@@ -172,24 +92,20 @@ const char * kv_append_reason(const KVCacheLayout & c, const KVAppendLayout & p)
     return "";
 }
 
-bool kv_append(Kernel & kernel, int id, void * k_pool, void * v_pool, void * q_out, const void * q, const void * k,
-               const void * v, const int * sequence, const int * position, const int * lengths, const int * table,
-               const float * cosine, const float * sine, const KVCacheLayout & c, const KVAppendLayout & given) {
-    std::lock_guard<std::recursive_mutex> lock(detail::mutex());
-    KVAppendLayout p = given;
-    if (!q) p.query_heads = 0;          // without queries their layout is ignored
-    if (*kv_append_reason(c, p) || !k_pool || !v_pool || !k || !v || !table) return false;
+bool rules::append_ok(const Pools & pools, const void * q_out, const void * q, const void * k, const void * v,
+                      const int * sequence, const int * position, const int * lengths, const int * table,
+                      const float * cosine, const float * sine, const KVCacheLayout & c, const KVAppendLayout & p) {
+    if (*kv_append_reason(c, p) || !pools.given() || !k || !v || !table) return false;
     const bool queries = q != nullptr;
     if (queries != (q_out != nullptr) || (queries && p.query_heads == 0)) return false;
     // a token's place: by position (with its sequence), or the newest of each sequence
     if (position ? !sequence : sequence || !lengths || p.tokens > p.sequences) return false;
     if (p.rotary > 0 && (!cosine || !sine)) return false;
     const int bytes = element_bytes(p.type);
-    if (!aligned_to(16, {k_pool, v_pool}) || !aligned_to(bytes, {q, q_out, k, v}) ||
+    if (!pools.aligned() || !aligned_to(bytes, {q, q_out, k, v}) ||
         !aligned_to(4, {sequence, position, lengths, table, cosine, sine}))
         return false;
     const int64_t row = (int64_t)c.heads * c.width, q_row = (int64_t)p.query_heads * c.width;
-    const Span keys = pool_span(k_pool, c), values = pool_span(v_pool, c);
     const Span k_in = rows_span(k, p.tokens, p.k_stride, row, bytes), v_in = rows_span(v, p.tokens, p.v_stride, row, bytes);
     const Span q_in = rows_span(q, p.tokens, p.q_stride, q_row, bytes);
     const Span out = rows_span(q_out, p.tokens, p.q_out_stride, q_row, bytes);
@@ -198,9 +114,8 @@ bool kv_append(Kernel & kernel, int id, void * k_pool, void * v_pool, void * q_o
     const Span at = ints(position, p.tokens), of = ints(sequence, p.tokens);
     const int64_t angles = p.rotary > 0 ? (int64_t)p.positions * (p.rotary / 2) : 0;
     const Span cosines = ints(cosine, angles), sines = ints(sine, angles);
-    if (wraps({keys, values, k_in, v_in, q_in, out, rows, counts, at, of, cosines, sines})) return false;
-    if (clash(keys, {values, k_in, v_in, q_in, out, rows, counts, at, of, cosines, sines}) ||
-        clash(values, {k_in, v_in, q_in, out, rows, counts, at, of, cosines, sines}) ||
+    if (wraps({k_in, v_in, q_in, out, rows, counts, at, of, cosines, sines}) || pools.wrap()) return false;
+    if (pools.meet_each_other() || pools.meet({k_in, v_in, q_in, out, rows, counts, at, of, cosines, sines}) ||
         clash(out, {rows, counts, at, of, cosines, sines}))
         return false;
     // q_out: q itself, rows of its own, or the q columns of rows that hold k and v too
@@ -214,7 +129,18 @@ bool kv_append(Kernel & kernel, int id, void * k_pool, void * v_pool, void * q_o
         const uintptr_t step = (uintptr_t)stride * bytes, delta = a > b ? a - b : b - a;
         return a > b ? delta >= row_bytes && delta + q_bytes <= step : delta >= q_bytes && delta + row_bytes <= step;
     };
-    if (queries && (!beside(k, p.k_stride) || !beside(v, p.v_stride))) return false;
+    return !queries || (beside(k, p.k_stride) && beside(v, p.v_stride));
+}
+
+bool kv_append(Kernel & kernel, int id, void * k_pool, void * v_pool, void * q_out, const void * q, const void * k,
+               const void * v, const int * sequence, const int * position, const int * lengths, const int * table,
+               const float * cosine, const float * sine, const KVCacheLayout & c, const KVAppendLayout & given) {
+    std::lock_guard<std::recursive_mutex> lock(detail::mutex());
+    KVAppendLayout p = given;
+    if (!q) p.query_heads = 0;          // without queries their layout is ignored
+    if (*kv_cache_reason(c) || !append_ok(Pools(k_pool, v_pool, c), q_out, q, k, v, sequence, position, lengths, table,
+                                          cosine, sine, c, p))
+        return false;
     Kernel::Impl & impl = *kernel.impl_;
     if (!usable(impl, id)) return false;
     detail::DeviceContext & ctx = detail::context(id);
@@ -237,26 +163,6 @@ const char * kv_pages_reason(const KVCacheLayout & c, const KVPagesLayout & p) {
     return "";
 }
 
-namespace {
-
-// The three arrays of a table, apart from each other and from `others`.
-struct TableSpans {
-    Span rows, lengths, references;
-    TableSpans(const void * table, const void * lengths_, const void * references_, const KVCacheLayout & c,
-               const KVPagesLayout & p)
-        : rows(ints(table, (int64_t)p.sequences * p.row_pages)), lengths(ints(lengths_, p.sequences)),
-          references(ints(references_, c.pages)) {}
-    bool bad(std::initializer_list<Span> others) const {
-        if (wraps({rows, lengths, references}) || wraps(others)) return true;
-        return clash(rows, {lengths, references}) || clash(lengths, {references}) || clash(rows, others) ||
-               clash(lengths, others) || clash(references, others);
-    }
-};
-
-bool list_ok(int count, int most) { return count > 0 && count <= most; }
-
-} // namespace
-
 bool kv_reserve(Kernel & kernel, int id, int * table, int * lengths, int * references, const int * rows,
                 const int * added, int count, const KVCacheLayout & c, const KVPagesLayout & p) {
     std::lock_guard<std::recursive_mutex> lock(detail::mutex());
@@ -276,17 +182,22 @@ bool kv_reserve(Kernel & kernel, int id, int * table, int * lengths, int * refer
     return true;
 }
 
+bool rules::fork_ok(const Pools & pools, const int * table, const int * lengths, const int * references,
+                    const int * parents, const int * children, int count, const KVCacheLayout & c, const KVPagesLayout & p) {
+    if (*kv_pages_reason(c, p) || !pools.given() || !table || !lengths || !references || !parents || !children ||
+        !list_ok(count, std::min(p.sequences, 65535)))
+        return false;
+    if (!pools.aligned() || !aligned_to(4, {table, lengths, references, parents, children})) return false;
+    const Span from = ints(parents, count), to = ints(children, count);
+    const TableSpans tables(table, lengths, references, c, p);
+    return !tables.bad({from, to}) && !pools.wrap() && !pools.meet_each_other() &&
+           !pools.meet({tables.rows, tables.lengths, tables.references, from, to});
+}
+
 bool kv_fork(Kernel & kernel, int id, void * k, void * v, int * table, int * lengths, int * references,
              const int * parents, const int * children, int count, const KVCacheLayout & c, const KVPagesLayout & p) {
     std::lock_guard<std::recursive_mutex> lock(detail::mutex());
-    if (*kv_pages_reason(c, p) || !k || !v || !table || !lengths || !references || !parents || !children ||
-        !list_ok(count, std::min(p.sequences, 65535)))
-        return false;
-    if (!aligned_to(16, {k, v}) || !aligned_to(4, {table, lengths, references, parents, children})) return false;
-    const Span keys = pool_span(k, c, p), values = pool_span(v, c, p), from = ints(parents, count),
-               to = ints(children, count);
-    if (TableSpans(table, lengths, references, c, p).bad({keys, values, from, to}) || clash(keys, {values, from, to}) ||
-        clash(values, {from, to}))
+    if (*kv_pages_reason(c, p) || !fork_ok(Pools(k, v, c, p), table, lengths, references, parents, children, count, c, p))
         return false;
     Kernel::Impl & impl = *kernel.impl_;
     if (!usable(impl, id)) return false;
@@ -315,21 +226,29 @@ bool kv_free(Kernel & kernel, int id, int * table, int * lengths, int * referenc
     return true;
 }
 
+bool rules::compact_ok(const Pools & pools, const int * table_out, const int * references_out, const int * used,
+                       const int * table, const int * lengths, const int * references, const KVCacheLayout & c,
+                       const KVPagesLayout & p) {
+    if (*kv_pages_reason(c, p) || !pools.given() || !table_out || !references_out || !used || !table || !lengths ||
+        !references)
+        return false;
+    if (!pools.aligned() || !aligned_to(4, {table_out, references_out, used, table, lengths, references})) return false;
+    const Span total = ints(used, 1);
+    const TableSpans in(table, lengths, references, c, p);
+    const Span rows = ints(table_out, (int64_t)p.sequences * p.row_pages), counts = ints(references_out, c.pages);
+    return !in.bad({total}) && !wraps({rows, counts}) && !pools.wrap() && !pools.meet_each_other() &&
+           !pools.meet({in.rows, in.lengths, in.references, rows, counts, total}) &&
+           !clash(rows, {counts, total, in.lengths, in.references}) && !clash(counts, {total, in.lengths, in.rows}) &&
+           (table_out == table || !clash(rows, {in.rows})) &&
+           (references_out == references || !clash(counts, {in.references}));
+}
+
 bool kv_compact(Kernel & kernel, int id, void * k, void * v, int * table_out, int * references_out, int * used,
                 const int * table, const int * lengths, const int * references, const KVCacheLayout & c,
                 const KVPagesLayout & p) {
     std::lock_guard<std::recursive_mutex> lock(detail::mutex());
-    if (*kv_pages_reason(c, p) || !k || !v || !table_out || !references_out || !used || !table || !lengths || !references)
-        return false;
-    if (!aligned_to(16, {k, v}) || !aligned_to(4, {table_out, references_out, used, table, lengths, references}))
-        return false;
-    const Span keys = pool_span(k, c, p), values = pool_span(v, c, p), total = ints(used, 1);
-    const TableSpans in(table, lengths, references, c, p);
-    const Span rows = ints(table_out, (int64_t)p.sequences * p.row_pages), counts = ints(references_out, c.pages);
-    if (in.bad({keys, values, total}) || wraps({rows, counts}) || clash(keys, {values, total}) || clash(values, {total}) ||
-        clash(rows, {counts, keys, values, total, in.lengths, in.references}) ||
-        clash(counts, {keys, values, total, in.lengths, in.rows}) || (table_out != table && clash(rows, {in.rows})) ||
-        (references_out != references && clash(counts, {in.references})))
+    if (*kv_pages_reason(c, p) ||
+        !compact_ok(Pools(k, v, c, p), table_out, references_out, used, table, lengths, references, c, p))
         return false;
     Kernel::Impl & impl = *kernel.impl_;
     if (!usable(impl, id)) return false;
@@ -343,14 +262,18 @@ bool kv_compact(Kernel & kernel, int id, void * k, void * v, int * table_out, in
     return true;
 }
 
+bool rules::copy_ok(const Pools & pools, const int * sources, const int * destinations, int count,
+                    const KVCacheLayout & c, const KVPagesLayout & p) {
+    if (*kv_pages_reason(c, p) || !pools.given() || !sources || !destinations || !list_ok(count, c.pages)) return false;
+    if (!pools.aligned() || !aligned_to(4, {sources, destinations})) return false;
+    const Span from = ints(sources, count), to = ints(destinations, count);
+    return !wraps({from, to}) && !pools.wrap() && !pools.meet_each_other() && !pools.meet({from, to});
+}
+
 bool kv_copy_pages(Kernel & kernel, int id, void * k, void * v, const int * sources, const int * destinations,
                    int count, const KVCacheLayout & c, const KVPagesLayout & p) {
     std::lock_guard<std::recursive_mutex> lock(detail::mutex());
-    if (*kv_pages_reason(c, p) || !k || !v || !sources || !destinations || !list_ok(count, c.pages)) return false;
-    if (!aligned_to(16, {k, v}) || !aligned_to(4, {sources, destinations})) return false;
-    const Span keys = pool_span(k, c, p), values = pool_span(v, c, p), from = ints(sources, count),
-               to = ints(destinations, count);
-    if (wraps({keys, values, from, to}) || clash(keys, {values, from, to}) || clash(values, {from, to})) return false;
+    if (*kv_pages_reason(c, p) || !copy_ok(Pools(k, v, c, p), sources, destinations, count, c, p)) return false;
     Kernel::Impl & impl = *kernel.impl_;
     if (!usable(impl, id)) return false;
     detail::DeviceContext & ctx = detail::context(id);

@@ -24,14 +24,27 @@ constexpr int kPlanWaves = kPlanThreads / kWave;
 constexpr int kCopyThreads = 256;
 
 struct PagesArgs {
-    _Float16 *k, *v;
+    char *k, *v;
+    float *k_scales, *v_scales;          // of 8-bit pools, else null
     int *table, *lengths, *references;
     int *status;
     PoolView pool;
-    kk::FastDiv per_row;                 // 16-byte vectors of a token's head
+    kk::FastDiv per_row;                 // vectors (8 values) of a token's head
     int64_t layer_stride;
     int sequences, row_pages, layers;
+    int blocks, block_tokens;            // scales of a page and head, tokens of each
+    // scales of a page, and where they stand in one layer's and pool's array
+    __device__ __forceinline__ int page_scales() const { return pool.heads * blocks; }
+    __device__ __forceinline__ float *scales_of(int in_v, int layer, int page) const {
+        return (in_v ? v_scales : k_scales) + ((int64_t)layer * pool.pages + page) * page_scales();
+    }
 };
+
+// Eight values of a pool, which hold 2 bytes each (uint4) or 1 (uint2); strides count values.
+template <typename V>
+__device__ __forceinline__ V *vector_at(char *pool, int64_t value) {
+    return reinterpret_cast<V *>(pool + value * static_cast<int>(sizeof(V) / 8));
+}
 
 // Sum of `v` over the threads before this one; `total` over all of them. Ends
 // with a barrier, so it may be called again at once.
@@ -284,7 +297,8 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int
 }
 
 // Fork i: its first workgroup releases the child's pages and writes the child's row,
-// the others copy the tokens of the parent's last page.
+// the others copy the tokens of the parent's last page, and their scales.
+template <typename V>
 __global__ __launch_bounds__(kCopyThreads) void fork_apply(PagesArgs a, const int *children, const ForkNote *notes,
                                                            const int *rows) {
     const int i = blockIdx.y;
@@ -320,18 +334,23 @@ __global__ __launch_bounds__(kCopyThreads) void fork_apply(PagesArgs a, const in
         if (blockIdx.x == 1 && threadIdx.x == 0) kk::report(a.status, kk::kBadPage);
         return;
     }
-    // 16 bytes a thread: a (layer, pool, head) at a time, its rows of `rest` tokens
+    // a vector a thread: a (layer, pool, head) at a time, its rows of `rest` tokens
     const int row_vectors = a.pool.width / 8, vectors = rest * row_vectors;
     const int blocks = a.layers * 2 * a.pool.heads;
     for (int b = blockIdx.x - 1; b < blocks; b += gridDim.x - 1) {
         const int head = b % a.pool.heads, pool = b / a.pool.heads % 2, layer = b / a.pool.heads / 2;
-        _Float16 *base = (pool ? a.v : a.k) + layer * a.layer_stride + head * a.pool.head_stride;
-        const _Float16 *src = base + page * a.pool.page_stride;
-        _Float16 *dst = base + note.page * a.pool.page_stride;
+        const int64_t base = layer * a.layer_stride + head * a.pool.head_stride;
+        char *const values = pool ? a.v : a.k;
+        const int64_t src = base + page * a.pool.page_stride, dst = base + note.page * a.pool.page_stride;
         for (int x = threadIdx.x; x < vectors; x += kCopyThreads) {
             const int token = a.per_row.div(x), at = x - token * row_vectors;
             const int64_t off = token * a.pool.token_stride + at * 8;
-            *reinterpret_cast<uint4 *>(dst + off) = *reinterpret_cast<const uint4 *>(src + off);
+            *vector_at<V>(values, dst + off) = *vector_at<V>(values, src + off);
+        }
+        if (a.k_scales) {
+            const float *from_scales = a.scales_of(pool, layer, page) + head * a.blocks;
+            float *to_scales = a.scales_of(pool, layer, note.page) + head * a.blocks;
+            for (int x = threadIdx.x; x * a.block_tokens < rest; x += kCopyThreads) to_scales[x] = from_scales[x];
         }
     }
 }
@@ -443,10 +462,9 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan(const int *referenc
 
 // Copies page src to dst in one layer's pool; the workgroup takes part `part` of
 // `parts`. DENSE: a page is one run of values.
-template <bool DENSE>
-__device__ __forceinline__ void copy_page(const PagesArgs &a, _Float16 *pool, int src, int dst, int part, int parts) {
-    const _Float16 *from = pool + src * a.pool.page_stride;
-    _Float16 *to = pool + dst * a.pool.page_stride;
+template <bool DENSE, typename V>
+__device__ __forceinline__ void copy_page(const PagesArgs &a, char *pool, int64_t layer, int src, int dst, int part, int parts) {
+    const int64_t from = layer + src * a.pool.page_stride, to = layer + dst * a.pool.page_stride;
     const int row_vectors = a.pool.width / 8;
     // up to 1024 x 65536 x 32 vectors
     const uint32_t vectors = static_cast<uint32_t>(a.pool.heads) * a.pool.page_tokens * row_vectors;
@@ -456,12 +474,12 @@ __device__ __forceinline__ void copy_page(const PagesArgs &a, _Float16 *pool, in
             const uint32_t row = a.per_row.div(x), head = a.pool.per_page.div(row), token = row - head * a.pool.page_tokens;
             off = head * a.pool.head_stride + token * a.pool.token_stride + (x - row * row_vectors) * 8;
         }
-        *reinterpret_cast<uint4 *>(to + off) = *reinterpret_cast<const uint4 *>(from + off);
+        *vector_at<V>(pool, to + off) = *vector_at<V>(pool, from + off);
     }
 }
 
 // Pages sources[i] -> destinations[i], i < *count: work items are (pair, layer, pool, part).
-template <bool DENSE>
+template <bool DENSE, typename V>
 __device__ __forceinline__ void copy_pairs(const PagesArgs &a, const int *sources, const int *destinations, int count,
                                            int parts, int item, int step) {
     const int per_pair = a.layers * 2 * parts;
@@ -475,24 +493,29 @@ __device__ __forceinline__ void copy_pairs(const PagesArgs &a, const int *source
             if (rest == 0 && threadIdx.x == 0) kk::report(a.status, kk::kBadPage);
             continue;
         }
-        copy_page<DENSE>(a, (pool ? a.v : a.k) + layer * a.layer_stride, src, dst, part, parts);
+        copy_page<DENSE, V>(a, pool ? a.v : a.k, layer * a.layer_stride, src, dst, part, parts);
+        if (a.k_scales && part == 0) {
+            const float *from = a.scales_of(pool, layer, src);
+            float *to = a.scales_of(pool, layer, dst);
+            for (int x = threadIdx.x; x < a.page_scales(); x += kCopyThreads) to[x] = from[x];
+        }
     }
 }
 
-template <bool DENSE>
+template <bool DENSE, typename V>
 __global__ __launch_bounds__(kCopyThreads) void copy_pages(PagesArgs a, const int *sources, const int *destinations,
                                                            int count, int parts) {
-    copy_pairs<DENSE>(a, sources, destinations, count, parts, blockIdx.x, gridDim.x);
+    copy_pairs<DENSE, V>(a, sources, destinations, count, parts, blockIdx.x, gridDim.x);
 }
 
 // The first `groups` workgroups rewrite the table and the counts, the others move the pages.
-template <bool DENSE>
+template <bool DENSE, typename V>
 __global__ __launch_bounds__(kCopyThreads) void compact_apply(PagesArgs a, const int *table, const int *references,
                                                               int *references_out, const int *used, const int *moves,
                                                               const int *holes, const int *movers, const int *fate,
                                                               int parts, int groups) {
     if (static_cast<int>(blockIdx.x) >= groups) {
-        copy_pairs<DENSE>(a, movers, holes, *moves, parts, blockIdx.x - groups, gridDim.x - groups);
+        copy_pairs<DENSE, V>(a, movers, holes, *moves, parts, blockIdx.x - groups, gridDim.x - groups);
         return;
     }
     const int u = *used;
@@ -527,8 +550,10 @@ __global__ __launch_bounds__(kCopyThreads) void compact_apply(PagesArgs a, const
 PagesArgs args_of(void *k, void *v, int *table, int *lengths, int *references, const kunlun::KVCacheLayout &c,
                   const kunlun::KVPagesLayout &p, int *status) {
     PagesArgs a;
-    a.k = static_cast<_Float16 *>(k);
-    a.v = static_cast<_Float16 *>(v);
+    a.k = static_cast<char *>(k);
+    a.v = static_cast<char *>(v);
+    a.k_scales = a.v_scales = nullptr;
+    a.blocks = a.block_tokens = 0;
     a.table = table;
     a.lengths = lengths;
     a.references = references;
@@ -551,9 +576,80 @@ bool dense(const kunlun::KVCacheLayout &c) {
 }
 
 // Workgroups that share a page's values in one pool: 16 KiB each.
-int parts_of(const kunlun::KVCacheLayout &c) {
-    const int64_t bytes = (int64_t)c.heads * c.page_tokens * c.width * 2;
+int parts_of(const kunlun::KVCacheLayout &c, int value_bytes) {
+    const int64_t bytes = (int64_t)c.heads * c.page_tokens * c.width * value_bytes;
     return static_cast<int>(std::min<int64_t>(64, (bytes + 16383) / 16384));
+}
+
+// An 8-bit pool's layout for the copies: pairs of values as one of 2 bytes where every row and stride is even vectors
+// of 16 bytes, else as it is, in vectors of 8.
+struct F8View {
+    kunlun::KVCacheLayout cache;
+    kunlun::KVPagesLayout pages;
+    bool pairs;
+};
+F8View view_of(const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p) {
+    F8View r{c, p, false};
+    const int64_t layer_stride = p.layers > 1 ? p.layer_stride : 0;
+    r.pairs = (c.width | c.page_stride | c.head_stride | c.token_stride | layer_stride) % 16 == 0;
+    if (r.pairs) {
+        r.cache.width /= 2;
+        r.cache.page_stride /= 2;
+        r.cache.head_stride /= 2;
+        r.cache.token_stride /= 2;
+        r.pages.layer_stride = layer_stride / 2;
+    }
+    return r;
+}
+void add_scales(PagesArgs &a, float *k_scales, float *v_scales, const kunlun::KVCacheF8Layout &f8) {
+    a.k_scales = k_scales;
+    a.v_scales = v_scales;
+    a.block_tokens = f8.block_tokens;
+    a.blocks = f8.cache.page_tokens / f8.block_tokens;
+}
+
+template <typename V>
+int fork(const PagesArgs &a, const int *parents, const int *children, int count, void *workspace, hipStream_t stream) {
+    ForkNote *notes = static_cast<ForkNote *>(workspace);
+    int *found = reinterpret_cast<int *>(notes + count), *rows = found + count;
+    int *far_claims = rows + (size_t)count * a.row_pages;
+    hipLaunchKernelGGL(fork_plan, dim3(1 + count), dim3(kPlanThreads), 0, stream, a, parents, children, count, notes,
+                       found, rows, far_claims);
+    // at most eight (layer, pool, head) blocks of the last page per workgroup
+    const int blocks = a.layers * 2 * a.pool.heads, copiers = std::max(1, std::min(blocks, 4096 / count));
+    hipLaunchKernelGGL(fork_apply<V>, dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);
+    return hipGetLastError();
+}
+
+template <typename V>
+int compact(const PagesArgs &a, bool dense, int parts, int *references_out, int *used, const int *table,
+            const int *references, void *workspace, int cus, hipStream_t stream) {
+    const int pages = a.pool.pages;
+    int *moves = static_cast<int *>(workspace), *holes = moves + 64, *movers = holes + pages, *fate = movers + pages;
+    const int tiles = (pages + kTile - 1) / kTile;
+    hipLaunchKernelGGL(compact_plan, dim3(std::min(tiles, cus)), dim3(kPlanThreads), 0, stream, references, pages, used,
+                       moves, holes, movers, fate);
+    const int groups = std::min(std::max(a.sequences, (pages + 4 * kCopyThreads - 1) / (4 * kCopyThreads)), 256);
+    const dim3 grid(groups + 8 * cus);
+    if (dense)
+        hipLaunchKernelGGL((compact_apply<true, V>), grid, dim3(kCopyThreads), 0, stream, a, table, references,
+                           references_out, used, moves, holes, movers, fate, parts, groups);
+    else
+        hipLaunchKernelGGL((compact_apply<false, V>), grid, dim3(kCopyThreads), 0, stream, a, table, references,
+                           references_out, used, moves, holes, movers, fate, parts, groups);
+    return hipGetLastError();
+}
+
+template <typename V>
+int copy(const PagesArgs &a, bool dense, int parts, const int *sources, const int *destinations, int count, int cus,
+         hipStream_t stream) {
+    const int64_t items = (int64_t)count * a.layers * 2 * parts;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(items, 8 * cus)));
+    if (dense)
+        hipLaunchKernelGGL((copy_pages<true, V>), grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
+    else
+        hipLaunchKernelGGL((copy_pages<false, V>), grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
+    return hipGetLastError();
 }
 
 } // namespace
@@ -578,16 +674,16 @@ extern "C" size_t kk_kv_fork_workspace_bytes(const kunlun::KVPagesLayout &p, int
 extern "C" int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *references, const int *parents, const int *children,
                int count, const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
                hipStream_t stream) {
-    const PagesArgs a = args_of(k, v, table, lengths, references, c, p, status);
-    ForkNote *notes = static_cast<ForkNote *>(workspace);
-    int *found = reinterpret_cast<int *>(notes + count), *rows = found + count;
-    int *far_claims = rows + (size_t)count * p.row_pages;
-    hipLaunchKernelGGL(fork_plan, dim3(1 + count), dim3(kPlanThreads), 0, stream, a, parents, children, count, notes,
-                       found, rows, far_claims);
-    // at most eight (layer, pool, head) blocks of the last page per workgroup
-    const int blocks = p.layers * 2 * c.heads, copiers = std::max(1, std::min(blocks, 4096 / count));
-    hipLaunchKernelGGL(fork_apply, dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);
-    return hipGetLastError();
+    return fork<uint4>(args_of(k, v, table, lengths, references, c, p, status), parents, children, count, workspace, stream);
+}
+extern "C" int kk_kv_fork_f8(void *k, void *v, float *k_scales, float *v_scales, int *table, int *lengths, int *references,
+                  const int *parents, const int *children, int count, const kunlun::KVCacheF8Layout &f8,
+                  const kunlun::KVPagesLayout &p, void *workspace, int *status, hipStream_t stream) {
+    const F8View view = view_of(f8.cache, p);
+    PagesArgs a = args_of(k, v, table, lengths, references, view.cache, view.pages, status);
+    add_scales(a, k_scales, v_scales, f8);
+    return view.pairs ? fork<uint4>(a, parents, children, count, workspace, stream)
+                      : fork<uint2>(a, parents, children, count, workspace, stream);
 }
 
 extern "C" int kk_kv_free(int *table, int *lengths, int *references, const int *rows, int count, const kunlun::KVCacheLayout &c,
@@ -603,33 +699,34 @@ extern "C" size_t kk_kv_compact_workspace_bytes(const kunlun::KVCacheLayout &c) 
 extern "C" int kk_kv_compact(void *k, void *v, int *table_out, int *references_out, int *used, const int *table,
                   const int *lengths, const int *references, const kunlun::KVCacheLayout &c,
                   const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus, hipStream_t stream) {
-    int *moves = static_cast<int *>(workspace), *holes = moves + 64, *movers = holes + c.pages, *fate = movers + c.pages;
-    const int tiles = (c.pages + kTile - 1) / kTile;
-    hipLaunchKernelGGL(compact_plan, dim3(std::min(tiles, cus)), dim3(kPlanThreads), 0, stream, references, c.pages, used,
-                       moves, holes, movers, fate);
     const PagesArgs a = args_of(k, v, table_out, const_cast<int *>(lengths), nullptr, c, p, status);
-    const int groups = std::min(std::max(p.sequences, (c.pages + 4 * kCopyThreads - 1) / (4 * kCopyThreads)), 256);
-    const int parts = parts_of(c);
-    const dim3 grid(groups + 8 * cus);
-    if (dense(c))
-        hipLaunchKernelGGL(compact_apply<true>, grid, dim3(kCopyThreads), 0, stream, a, table, references, references_out,
-                           used, moves, holes, movers, fate, parts, groups);
-    else
-        hipLaunchKernelGGL(compact_apply<false>, grid, dim3(kCopyThreads), 0, stream, a, table, references, references_out,
-                           used, moves, holes, movers, fate, parts, groups);
-    return hipGetLastError();
+    return compact<uint4>(a, dense(c), parts_of(c, 2), references_out, used, table, references, workspace, cus, stream);
+}
+extern "C" int kk_kv_compact_f8(void *k, void *v, float *k_scales, float *v_scales, int *table_out, int *references_out,
+                     int *used, const int *table, const int *lengths, const int *references,
+                     const kunlun::KVCacheF8Layout &f8, const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus,
+                     hipStream_t stream) {
+    const F8View view = view_of(f8.cache, p);
+    PagesArgs a = args_of(k, v, table_out, const_cast<int *>(lengths), nullptr, view.cache, view.pages, status);
+    add_scales(a, k_scales, v_scales, f8);
+    const int parts = parts_of(f8.cache, 1);
+    return view.pairs ? compact<uint4>(a, dense(view.cache), parts, references_out, used, table, references, workspace, cus, stream)
+                      : compact<uint2>(a, dense(view.cache), parts, references_out, used, table, references, workspace, cus, stream);
 }
 
 extern "C" int kk_kv_copy_pages(void *k, void *v, const int *sources, const int *destinations, int count,
                      const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, int *status, int cus,
                      hipStream_t stream) {
     const PagesArgs a = args_of(k, v, nullptr, nullptr, nullptr, c, p, status);
-    const int parts = parts_of(c);
-    const int64_t items = (int64_t)count * p.layers * 2 * parts;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(items, 8 * cus)));
-    if (dense(c))
-        hipLaunchKernelGGL(copy_pages<true>, grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
-    else
-        hipLaunchKernelGGL(copy_pages<false>, grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
-    return hipGetLastError();
+    return copy<uint4>(a, dense(c), parts_of(c, 2), sources, destinations, count, cus, stream);
+}
+extern "C" int kk_kv_copy_pages_f8(void *k, void *v, float *k_scales, float *v_scales, const int *sources,
+                        const int *destinations, int count, const kunlun::KVCacheF8Layout &f8, const kunlun::KVPagesLayout &p,
+                        int *status, int cus, hipStream_t stream) {
+    const F8View view = view_of(f8.cache, p);
+    PagesArgs a = args_of(k, v, nullptr, nullptr, nullptr, view.cache, view.pages, status);
+    add_scales(a, k_scales, v_scales, f8);
+    const int parts = parts_of(f8.cache, 1);
+    return view.pairs ? copy<uint4>(a, dense(view.cache), parts, sources, destinations, count, cus, stream)
+                      : copy<uint2>(a, dense(view.cache), parts, sources, destinations, count, cus, stream);
 }

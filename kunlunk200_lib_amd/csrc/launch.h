@@ -183,6 +183,32 @@ int kk_kv_copy_pages(void *k, void *v, const int *sources, const int *destinatio
                      const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, int *status, int cus,
                      hipStream_t stream);
 
+// The cache in 8 bits (k200.h): attention over it (workspace and sums as above), new tokens into it, tokens
+// read back, and pages with their scales (workspaces as above).
+size_t kk_paged_attention_f8_workspace_bytes(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p,
+                                             int cus);
+const char *kk_paged_attention_f8_route(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout &p, int cus);
+int kk_paged_attention_f8(void *y, const void *q, const void *k, const void *v, const float *k_scales,
+                          const float *v_scales, const int *table, const int *lengths, const kunlun::KVCacheF8Layout &f8,
+                          const kunlun::PagedAttentionLayout &p, void *workspace, int *status, int cus,
+                          hipStream_t stream);
+int kk_kv_append_f8(void *k_pool, void *v_pool, float *k_scales, float *v_scales, void *q_out, const void *q,
+                    const void *k, const void *v, const int *sequence, const int *position, const int *lengths,
+                    const int *table, const float *cosine, const float *sine, const kunlun::KVCacheF8Layout &f8,
+                    const kunlun::KVAppendLayout &p, int *status, hipStream_t stream);
+int kk_kv_read_f8(void *k_out, void *v_out, const void *k_pool, const void *v_pool, const float *k_scales,
+                  const float *v_scales, const int *sequence, const int *position, const int *lengths, const int *table,
+                  const kunlun::KVCacheF8Layout &f8, const kunlun::KVReadLayout &p, int *status, hipStream_t stream);
+int kk_kv_fork_f8(void *k, void *v, float *k_scales, float *v_scales, int *table, int *lengths, int *references,
+                  const int *parents, const int *children, int count, const kunlun::KVCacheF8Layout &f8,
+                  const kunlun::KVPagesLayout &p, void *workspace, int *status, hipStream_t stream);
+int kk_kv_compact_f8(void *k, void *v, float *k_scales, float *v_scales, int *table_out, int *references_out, int *used,
+                     const int *table, const int *lengths, const int *references, const kunlun::KVCacheF8Layout &f8,
+                     const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus, hipStream_t stream);
+int kk_kv_copy_pages_f8(void *k, void *v, float *k_scales, float *v_scales, const int *sources, const int *destinations,
+                        int count, const kunlun::KVCacheF8Layout &f8, const kunlun::KVPagesLayout &p, int *status, int cus,
+                        hipStream_t stream);
+
 // Penalties, biases and a mask on rows of logits (k200.h).
 int kk_process_logits(float *y, const float *logits, const float *penalties, const int *history,
                       const int *history_lengths, const int *bias_ids, const float *bias_values,
