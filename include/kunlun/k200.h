@@ -530,7 +530,8 @@ bool paged_attention_f8(Kernel &, int device, void * y, const void * q, const vo
 // holds earlier tokens and their scale is larger; where it grows, the earlier tokens' codes are rounded to the new one.
 // A new value is rounded once, to the nearest code of its F64 rotation (ties to the even code). A value that is not finite
 // makes its block's scale, so all of the block, not a number, until the block is begun again. Tokens of one block must
-// be consecutive entries of rising positions; what the block held from the first of them on is forgotten.
+// stand in consecutive entries of consecutive positions (some of which may be left out); what the block held from the first
+// of them on is forgotten.
 // Up to 2^31 threads: (query_heads * width / 8 + 512 * heads) * tokens.
 const char * kv_append_f8_reason(const KVCacheF8Layout &, const KVAppendLayout &);
 bool kv_append_f8(Kernel &, int device, void * k_pool, void * v_pool, float * k_scales, float * v_scales, void * q_out,

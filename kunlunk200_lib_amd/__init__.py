@@ -822,7 +822,7 @@ def paged_attention_f8(kernel: Kernel, device: int, y, q, k, v, k_scales, v_scal
 def kv_append_f8(kernel: Kernel, device: int, k_pool, v_pool, k_scales, v_scales, q_out, q, k, v, sequence, position,
                  lengths, table, cosine, sine, cache: KVCacheF8Layout, call: KVAppendLayout) -> bool:
     """Submit new tokens: q and k turned by their positions' angles, k and v quantised into their pages
-    (tokens of one block in consecutive entries of rising positions)."""
+    (tokens of one block in consecutive entries of consecutive positions)."""
     return bool(load().kunlun_kv_append_f8(kernel.handle, int(device), _ptr(k_pool), _ptr(v_pool), _ptr(k_scales),
                                            _ptr(v_scales), _ptr(q_out), _ptr(q), _ptr(k), _ptr(v), _ptr(sequence),
                                            _ptr(position), _ptr(lengths), _ptr(table), _ptr(cosine), _ptr(sine),

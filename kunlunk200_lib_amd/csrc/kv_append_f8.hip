@@ -8,7 +8,7 @@
 // once: keys are turned in F64, where products of F32 factors are exact, and reach F32 rounded to odd, so that rounding
 // that to a code's four bits rounds the F64 value (in F32 throughout one code in 2^19 is the neighbour of the nearest).
 //
-// The first new token of a block finds how many follow it; its GROUP lanes (16 to 256, by the block's values) hold all of
+// The first new token of a block finds which follow it; its GROUP lanes (16 to 256, by the block's values) hold all of
 // the block's new values of one head in registers between the largest and the codes. The other tokens' lanes leave at once.
 // One launch with the queries in front; bound by the bytes it reads and writes.
 #include "device_common.h"
@@ -189,26 +189,24 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
     const int block_tokens = 1 << a.block_log2;
     const int page_at = a.pool.per_page.div(at.pos), within = at.pos - page_at * a.pool.page_tokens;
     const int earlier = within & (block_tokens - 1);                      // tokens of the block before this one
-    if (earlier > 0 && token > 0) {
-        const Place before = place_of(a, token - 1);
-        if (!before.out && before.s == at.s && before.pos == at.pos - 1) return;      // that one's lanes, or an earlier one's, have it
-    }
+    // Whether a token before this one in the block is among the entries before it (that one's lanes, or an earlier one's,
+    // have this one too), and which of those that may follow do; entries in between may be left out.
+    auto names = [&](int distance) {
+        const Place x = place_of(a, token + distance);
+        return !x.out && x.s == at.s && x.pos == at.pos + distance;
+    };
+    const bool precedes = in_wave < min(earlier, token) && names(-1 - in_wave);
+    const bool follows = in_wave == 0 || (in_wave < min(block_tokens - earlier, a.tokens - token) && names(in_wave));
+    const int shift = static_cast<int>(threadIdx.x % kWave) - in_wave;
+    const uint64_t own = (kLanes < kWave ? (uint64_t(1) << kLanes % kWave) - 1 : ~uint64_t(0));
+    if ((__ballot(precedes) >> shift) & own) return;
+    const uint64_t members = (__ballot(follows) >> shift) & own;
     int page;
     if (!page_of(a, at, page)) {
         if (hk == 0 && lane == 0) kk::report(a.status, kk::kBadPage);
         return;
     }
-    // the tokens that follow in the block
-    bool follows = in_wave == 0;
-    if (in_wave > 0 && in_wave < block_tokens - earlier && token + in_wave < a.tokens) {
-        const Place next = place_of(a, token + in_wave);
-        follows = !next.out && next.s == at.s && next.pos == at.pos + in_wave;
-    }
-    const int shift = static_cast<int>(threadIdx.x % kWave) - in_wave;
-    const uint64_t all = ~(__ballot(follows) >> shift);
-    const int run = min(kLanes, all ? __builtin_ctzll(all) : kWave);
-
-    const int units = a.units_per_head.d, fresh = run * units;
+    const int units = a.units_per_head.d, fresh = (kWave - __builtin_clzll(members)) * units;     // up to the last one's end
     const T *from = (is_k ? static_cast<const T *>(a.k) + token * a.k_stride : static_cast<const T *>(a.v) + token * a.v_stride) +
                     h * a.pool.width;
     const int64_t stride = is_k ? a.k_stride : a.v_stride;
@@ -220,6 +218,7 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
         const int number = lane + n * GROUP;
         if (number >= fresh) break;
         const int j = a.units_per_head.div(number);
+        if (!(members >> j & 1)) continue;
         const Unit<T, HALVES, VEC> unit(number - j * units, rotary);
         unit.load(from + j * stride, x[n]);
     }
@@ -228,6 +227,7 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
         const int number = lane + n * GROUP;
         if (number >= fresh) break;
         const int j = a.units_per_head.div(number);
+        if (!(members >> j & 1)) continue;
         const Unit<T, HALVES, VEC> unit(number - j * units, rotary);
         const int64_t angles = (int64_t)(at.pos + j) * unit.half;
         unit.each_pair(a.cosine + angles, a.sine + angles, x[n], [](float &p, float &r, float cs, float sn) {
@@ -274,6 +274,7 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
         const int number = lane + n * GROUP;
         if (number >= fresh) break;
         const int j = a.units_per_head.div(number);
+        if (!(members >> j & 1)) continue;
         const Unit<T, HALVES, VEC> unit(number - j * units, rotary);
         uint8_t *to = block + (earlier + j) * a.pool.token_stride;
         const uint32_t low = four_codes(x[n][0] * by, x[n][1] * by, x[n][2] * by, x[n][3] * by);

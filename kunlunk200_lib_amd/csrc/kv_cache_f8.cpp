@@ -125,11 +125,7 @@ bool kv_read_f8(Kernel & kernel, int id, void * k, void * v, const void * k_pool
 
 const char * kv_pages_f8_reason(const KVCacheF8Layout & f, const KVPagesLayout & p) {
     const char * cache = kv_cache_f8_reason(f);
-    if (*cache) return cache;
-    const char * pages = kv_pages_reason(f.cache, p);
-    if (*pages) return pages;
-    const int64_t scales = (int64_t)f.cache.pages * f.cache.heads * (f.cache.page_tokens / f.block_tokens);   // below 2^57
-    return scales > (INT64_MAX / 16) / p.layers ? "byte extent" : "";
+    return *cache ? cache : kv_pages_reason(f.cache, p);
 }
 
 bool kv_fork_f8(Kernel & kernel, int id, void * k, void * v, float * k_scales, float * v_scales, int * table, int * lengths,
