@@ -8,13 +8,16 @@
 // once: keys are turned in F64, where products of F32 factors are exact, and reach F32 rounded to odd, so that rounding
 // that to a code's four bits rounds the F64 value (in F32 throughout one code in 2^19 is the neighbour of the nearest).
 //
-// The first new token of a block finds which follow it; its GROUP lanes (16 to 256, by the block's values) hold all of
-// the block's new values of one head in registers between the largest and the codes. The other tokens' lanes leave at once.
+// The first new token of a block finds which follow it. Its lanes, a wave or less for a few tokens as in decoding, a
+// workgroup of up to 1024 for more, hold all of the block's new values of one head in registers between the largest and the
+// codes; the others leave at once.
 // One launch with the queries in front; bound by the bytes it reads and writes.
 #include "device_common.h"
 #include "kv_rows.h"
 #include "launch.h"
 #include "paged.h"
+
+#include <algorithm>
 
 namespace {
 
@@ -23,6 +26,8 @@ using kk::PoolView;
 
 constexpr int kThreads = 256;
 constexpr int kLeastExponent = -64;      // of a scale
+constexpr int kMostGroups = 2048;        // that look through one entry each
+constexpr int kMostWaves = 16;           // of a workgroup
 
 typedef float float2v __attribute__((ext_vector_type(2)));
 
@@ -36,32 +41,36 @@ struct F8Args {
     int *status;
     PoolView pool;
     int64_t q_stride, k_stride, v_stride, q_out_stride;
-    kk::FastDiv q_units_per_token, units_per_head, heads_per_token;   // heads_per_token: keys' and values'
+    kk::FastDiv q_units_per_token;
+    kk::FastDiv units_per_head;          // append: of 8 values; read: pieces of 16 bytes
+    kk::FastDiv heads_per_token;         // append: keys' and values'; read: a token's parts
     int tokens, sequences, row_pages, query_heads, rotary, positions;
     int block_log2, blocks;              // tokens of a scale are 2^block_log2; scales of a page and head
-    uint32_t q_units, q_groups;          // 8-value units of all queries, and the workgroups that take them
-    int64_t items;                       // tokens x heads_per_token
+    uint32_t q_units;                    // units of kQueryHeads query heads, of all tokens
+    uint32_t large_groups;               // workgroups for many new tokens of a block
+    uint32_t q_step;                     // the queries' share of all workgroups, of 2^32
+    int window;                          // append: entries that a group of lanes looks through
+    uint32_t items;                      // append: windows x heads_per_token; read: tokens x parts of one
 };
 
 // Where token i goes: its sequence and position, or why it goes nowhere.
 struct Place {
     int s, pos;
-    bool out, bad;                       // left out; reported
+    bool out, bad;                       // left out; reported too
 };
 __device__ __forceinline__ Place place_of(const F8Args &a, int i) {
-    Place r{a.sequence ? a.sequence[i] : i, -1, true, false};
-    if (r.s < 0) return r;
-    r.bad = r.s >= a.sequences;
-    if (r.bad) return r;
-    r.pos = a.position ? a.position[i] : a.lengths[r.s] - 1;
-    if (r.pos < 0) return r;
-    r.bad = a.pool.per_page.div(r.pos) >= static_cast<uint32_t>(a.row_pages) || (a.rotary > 0 && r.pos >= a.positions);
-    r.out = r.bad;
-    return r;
+    // both loads on their way at once (without positions there are no sequences either: token i is the newest of sequence i)
+    const int s = a.sequence ? a.sequence[i] : i, pos = a.position ? a.position[i] : a.lengths[i] - 1;
+    const bool bad = s >= a.sequences || (s >= 0 && pos >= 0 && (a.pool.per_page.div(pos) >= static_cast<uint32_t>(a.row_pages) ||
+                                                                 (a.rotary > 0 && pos >= a.positions)));
+    return Place{s, pos, bad || s < 0 || pos < 0, bad};
 }
 
-__device__ __forceinline__ bool page_of(const F8Args &a, const Place &at, int &page) {
-    page = a.table[(int64_t)at.s * a.row_pages + a.pool.per_page.div(at.pos)];
+// The page of a token that is not left out; it may be one that the pool does not have.
+__device__ __forceinline__ int page_of(const F8Args &a, const Place &at) {
+    return a.table[(int64_t)at.s * a.row_pages + a.pool.per_page.div(at.pos)];
+}
+__device__ __forceinline__ bool in_pool(const F8Args &a, int page) {
     return static_cast<unsigned>(page) < static_cast<unsigned>(a.pool.pages);
 }
 
@@ -102,49 +111,61 @@ struct Unit {
             for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(from[element(i)]);
         }
     }
-    // turn(a, b, cos, sin) on every pair
+    // turn(low, high, cos, sin) for every pair's places in the unit
     template <typename Turn>
-    __device__ __forceinline__ void each_pair(const float *cosine, const float *sine, float (&x)[8], Turn turn) const {
+    __device__ __forceinline__ void each_pair(const float *cosine, const float *sine, Turn turn) const {
         if constexpr (VEC) {
             if (!turned) return;
             float cs[8], sn[8];
             kk::load_values<float, 4>(cosine + u * 4, cs, 0);
             kk::load_values<float, 4>(sine + u * 4, sn, 0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) turn(x[low(j)], x[high(j)], cs[j], sn[j]);
+            for (int j = 0; j < 4; ++j) turn(low(j), high(j), cs[j], sn[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (j < pairs) turn(x[2 * j], x[2 * j + 1], cosine[u * 4 + j], sine[u * 4 + j]);
+                if (j < pairs) turn(2 * j, 2 * j + 1, cosine[u * 4 + j], sine[u * 4 + j]);
         }
     }
 };
 
+// The same unit of kQueryHeads neighbouring query heads of a token, which share its angles.
+constexpr int kQueryHeads = 4;
 template <typename T, bool HALVES, bool VEC>
-__device__ __forceinline__ void turn_query(const F8Args &a) {
-    const uint32_t number = blockIdx.x * kThreads + threadIdx.x;
+__device__ __forceinline__ void turn_queries(const F8Args &a, uint32_t number) {
     if (number >= a.q_units) return;
     const int token = a.q_units_per_token.div(number), in_token = number - token * a.q_units_per_token.d;
-    const int head = a.units_per_head.div(in_token);
+    const int head_group = a.units_per_head.div(in_token), first = head_group * kQueryHeads;
+    const int heads = min(kQueryHeads, a.query_heads - first);
     const Place at = place_of(a, token);
-    int page;
-    if (at.out || !page_of(a, at, page)) return;     // reported with the keys
-    const Unit<T, HALVES, VEC> unit(in_token - head * a.units_per_head.d, a.rotary);
-    float x[8];
-    unit.load(static_cast<const T *>(a.q) + token * a.q_stride + head * a.pool.width, x);
-    const int64_t angles = (int64_t)at.pos * unit.half;
-    unit.each_pair(a.cosine + angles, a.sine + angles, x, [](float &p, float &r, float cs, float sn) {
-        const float y = fmaf(p, cs, -(r * sn));
-        r = fmaf(p, sn, r * cs);
-        p = y;
-    });
-    T *to = static_cast<T *>(a.q_out) + token * a.q_out_stride + head * a.pool.width;
-    if constexpr (VEC) {
-        kk::store_values<T, 4>(to + unit.element(0), x, 0);
-        kk::store_values<T, 4>(to + unit.element(4), x, 4);
-    } else {
+    if (at.out) return;                              // reported with the keys
+    const int page = page_of(a, at);
+    const Unit<T, HALVES, VEC> unit(in_token - head_group * a.units_per_head.d, a.rotary);
+    float x[kQueryHeads][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) to[unit.element(i)] = static_cast<T>(x[i]);
+    for (int n = 0; n < kQueryHeads; ++n)
+        unit.load(static_cast<const T *>(a.q) + token * a.q_stride + (first + min(n, heads - 1)) * a.pool.width, x[n]);
+    const int64_t angles = (int64_t)at.pos * unit.half;
+    unit.each_pair(a.cosine + angles, a.sine + angles, [&](int low, int high, float cs, float sn) {
+#pragma unroll
+        for (int n = 0; n < kQueryHeads; ++n) {
+            const float p = x[n][low], r = x[n][high];
+            x[n][low] = fmaf(p, cs, -(r * sn));
+            x[n][high] = fmaf(p, sn, r * cs);
+        }
+    });
+    if (!in_pool(a, page)) return;                   // reported with the keys
+#pragma unroll
+    for (int n = 0; n < kQueryHeads; ++n) {
+        if (n >= heads) break;
+        T *to = static_cast<T *>(a.q_out) + token * a.q_out_stride + (first + n) * a.pool.width;
+        if constexpr (VEC) {
+            kk::store_values<T, 4>(to + unit.element(0), x[n], 0);
+            kk::store_values<T, 4>(to + unit.element(4), x[n], 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[unit.element(i)] = static_cast<T>(x[n][i]);
+        }
     }
 }
 
@@ -165,48 +186,19 @@ __device__ __forceinline__ void eight_values(uint2 codes, float scale, float (&x
     x[4] = c[0] * scale, x[5] = c[1] * scale, x[6] = d[0] * scale, x[7] = d[1] * scale;
 }
 
-// UNITS: units a lane holds at most.
+// The new tokens of a block, one head of keys or values, by GROUP lanes that hold UNITS units each: entries token + j for
+// the bits j of `members`, of which the first stands at sequence s and position pos.
 template <typename T, bool HALVES, bool VEC, int GROUP, int UNITS>
-__global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
-    if (blockIdx.x < a.q_groups) {
-        turn_query<T, HALVES, VEC>(a);
-        return;
-    }
+__device__ __forceinline__ void store_block(const F8Args &a, int token, int s, int pos, uint64_t members, int hk, int lane,
+                                            uint32_t (*tops)[kMostWaves], int &turn) {
     constexpr int kLanes = GROUP < kWave ? GROUP : kWave;                 // of the group that are in one wave
-    __shared__ uint32_t tops[kThreads / kWave];
-    const int64_t number = (int64_t)(blockIdx.x - a.q_groups) * (kThreads / GROUP) + threadIdx.x / GROUP;
-    if (number >= a.items) return;
-    const int lane = threadIdx.x % GROUP, in_wave = threadIdx.x % kLanes;
-    const uint32_t item = static_cast<uint32_t>(number);
-    const int token = a.heads_per_token.div(item), hk = item - token * a.heads_per_token.d;
+    const int units = a.units_per_head.d;
     const bool is_k = hk < a.pool.heads;
     const int h = is_k ? hk : hk - a.pool.heads;
-    const Place at = place_of(a, token);
-    if (at.out) {
-        if (at.bad && hk == 0 && lane == 0) kk::report(a.status, kk::kBadIndex);
-        return;
-    }
-    const int block_tokens = 1 << a.block_log2;
-    const int page_at = a.pool.per_page.div(at.pos), within = at.pos - page_at * a.pool.page_tokens;
-    const int earlier = within & (block_tokens - 1);                      // tokens of the block before this one
-    // Whether a token before this one in the block is among the entries before it (that one's lanes, or an earlier one's,
-    // have this one too), and which of those that may follow do; entries in between may be left out.
-    auto names = [&](int distance) {
-        const Place x = place_of(a, token + distance);
-        return !x.out && x.s == at.s && x.pos == at.pos + distance;
-    };
-    const bool precedes = in_wave < min(earlier, token) && names(-1 - in_wave);
-    const bool follows = in_wave == 0 || (in_wave < min(block_tokens - earlier, a.tokens - token) && names(in_wave));
-    const int shift = static_cast<int>(threadIdx.x % kWave) - in_wave;
-    const uint64_t own = (kLanes < kWave ? (uint64_t(1) << kLanes % kWave) - 1 : ~uint64_t(0));
-    if ((__ballot(precedes) >> shift) & own) return;
-    const uint64_t members = (__ballot(follows) >> shift) & own;
-    int page;
-    if (!page_of(a, at, page)) {
-        if (hk == 0 && lane == 0) kk::report(a.status, kk::kBadPage);
-        return;
-    }
-    const int units = a.units_per_head.d, fresh = (kWave - __builtin_clzll(members)) * units;     // up to the last one's end
+    const int page_at = a.pool.per_page.div(pos), within = pos - page_at * a.pool.page_tokens;
+    const int earlier = within & ((1 << a.block_log2) - 1);               // tokens of the block before these
+    const int fresh = (kWave - __builtin_clzll(members)) * units;         // units up to the last one's end
+    const int page = a.table[(int64_t)s * a.row_pages + page_at];         // asked about after the values are on their way
     const T *from = (is_k ? static_cast<const T *>(a.k) + token * a.k_stride : static_cast<const T *>(a.v) + token * a.v_stride) +
                     h * a.pool.width;
     const int64_t stride = is_k ? a.k_stride : a.v_stride;
@@ -222,6 +214,10 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
         const Unit<T, HALVES, VEC> unit(number - j * units, rotary);
         unit.load(from + j * stride, x[n]);
     }
+    if (!in_pool(a, page)) {
+        if (hk == 0 && lane == 0) kk::report(a.status, kk::kBadPage);
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < UNITS; ++n) {
         const int number = lane + n * GROUP;
@@ -229,11 +225,11 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
         const int j = a.units_per_head.div(number);
         if (!(members >> j & 1)) continue;
         const Unit<T, HALVES, VEC> unit(number - j * units, rotary);
-        const int64_t angles = (int64_t)(at.pos + j) * unit.half;
-        unit.each_pair(a.cosine + angles, a.sine + angles, x[n], [](float &p, float &r, float cs, float sn) {
-            const double dp = p, dr = r, dc = cs, ds = sn;
-            p = to_odd(fma(dp, dc, -(dr * ds)));
-            r = to_odd(fma(dp, ds, dr * dc));
+        const int64_t angles = (int64_t)(pos + j) * unit.half;
+        unit.each_pair(a.cosine + angles, a.sine + angles, [&](int low, int high, float cs, float sn) {
+            const double p = x[n][low], r = x[n][high], dc = cs, ds = sn;
+            x[n][low] = to_odd(fma(p, dc, -(r * ds)));
+            x[n][high] = to_odd(fma(p, ds, r * dc));
         });
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[n][i]) & 0x7fffffffu);
@@ -242,10 +238,12 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
     for (int offset = kLanes / 2; offset > 0; offset >>= 1)
         top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), offset, kWave)));
     if constexpr (GROUP > kWave) {
-        if (in_wave == 0) tops[threadIdx.x / kWave] = top;
+        // in turn, so that the next block's do not reach these before every wave has read them
+        uint32_t *of_waves = tops[turn ^= 1];
+        if (lane % kWave == 0) of_waves[lane / kWave] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kThreads / kWave; ++w) top = max(top, tops[w]);
+        for (int w = 0; w < GROUP / kWave; ++w) top = max(top, of_waves[w]);
     }
 
     float *scale_at = (is_k ? a.k_scales : a.v_scales) + ((int64_t)page * a.pool.heads + h) * a.blocks + (within >> a.block_log2);
@@ -293,55 +291,152 @@ __global__ __launch_bounds__(kThreads) void append_f8(F8Args a) {
     }
 }
 
-template <typename T, bool HALVES, bool VEC>
-int launch(const F8Args &a, hipStream_t stream) {
-    const int units = a.units_per_head.d << a.block_log2;                 // of a whole block, up to 2048
-    const int group = units <= 16 ? 16 : units <= 32 ? 32 : units <= 4 * kWave ? 64 : 256;
-    const int64_t groups = a.q_groups + (a.items + kThreads / group - 1) / (kThreads / group);
-    if (groups > INT32_MAX / kThreads) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(groups));
-    if (group == 16) hipLaunchKernelGGL((append_f8<T, HALVES, VEC, 16, 1>), grid, dim3(kThreads), 0, stream, a);
-    else if (group == 32) hipLaunchKernelGGL((append_f8<T, HALVES, VEC, 32, 1>), grid, dim3(kThreads), 0, stream, a);
-    else if (group == 64) hipLaunchKernelGGL((append_f8<T, HALVES, VEC, 64, 4>), grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((append_f8<T, HALVES, VEC, 256, 8>), grid, dim3(kThreads), 0, stream, a);
+// An entry, in terms that the tokens of one block share where they stand in consecutive entries of consecutive positions.
+struct Entry {
+    int s, lag, block;                   // sequence, position less number, block of the sequence; s -1: left out
+    __device__ __forceinline__ bool same(const Entry &o) const { return s == o.s && lag == o.lag && block == o.block; }
+};
+__device__ __forceinline__ Entry entry_of(const F8Args &a, int i, bool &bad) {
+    const bool there = i >= 0 && i < a.tokens;
+    const Place at = place_of(a, there ? i : 0);
+    bad = there && at.bad;
+    return Entry{there && !at.out ? at.s : -1, at.pos - i, at.pos >> a.block_log2};
+}
+
+// The blocks that the entries of one window begin, one head of keys or values, by GROUP lanes. `little`: those whose
+// new tokens fit the first kWave units, else the others.
+template <typename T, bool HALVES, bool VEC, int GROUP, int UNITS>
+__device__ __forceinline__ void store_window(const F8Args &a, uint32_t item, int size, bool little, uint32_t (*tops)[kMostWaves]) {
+    constexpr int kLanes = GROUP < kWave ? GROUP : kWave;
+    const int lane = threadIdx.x % GROUP, in_wave = threadIdx.x % kLanes, shift = static_cast<int>(threadIdx.x % kWave) - in_wave;
+    const int window = a.heads_per_token.div(item), hk = item - window * a.heads_per_token.d, first = window * size;
+    const uint64_t own = kLanes < kWave ? (uint64_t(1) << kLanes % kWave) - 1 : ~uint64_t(0);
+    auto of_group = [&](bool what) { return (__ballot(what) >> shift) & own; };
+    // the entries before the window, from its first on, and after those: a block's are less than kLanes apart
+    bool bad, unused;
+    const Entry none{-1, 0, 0}, here = entry_of(a, first + in_wave, bad);
+    Entry before = none, after = none, last = none;
+    if (a.block_log2 > 0) {
+        before = entry_of(a, first + in_wave - kLanes, unused);
+        after = entry_of(a, first + in_wave + kLanes, unused);
+        last = entry_of(a, first + in_wave - 1, unused);
+    }
+    if (bad && in_wave < size && little && hk == 0) kk::report(a.status, kk::kBadIndex);
+    int turn = 0;
+    for (uint64_t left = of_group(in_wave < size && here.s >= 0 && !here.same(last)); left; left &= left - 1) {
+        const int at = __builtin_ctzll(left);
+        const Entry x{__shfl(here.s, shift + at, kWave), __shfl(here.lag, shift + at, kWave), __shfl(here.block, shift + at, kWave)};
+        const uint64_t window_has = of_group(x.same(here));
+        // (it follows a left-out entry: an earlier one begins its block)
+        if (of_group(x.same(before)) || window_has & ((uint64_t(1) << at) - 1)) continue;
+        const uint64_t members = window_has >> at | (at ? of_group(x.same(after)) << (kLanes - at) : 0);
+        if (((kWave - __builtin_clzll(members)) * static_cast<int>(a.units_per_head.d) <= kWave) != little) continue;
+        const int token = first + at;
+        store_block<T, HALVES, VEC, GROUP, UNITS>(a, token, x.s, x.lag + token, members, hk, lane, tops, turn);
+    }
+}
+
+// The workgroups of the queries, which stream, lie evenly among those of keys and values, which wait for one another's
+// results, so that a CU holds both (2047 tokens of 32 + 8 heads of 128: SPREAD us, one kind after the other 25). Of the
+// latter first come those that take many new tokens of a block together, then those of SMALL lanes for a block's few new
+// tokens (all of them, where a whole block has no more units).
+template <typename T, bool HALVES, bool VEC, int SMALL, int LARGE, int UNITS>
+__global__ __launch_bounds__(LARGE ? LARGE : kThreads) void append_f8(F8Args a) {
+    constexpr int kGroup = LARGE ? LARGE : kThreads;
+    __shared__ uint32_t tops[2][kMostWaves];
+    const uint32_t queries = __umulhi(blockIdx.x, a.q_step), number = blockIdx.x - queries;    // of the workgroups before this one
+    if (__umulhi(blockIdx.x + 1, a.q_step) != queries) {
+        turn_queries<T, HALVES, VEC>(a, queries * kGroup + threadIdx.x);
+    } else if (LARGE > 0 && number < a.large_groups) {
+        if constexpr (LARGE > 0) store_window<T, HALVES, VEC, LARGE, UNITS>(a, number, 1 << a.block_log2, false, tops);
+    } else {
+        const uint32_t item = (number - a.large_groups) * (kGroup / SMALL) + threadIdx.x / SMALL;
+        if (item < a.items) store_window<T, HALVES, VEC, SMALL, 1>(a, item, a.window, true, tops);
+    }
+}
+
+template <typename T, bool HALVES, bool VEC, int SMALL, int LARGE, int UNITS>
+int launch_groups(F8Args a, hipStream_t stream) {
+    const int threads = LARGE ? LARGE : kThreads, units = a.units_per_head.d, pairs = a.heads_per_token.d;
+    const uint32_t q_groups = (a.q_units + threads - 1) / threads;
+    // one entry a group, or as many as leave the groups within what the card holds at once
+    a.window = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(1 << a.block_log2, (int64_t)a.tokens * pairs / kMostGroups)));
+    a.items = static_cast<uint32_t>((a.tokens + a.window - 1) / a.window * pairs);
+    const uint32_t small_groups = (a.items * SMALL + threads - 1) / threads;
+    const int windows = (a.tokens + (1 << a.block_log2) - 1) >> a.block_log2;
+    a.large_groups = LARGE && (int64_t)a.tokens * units > kWave ? windows * pairs : 0;
+    // 2^32 q_groups / groups rounded up: the queries' share of the first n is n q_step / 2^32, whole at the last
+    const uint64_t groups = (uint64_t)a.large_groups + small_groups + q_groups;
+    a.q_step = static_cast<uint32_t>((((uint64_t)q_groups << 32) + groups - 1) / groups);
+    hipLaunchKernelGGL((append_f8<T, HALVES, VEC, SMALL, LARGE, UNITS>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0,
+                       stream, a);
     return hipGetLastError();
 }
 
-// Token i of the list: its keys' and values' codes times their scales, rounded once where rows are F16. A thread takes 8
-// values.
+template <typename T, bool HALVES, bool VEC>
+int launch(const F8Args &a, hipStream_t stream) {
+    const int units = a.units_per_head.d << a.block_log2;                 // of a whole block, up to 2048
+    if (units <= 16) return launch_groups<T, HALVES, VEC, 16, 0, 1>(a, stream);
+    if (units <= 32) return launch_groups<T, HALVES, VEC, 32, 0, 1>(a, stream);
+    if (units <= 64) return launch_groups<T, HALVES, VEC, 64, 0, 1>(a, stream);
+    if (units <= 256) return launch_groups<T, HALVES, VEC, 64, 256, 1>(a, stream);
+    if (units <= 1024) return launch_groups<T, HALVES, VEC, 64, 512, 2>(a, stream);
+    return launch_groups<T, HALVES, VEC, 64, 1024, 2>(a, stream);
+}
+
+// Tokens of the list: their keys' and values' codes times their scales, rounded once where rows are F16. A wave takes one
+// token, or a part of its codes, kAhead pieces of N codes a lane with all loads ahead of the stores, which are whole 16-byte
+// pieces side by side. Bound by the bytes.
+constexpr int kAhead = 8;
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void read_f8(F8Args a, T *k_out, T *v_out) {
-    const int64_t number = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (number >= a.items) return;
-    const uint32_t item = a.units_per_head.div(static_cast<uint32_t>(number));
-    const int u = static_cast<uint32_t>(number) - item * a.units_per_head.d;
-    const int token = a.heads_per_token.div(item), hk = item - token * a.heads_per_token.d;
-    const bool is_k = hk < a.pool.heads;
-    const int h = is_k ? hk : hk - a.pool.heads;
+    constexpr int N = 16 / sizeof(T);
+    const uint32_t item = blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if (item >= a.items) return;
+    const int token = a.heads_per_token.div(item), part = item - token * a.heads_per_token.d, lane = threadIdx.x % kWave;
     const Place at = place_of(a, token);
     if (at.out) {
-        if (at.bad && hk == 0 && u == 0) kk::report(a.status, kk::kBadIndex);
+        if (at.bad && part == 0 && lane == 0) kk::report(a.status, kk::kBadIndex);
         return;
     }
-    int page;
-    if (!page_of(a, at, page)) {
-        if (hk == 0 && u == 0) kk::report(a.status, kk::kBadPage);
+    const int page = page_of(a, at);
+    if (!in_pool(a, page)) {
+        if (part == 0 && lane == 0) kk::report(a.status, kk::kBadPage);
         return;
     }
     const int within = at.pos - a.pool.per_page.div(at.pos) * a.pool.page_tokens;
-    const float scale = (is_k ? a.k_scales : a.v_scales)[((int64_t)page * a.pool.heads + h) * a.blocks + (within >> a.block_log2)];
-    const uint8_t *codes = (is_k ? a.k_pool : a.v_pool) + page * a.pool.page_stride + h * a.pool.head_stride +
-                           within * a.pool.token_stride + u * 8;
-    float x[8];
-    eight_values(*reinterpret_cast<const uint2 *>(codes), scale, x);
-    T *to = (is_k ? k_out + token * a.k_stride : v_out + token * a.v_stride) + h * a.pool.width + u * 8;
-    if constexpr (VEC) {
-        constexpr int N = 16 / sizeof(T);
+    const int64_t row = page * a.pool.page_stride + within * a.pool.token_stride;
+    const int64_t scales = (int64_t)page * a.pool.heads * a.blocks + (within >> a.block_log2);
+    const int pieces = a.units_per_head.d, all = 2 * a.pool.heads * pieces;        // pieces of N codes of a head, of the token
+    uint2 codes[kAhead];
+    float scale[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; i += N) kk::store_values<T, N>(to + i, x, i);
-    } else {
+    for (int n = 0; n < kAhead; ++n) {
+        const int x = min((part * kAhead + n) * kWave + lane, all - 1);
+        const int hk = a.units_per_head.div(x), piece = x - hk * pieces;
+        const bool is_k = hk < a.pool.heads;
+        const int h = is_k ? hk : hk - a.pool.heads;
+        const uint8_t *from = (is_k ? a.k_pool : a.v_pool) + row + h * a.pool.head_stride + piece * N;
+        if constexpr (N == 4) codes[n] = make_uint2(*reinterpret_cast<const uint32_t *>(from), 0);
+        else codes[n] = *reinterpret_cast<const uint2 *>(from);
+        scale[n] = (is_k ? a.k_scales : a.v_scales)[scales + (int64_t)h * a.blocks];
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) to[i] = static_cast<T>(x[i]);
+    for (int n = 0; n < kAhead; ++n) {
+        const int x = (part * kAhead + n) * kWave + lane;
+        if (x >= all) break;
+        const int hk = a.units_per_head.div(x), piece = x - hk * pieces;
+        const bool is_k = hk < a.pool.heads;
+        float y[8];
+        eight_values(codes[n], scale[n], y);
+        T *to = (is_k ? k_out + token * a.k_stride + hk * a.pool.width
+                      : v_out + token * a.v_stride + (hk - a.pool.heads) * a.pool.width) + piece * N;
+        if constexpr (VEC) {
+            kk::store_values<T, N>(to, y, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) to[i] = static_cast<T>(y[i]);
+        }
     }
 }
 
@@ -397,10 +492,9 @@ extern "C" int kk_kv_append_f8(void *k_pool, void *v_pool, float *k_scales, floa
     a.query_heads = static_cast<int>(query_heads);
     a.rotary = p.rotary;
     a.positions = p.positions;
-    a.q_units_per_token = kk::FastDiv(static_cast<uint32_t>(query_heads ? query_heads * per_head : 1));
-    a.q_units = static_cast<uint32_t>(query_heads * per_head * p.tokens);
-    a.q_groups = (a.q_units + kThreads - 1) / kThreads;
-    a.items = (int64_t)p.tokens * 2 * c.heads;
+    const int64_t query_groups = (query_heads + kQueryHeads - 1) / kQueryHeads;
+    a.q_units_per_token = kk::FastDiv(static_cast<uint32_t>(query_heads ? query_groups * per_head : 1));
+    a.q_units = static_cast<uint32_t>(query_groups * per_head * p.tokens);
     const bool f16 = p.type == kunlun::InputType::f16, halves = p.pairs == kunlun::RotaryPairs::halves;
     // loads and stores of 4 values: rows on 4 values, the rotated part whole units
     const int64_t strides = p.k_stride | p.v_stride | (q ? p.q_stride | p.q_out_stride : 0);
@@ -422,11 +516,15 @@ extern "C" int kk_kv_read_f8(void *k_out, void *v_out, const void *k_pool, const
                        p.row_pages, status);
     a.k_stride = p.k_stride;
     a.v_stride = p.v_stride;
-    a.items = (int64_t)p.tokens * 2 * c.heads * (c.width / 8);
-    if (a.items > INT32_MAX - 1024) return hipErrorInvalidValue;
+    if ((int64_t)p.tokens * 2 * c.heads * (c.width / 8) > INT32_MAX - 1024) return hipErrorInvalidValue;
     const bool f16 = p.type == kunlun::InputType::f16;
     const bool vec = ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0 && (p.k_stride | p.v_stride) % (f16 ? 8 : 4) == 0;
-    const dim3 grid(static_cast<unsigned>((a.items + kThreads - 1) / kThreads));
+    // pieces of 16 bytes of a row; parts of a token that a wave takes
+    const int pieces = c.width / (f16 ? 8 : 4), parts = (2 * c.heads * pieces + kAhead * kWave - 1) / (kAhead * kWave);
+    a.units_per_head = kk::FastDiv(pieces);
+    a.heads_per_token = kk::FastDiv(parts);
+    a.items = static_cast<uint32_t>(p.tokens * parts);
+    const dim3 grid((a.items + kThreads / kWave - 1) / (kThreads / kWave));
     _Float16 *kh = static_cast<_Float16 *>(k_out), *vh = static_cast<_Float16 *>(v_out);
     float *kf = static_cast<float *>(k_out), *vf = static_cast<float *>(v_out);
     if (f16 && vec) hipLaunchKernelGGL((read_f8<_Float16, true>), grid, dim3(kThreads), 0, stream, a, kh, vh);
