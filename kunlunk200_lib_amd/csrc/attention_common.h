@@ -18,7 +18,6 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kStep = 32;                // tokens of a wave's step
-constexpr int kRowSteps = 1;             // what beginning a row counts in a share
 constexpr float kWeightScale = 16384.0f; // of the weights' F16 parts
 constexpr float kLeastPart = 0x1p-24f;    // the least F16 above 0
 
@@ -236,7 +235,7 @@ __device__ __forceinline__ int sum_to_lane(int v) {
 }
 
 // The part of one workgroup of attend_even: of all steps in the order (sequence, four heads, step), `left` from `at` on.
-// A row's first kRowSteps steps are empty: what it costs to begin it.
+// A row's first ROW_STEPS steps are empty: what it costs to begin it.
 struct Share {
     int at, left;
     int s, four, step;                               // where `at` is
@@ -247,16 +246,22 @@ struct Share {
     }
 };
 
-__device__ __forceinline__ Share share_of(const AttendArgs &a, int number, int fours, int lane, bool tell) {
+// Sequence s's length as a lane reads it.
+__device__ __forceinline__ int lane_length(const AttendArgs &a, int s, bool tell) {
+    int len = a.lengths[s];
+    if (len < 0 || len > a.longest) {
+        if (tell) kk::report(a.status, kk::kBadIndex);
+        len = len < 0 ? 0 : a.longest;
+    }
+    return len;
+}
+
+template <int ROW_STEPS, typename Length>
+__device__ __forceinline__ Share share_of(const AttendArgs &a, int number, int fours, int lane, Length length) {
     auto steps = [&](int s) {
         if (s >= a.sequences) return 0;
-        int len = a.lengths[s];
-        if (len < 0 || len > a.longest) {
-            if (tell) kk::report(a.status, kk::kBadIndex);
-            len = len < 0 ? 0 : a.longest;
-        }
-        const int n = steps_of(a, len);
-        return n ? (n + kRowSteps) * fours : 0;
+        const int n = steps_of(a, length(s));
+        return n ? (n + ROW_STEPS) * fours : 0;
     };
     const int mine = steps(lane), mine_to_lane = sum_to_lane(mine);        // of the first 64 sequences; more are read twice
     int total = __builtin_amdgcn_readlane(mine_to_lane, kWave - 1);

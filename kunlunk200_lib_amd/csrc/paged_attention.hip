@@ -51,6 +51,7 @@ constexpr int kMinChunk = kWaves * kStep;
 constexpr int kMaxChunk = 512, kMaxChunkMany = 1024;
 constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
+constexpr int kRowSteps = 1;             // what beginning a row counts in a share
 constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even goes through
 constexpr float kLeastWeight = 0x1p100f;  // p times this is above kLeastPart for every normal p
 
@@ -373,7 +374,8 @@ __global__ __launch_bounds__(kThreads, 1) void attend_even(AttendArgs a) {
     const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, G = lane >> 4;
     const int fours = a.pool.heads / kWaves, heads = a.group;
-    const Share share = share_of(a, blockIdx.x, fours, lane, blockIdx.x == 0 && wave == 0);
+    const Share share = share_of<kRowSteps>(a, blockIdx.x, fours, lane,
+                                            [&](int s) { return lane_length(a, s, blockIdx.x == 0 && wave == 0); });
     if (share.left == 0 || share.step + share.left <= kRowSteps) return;     // (or ends among a row's empty steps)
 
     // what a share has of one row

@@ -13,6 +13,11 @@
 // Rows. A lane's part of a K row is one run of bytes (piece G * D32 + d of 8 values in place of d * 4 + G: the sum over a
 // row's values has no order), so that 16-byte loads fetch it; q is taken in the same order.
 //
+// What bounds it: reading codes (2 * width bytes per token and head, and 8 / block_tokens of scales). 32 sequences of 32768 tokens
+// x 8 heads 335 us, 6.4 TB/s, what a kernel that only reads reaches; below, a launch's chains of latencies (some 6 us), the
+// beginnings of rows and the join's launch (4.5) stand beside it: 1 x 32768 16.8 us and 4.4 (the codes alone 10.2), 64 ragged to
+// 2048 x 8 heads 39 (21). A second step's rows on their way changed nothing that paid: 335 -> 346, 39 -> 45 us.
+//
 // Weights. w_t vs_t has the scales' range, not that of [0, 1]: it is multiplied by a power of two (`lift`) that takes the
 // largest one so far to [2^13, 2^14) before it is split into F16 parts, and the sums move along when that one grows, as
 // they do with m. So a weight times its scale is held to 2^-22 of itself or 2^-39 of the largest, whichever is more.
@@ -30,6 +35,7 @@ constexpr int kMinChunk = kWaves * kStep;
 constexpr int kMaxChunk = 512, kMaxChunkMany = 1024;
 constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
+constexpr int kRowSteps = 2;             // what beginning a row counts in a share (64 ragged to 2048 x 8 heads 40.0 us, 1: 44.0)
 constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even_f8 goes through
 constexpr int kLift = 13;                // exponent of the largest weight times its scale, as F16 parts
 
@@ -66,9 +72,12 @@ __device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const floa
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         float sc[8], p[8], top = -INFINITY, heaviest = 0.0f;
-        whole_scores(scores[nt], undo[nt], c, sc);
+        // a factor above 1 (queries of a thousand and more) joins the scale, so that no partial product is infinite or
+        // rounded to nothing where the score is not
+        whole_scores(scores[nt], fminf(undo[nt], 1.0f), c, sc);
+        const float more = fmaxf(undo[nt], 1.0f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sc[i] *= ks[i];
+        for (int i = 0; i < 8; ++i) sc[i] *= ks[i] * more;
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sc[i] = there(i) ? sc[i] : -INFINITY;
@@ -482,7 +491,8 @@ __global__ __launch_bounds__(kThreads) void attend_even_f8(AttendF8Args a) {
     const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int c = lane & 15, G = lane >> 4;
     const int fours = a.pool.heads / kWaves, heads = a.group;
-    const Share share = share_of(a, blockIdx.x, fours, lane, blockIdx.x == 0 && wave == 0);
+    const Share share = share_of<kRowSteps>(a, blockIdx.x, fours, lane,
+                                            [&](int s) { return lane_length(a, s, blockIdx.x == 0 && wave == 0); });
     if (share.left == 0 || share.step + share.left <= kRowSteps) return;     // (or ends among a row's empty steps)
 
     // what a share has of one row
@@ -678,6 +688,10 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     r.tiles = (r.group + 8 * r.nt - 1) / (8 * r.nt);
     const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
+    // The rules are the F16 cache's (rows whole on eight waves or four, parts of one size, equal shares), whose chains of
+    // latencies they balance and which are the same here; measured for this cache (us): 1 x 32768 tokens x 8 heads in parts of
+    // 512 21.3, of 256 24.5; 64 x 1024 x 8 whole 25.3 ragged and 28.9 full, in shares 26.7 and 35.1; 200 x 700 x 8 whole 45.3,
+    // in shares 47.6, on eight waves 64.8.
     const int whole = kMaxChunk + kStep;             // a window starts up to kStep - 1 tokens early
     r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
              longest <= (rows > cus / 2 ? 2 * whole : whole);
@@ -695,7 +709,11 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int64_t parts = std::max(std::min(asked, most_parts), id_parts), chunk = (longest + parts - 1) / parts;
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
-    r.narrow = r.nt == 1 && rows > 2 * cus && longest <= 4 * kStep;
+    // One wave to a workgroup for many rows of up to four steps, or eight where the rows are very many or four waves' registers
+    // leave a CU to one workgroup (us on four waves and on one, 250 tokens ragged: 512 sequences x 8 heads 52.3 / 45.6; 300 x 4
+    // heads of 256 37.6 / 30.6; but 300 x 8 of 64 20.8 / 22.9, and 80 x 8, full rows, 14.3 / 18.1)
+    const bool eight = c.width > 128 || (c.width > 64 && rows > 8 * cus);
+    r.narrow = r.nt == 1 && rows > 2 * cus && longest <= (eight ? 8 : 4) * kStep;
     r.once = r.tiles == 1 && (int64_t)p.sequences * longest * c.heads * c.width * 2 > (64 << 20);
     const bool together = c.head_stride < c.token_stride;
     const bool share_whole = !r.wide && (c.width > 128 ? longest > kMaxChunk : together && longest > 6 * kMinChunk);
@@ -704,7 +722,9 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
         (c.width % 64 == 0 || c.width == 96) && p.sequences <= kMostEven &&
         (p.sequences > 1 || (int64_t)longest * c.heads * c.width * 2 > (256 << 20)) &&
         (int64_t)p.sequences * c.heads * (longest / kStep + 3) < INT32_MAX)
-        r.shares = 2 * cus;
+        // two workgroups to a CU, whose registers allow it up to width 128 (64 sequences ragged to 2048 x 8 heads of 128 39.1 us,
+        // one 45.5; 32 x 32768 335 and 398; three, which spill, 375; 4 heads of 256 one 48.3, two 55.6)
+        r.shares = c.width <= 128 ? 2 * cus : cus;
     return r;
 }
 
@@ -723,9 +743,11 @@ hipError_t launch_tiles(const AttendF8Args &a, const Plan &p, int sequences, int
     if (!p.halves) return launch<D32, VW, NT, false, false, false, kEach, WAVES>(a, p, sequences, heads, stream);
     if (a.pool.width != 32 * D32) return launch<D32, VW, NT, true, false, false, kEach, WAVES>(a, p, sequences, heads, stream);
     if constexpr (WAVES == kWaves) {
-        if (p.once && a.block_log2 >= 4) return launch<D32, VW, NT, true, true, true, kSixteen, WAVES>(a, p, sequences, heads, stream);
-        if (p.once && a.block_log2 >= 2) return launch<D32, VW, NT, true, true, true, kFour, WAVES>(a, p, sequences, heads, stream);
-        if (p.once) return launch<D32, VW, NT, true, true, true, kEach, WAVES>(a, p, sequences, heads, stream);
+        if (p.once) {
+            if (a.block_log2 >= 4) return launch<D32, VW, NT, true, true, true, kSixteen, WAVES>(a, p, sequences, heads, stream);
+            if (a.block_log2 >= 2) return launch<D32, VW, NT, true, true, true, kFour, WAVES>(a, p, sequences, heads, stream);
+            return launch<D32, VW, NT, true, true, true, kEach, WAVES>(a, p, sequences, heads, stream);
+        }
     }
     if (a.block_log2 >= 4) return launch<D32, VW, NT, true, true, false, kSixteen, WAVES>(a, p, sequences, heads, stream);
     if (a.block_log2 >= 2) return launch<D32, VW, NT, true, true, false, kFour, WAVES>(a, p, sequences, heads, stream);
@@ -736,9 +758,10 @@ template <int D32, int VW>
 hipError_t launch_width(const AttendF8Args &a, const Plan &p, int sequences, int heads, hipStream_t stream) {
     if (p.shares) {                                  // before any other choice: the join reads what only this kernel writes
         if (a.pool.width != 32 * D32 || !p.halves || p.nt != 1) return hipErrorInvalidValue;
-        if (a.block_log2 >= 4) hipLaunchKernelGGL((attend_even_f8<D32, VW, kSixteen>), dim3(p.shares), dim3(kThreads), 0, stream, a);
-        else if (a.block_log2 >= 2) hipLaunchKernelGGL((attend_even_f8<D32, VW, kFour>), dim3(p.shares), dim3(kThreads), 0, stream, a);
-        else hipLaunchKernelGGL((attend_even_f8<D32, VW, kEach>), dim3(p.shares), dim3(kThreads), 0, stream, a);
+        const dim3 grid(p.shares), threads(kThreads);
+        if (a.block_log2 >= 4) hipLaunchKernelGGL((attend_even_f8<D32, VW, kSixteen>), grid, threads, 0, stream, a);
+        else if (a.block_log2 >= 2) hipLaunchKernelGGL((attend_even_f8<D32, VW, kFour>), grid, threads, 0, stream, a);
+        else hipLaunchKernelGGL((attend_even_f8<D32, VW, kEach>), grid, threads, 0, stream, a);
         return hipGetLastError();
     }
     if (p.narrow) return launch_tiles<D32, VW, 1, 1>(a, p, sequences, heads, stream);
