@@ -297,8 +297,8 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan(PagesArgs a, const int
 }
 
 // Fork i: its first workgroup releases the child's pages and writes the child's row,
-// the others copy the tokens of the parent's last page, and their scales.
-template <typename V>
+// the others copy the tokens of the parent's last page, SCALED: and their scales.
+template <typename V, bool SCALED>
 __global__ __launch_bounds__(kCopyThreads) void fork_apply(PagesArgs a, const int *children, const ForkNote *notes,
                                                            const int *rows) {
     const int i = blockIdx.y;
@@ -340,14 +340,14 @@ __global__ __launch_bounds__(kCopyThreads) void fork_apply(PagesArgs a, const in
     for (int b = blockIdx.x - 1; b < blocks; b += gridDim.x - 1) {
         const int head = b % a.pool.heads, pool = b / a.pool.heads % 2, layer = b / a.pool.heads / 2;
         const int64_t base = layer * a.layer_stride + head * a.pool.head_stride;
-        char *const values = pool ? a.v : a.k;
-        const int64_t src = base + page * a.pool.page_stride, dst = base + note.page * a.pool.page_stride;
+        const V *src = vector_at<V>(pool ? a.v : a.k, base + page * a.pool.page_stride);
+        V *dst = vector_at<V>(pool ? a.v : a.k, base + note.page * a.pool.page_stride);
         for (int x = threadIdx.x; x < vectors; x += kCopyThreads) {
             const int token = a.per_row.div(x), at = x - token * row_vectors;
-            const int64_t off = token * a.pool.token_stride + at * 8;
-            *vector_at<V>(values, dst + off) = *vector_at<V>(values, src + off);
+            const int64_t off = token * (a.pool.token_stride / 8) + at;
+            dst[off] = src[off];
         }
-        if (a.k_scales) {
+        if constexpr (SCALED) {
             const float *from_scales = a.scales_of(pool, layer, page) + head * a.blocks;
             float *to_scales = a.scales_of(pool, layer, note.page) + head * a.blocks;
             for (int x = threadIdx.x; x * a.block_tokens < rest; x += kCopyThreads) to_scales[x] = from_scales[x];
@@ -464,22 +464,23 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan(const int *referenc
 // `parts`. DENSE: a page is one run of values.
 template <bool DENSE, typename V>
 __device__ __forceinline__ void copy_page(const PagesArgs &a, char *pool, int64_t layer, int src, int dst, int part, int parts) {
-    const int64_t from = layer + src * a.pool.page_stride, to = layer + dst * a.pool.page_stride;
+    const V *from = vector_at<V>(pool, layer + src * a.pool.page_stride);
+    V *to = vector_at<V>(pool, layer + dst * a.pool.page_stride);
     const int row_vectors = a.pool.width / 8;
     // up to 1024 x 65536 x 32 vectors
     const uint32_t vectors = static_cast<uint32_t>(a.pool.heads) * a.pool.page_tokens * row_vectors;
     for (uint32_t x = part * kCopyThreads + threadIdx.x; x < vectors; x += parts * kCopyThreads) {
-        int64_t off = (int64_t)x * 8;
+        int64_t off = x;
         if constexpr (!DENSE) {
             const uint32_t row = a.per_row.div(x), head = a.pool.per_page.div(row), token = row - head * a.pool.page_tokens;
-            off = head * a.pool.head_stride + token * a.pool.token_stride + (x - row * row_vectors) * 8;
+            off = head * (a.pool.head_stride / 8) + token * (a.pool.token_stride / 8) + (x - row * row_vectors);
         }
-        *vector_at<V>(pool, to + off) = *vector_at<V>(pool, from + off);
+        to[off] = from[off];
     }
 }
 
 // Pages sources[i] -> destinations[i], i < *count: work items are (pair, layer, pool, part).
-template <bool DENSE, typename V>
+template <bool DENSE, typename V, bool SCALED>
 __device__ __forceinline__ void copy_pairs(const PagesArgs &a, const int *sources, const int *destinations, int count,
                                            int parts, int item, int step) {
     const int per_pair = a.layers * 2 * parts;
@@ -494,7 +495,7 @@ __device__ __forceinline__ void copy_pairs(const PagesArgs &a, const int *source
             continue;
         }
         copy_page<DENSE, V>(a, pool ? a.v : a.k, layer * a.layer_stride, src, dst, part, parts);
-        if (a.k_scales && part == 0) {
+        if (SCALED && part == 0) {
             const float *from = a.scales_of(pool, layer, src);
             float *to = a.scales_of(pool, layer, dst);
             for (int x = threadIdx.x; x < a.page_scales(); x += kCopyThreads) to[x] = from[x];
@@ -502,20 +503,20 @@ __device__ __forceinline__ void copy_pairs(const PagesArgs &a, const int *source
     }
 }
 
-template <bool DENSE, typename V>
+template <bool DENSE, typename V, bool SCALED>
 __global__ __launch_bounds__(kCopyThreads) void copy_pages(PagesArgs a, const int *sources, const int *destinations,
                                                            int count, int parts) {
-    copy_pairs<DENSE, V>(a, sources, destinations, count, parts, blockIdx.x, gridDim.x);
+    copy_pairs<DENSE, V, SCALED>(a, sources, destinations, count, parts, blockIdx.x, gridDim.x);
 }
 
 // The first `groups` workgroups rewrite the table and the counts, the others move the pages.
-template <bool DENSE, typename V>
+template <bool DENSE, typename V, bool SCALED>
 __global__ __launch_bounds__(kCopyThreads) void compact_apply(PagesArgs a, const int *table, const int *references,
                                                               int *references_out, const int *used, const int *moves,
                                                               const int *holes, const int *movers, const int *fate,
                                                               int parts, int groups) {
     if (static_cast<int>(blockIdx.x) >= groups) {
-        copy_pairs<DENSE, V>(a, movers, holes, *moves, parts, blockIdx.x - groups, gridDim.x - groups);
+        copy_pairs<DENSE, V, SCALED>(a, movers, holes, *moves, parts, blockIdx.x - groups, gridDim.x - groups);
         return;
     }
     const int u = *used;
@@ -608,7 +609,7 @@ void add_scales(PagesArgs &a, float *k_scales, float *v_scales, const kunlun::KV
     a.blocks = f8.cache.page_tokens / f8.block_tokens;
 }
 
-template <typename V>
+template <typename V, bool SCALED>
 int fork(const PagesArgs &a, const int *parents, const int *children, int count, void *workspace, hipStream_t stream) {
     ForkNote *notes = static_cast<ForkNote *>(workspace);
     int *found = reinterpret_cast<int *>(notes + count), *rows = found + count;
@@ -617,11 +618,11 @@ int fork(const PagesArgs &a, const int *parents, const int *children, int count,
                        found, rows, far_claims);
     // at most eight (layer, pool, head) blocks of the last page per workgroup
     const int blocks = a.layers * 2 * a.pool.heads, copiers = std::max(1, std::min(blocks, 4096 / count));
-    hipLaunchKernelGGL(fork_apply<V>, dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);
+    hipLaunchKernelGGL((fork_apply<V, SCALED>), dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);
     return hipGetLastError();
 }
 
-template <typename V>
+template <typename V, bool SCALED>
 int compact(const PagesArgs &a, bool dense, int parts, int *references_out, int *used, const int *table,
             const int *references, void *workspace, int cus, hipStream_t stream) {
     const int pages = a.pool.pages;
@@ -632,23 +633,25 @@ int compact(const PagesArgs &a, bool dense, int parts, int *references_out, int 
     const int groups = std::min(std::max(a.sequences, (pages + 4 * kCopyThreads - 1) / (4 * kCopyThreads)), 256);
     const dim3 grid(groups + 8 * cus);
     if (dense)
-        hipLaunchKernelGGL((compact_apply<true, V>), grid, dim3(kCopyThreads), 0, stream, a, table, references,
+        hipLaunchKernelGGL((compact_apply<true, V, SCALED>), grid, dim3(kCopyThreads), 0, stream, a, table, references,
                            references_out, used, moves, holes, movers, fate, parts, groups);
     else
-        hipLaunchKernelGGL((compact_apply<false, V>), grid, dim3(kCopyThreads), 0, stream, a, table, references,
+        hipLaunchKernelGGL((compact_apply<false, V, SCALED>), grid, dim3(kCopyThreads), 0, stream, a, table, references,
                            references_out, used, moves, holes, movers, fate, parts, groups);
     return hipGetLastError();
 }
 
-template <typename V>
+template <typename V, bool SCALED>
 int copy(const PagesArgs &a, bool dense, int parts, const int *sources, const int *destinations, int count, int cus,
          hipStream_t stream) {
     const int64_t items = (int64_t)count * a.layers * 2 * parts;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(items, 8 * cus)));
     if (dense)
-        hipLaunchKernelGGL((copy_pages<true, V>), grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
+        hipLaunchKernelGGL((copy_pages<true, V, SCALED>), grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count,
+                           parts);
     else
-        hipLaunchKernelGGL((copy_pages<false, V>), grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count, parts);
+        hipLaunchKernelGGL((copy_pages<false, V, SCALED>), grid, dim3(kCopyThreads), 0, stream, a, sources, destinations, count,
+                           parts);
     return hipGetLastError();
 }
 
@@ -674,7 +677,7 @@ extern "C" size_t kk_kv_fork_workspace_bytes(const kunlun::KVPagesLayout &p, int
 extern "C" int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *references, const int *parents, const int *children,
                int count, const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
                hipStream_t stream) {
-    return fork<uint4>(args_of(k, v, table, lengths, references, c, p, status), parents, children, count, workspace, stream);
+    return fork<uint4, false>(args_of(k, v, table, lengths, references, c, p, status), parents, children, count, workspace, stream);
 }
 extern "C" int kk_kv_fork_f8(void *k, void *v, float *k_scales, float *v_scales, int *table, int *lengths, int *references,
                   const int *parents, const int *children, int count, const kunlun::KVCacheF8Layout &f8,
@@ -682,8 +685,8 @@ extern "C" int kk_kv_fork_f8(void *k, void *v, float *k_scales, float *v_scales,
     const F8View view = view_of(f8.cache, p);
     PagesArgs a = args_of(k, v, table, lengths, references, view.cache, view.pages, status);
     add_scales(a, k_scales, v_scales, f8);
-    return view.pairs ? fork<uint4>(a, parents, children, count, workspace, stream)
-                      : fork<uint2>(a, parents, children, count, workspace, stream);
+    return view.pairs ? fork<uint4, true>(a, parents, children, count, workspace, stream)
+                      : fork<uint2, true>(a, parents, children, count, workspace, stream);
 }
 
 extern "C" int kk_kv_free(int *table, int *lengths, int *references, const int *rows, int count, const kunlun::KVCacheLayout &c,
@@ -700,7 +703,7 @@ extern "C" int kk_kv_compact(void *k, void *v, int *table_out, int *references_o
                   const int *lengths, const int *references, const kunlun::KVCacheLayout &c,
                   const kunlun::KVPagesLayout &p, void *workspace, int *status, int cus, hipStream_t stream) {
     const PagesArgs a = args_of(k, v, table_out, const_cast<int *>(lengths), nullptr, c, p, status);
-    return compact<uint4>(a, dense(c), parts_of(c, 2), references_out, used, table, references, workspace, cus, stream);
+    return compact<uint4, false>(a, dense(c), parts_of(c, 2), references_out, used, table, references, workspace, cus, stream);
 }
 extern "C" int kk_kv_compact_f8(void *k, void *v, float *k_scales, float *v_scales, int *table_out, int *references_out,
                      int *used, const int *table, const int *lengths, const int *references,
@@ -709,16 +712,15 @@ extern "C" int kk_kv_compact_f8(void *k, void *v, float *k_scales, float *v_scal
     const F8View view = view_of(f8.cache, p);
     PagesArgs a = args_of(k, v, table_out, const_cast<int *>(lengths), nullptr, view.cache, view.pages, status);
     add_scales(a, k_scales, v_scales, f8);
-    const int parts = parts_of(f8.cache, 1);
-    return view.pairs ? compact<uint4>(a, dense(view.cache), parts, references_out, used, table, references, workspace, cus, stream)
-                      : compact<uint2>(a, dense(view.cache), parts, references_out, used, table, references, workspace, cus, stream);
+    const auto run = view.pairs ? compact<uint4, true> : compact<uint2, true>;
+    return run(a, dense(view.cache), parts_of(f8.cache, 1), references_out, used, table, references, workspace, cus, stream);
 }
 
 extern "C" int kk_kv_copy_pages(void *k, void *v, const int *sources, const int *destinations, int count,
                      const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, int *status, int cus,
                      hipStream_t stream) {
     const PagesArgs a = args_of(k, v, nullptr, nullptr, nullptr, c, p, status);
-    return copy<uint4>(a, dense(c), parts_of(c, 2), sources, destinations, count, cus, stream);
+    return copy<uint4, false>(a, dense(c), parts_of(c, 2), sources, destinations, count, cus, stream);
 }
 extern "C" int kk_kv_copy_pages_f8(void *k, void *v, float *k_scales, float *v_scales, const int *sources,
                         const int *destinations, int count, const kunlun::KVCacheF8Layout &f8, const kunlun::KVPagesLayout &p,
@@ -726,7 +728,6 @@ extern "C" int kk_kv_copy_pages_f8(void *k, void *v, float *k_scales, float *v_s
     const F8View view = view_of(f8.cache, p);
     PagesArgs a = args_of(k, v, nullptr, nullptr, nullptr, view.cache, view.pages, status);
     add_scales(a, k_scales, v_scales, f8);
-    const int parts = parts_of(f8.cache, 1);
-    return view.pairs ? copy<uint4>(a, dense(view.cache), parts, sources, destinations, count, cus, stream)
-                      : copy<uint2>(a, dense(view.cache), parts, sources, destinations, count, cus, stream);
+    const auto run = view.pairs ? copy<uint4, true> : copy<uint2, true>;
+    return run(a, dense(view.cache), parts_of(f8.cache, 1), sources, destinations, count, cus, stream);
 }
