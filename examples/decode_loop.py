@@ -1,13 +1,15 @@
 """A decoding loop over the paged key-value cache: a small Llama-like model with Q4_0 weights (random
 ones, since the loop is the point) decodes several prompts at once, continues one of them in three ways, gives the
-finished sequences' pages back and compacts the pool.
+finished sequences' pages back and compacts the pool. With --block-tokens the cache holds 8 bits a value and a scale
+for each block of so many tokens and head, with the operators of that cache (kv_append_f8, paged_attention_f8, ...).
 
 Each step takes one token of every row: room for it (kv_reserve), then per layer the QKV
 product, its rotation and storage (kv_append), attention over the pages (paged_attention), the output product and the
 feed-forward block, then the LM head and the penalties on its logits (process_logits).
 
-Run on a machine with the library built:  python examples/decode_loop.py
+Run on a machine with the library built:  python examples/decode_loop.py [--block-tokens 16]
 """
+import argparse
 import os
 import sys
 
@@ -56,14 +58,23 @@ class Weights:
 
 
 class Decoder:
-    def __init__(self, c, weights):
+    def __init__(self, c, weights, block_tokens=0):
         self.c, self.w, self.kernel = c, weights, kl.Kernel()
         pool = c.heads * c.page_tokens * c.width                       # values of a page
         self.cache = kl.KVCacheLayout(c.pages, c.page_tokens, c.heads, c.width, pool, c.page_tokens * c.width, c.width)
         self.pages = kl.KVPagesLayout(c.rows, c.row_pages, c.layers, c.pages * pool)
-        self.layer_bytes = c.pages * pool * 2
-        zeros = np.zeros(c.layers * c.pages * pool, np.float16)
+        self.layer_bytes = c.pages * pool * (1 if block_tokens else 2)
+        zeros = np.zeros(c.layers * self.layer_bytes, np.uint8)
         self.k, self.v = upload(zeros), upload(zeros)
+        # 8-bit pools: their scales, and the cache's layout with the block's size in the page operations' arguments
+        self.pools, self.eight_bit, self.scale_layer = (self.k, self.v), bool(block_tokens), 0
+        self.page_cache = self.cache
+        if block_tokens:
+            self.cache8 = self.page_cache = kl.KVCacheF8Layout(self.cache, block_tokens)
+            ones = np.ones(c.layers * c.pages * c.heads * (c.page_tokens // block_tokens), np.float32)
+            self.k_scales, self.v_scales = upload(ones), upload(ones)
+            self.scale_layer = ones.nbytes // c.layers
+            self.pools += (self.k_scales, self.v_scales)
         self.table = upload(np.full((c.rows, c.row_pages), -1, np.int32))
         self.lengths = upload(np.zeros(c.rows, np.int32))
         self.references = upload(np.zeros(c.pages, np.int32))
@@ -127,10 +138,19 @@ class Decoder:
         self._norm(self.h, self.x)
         kl.matmul(kernel, DEVICE, self.qkv, w["qkv"], self.h, c.hidden, c.qkv, c.rows, q4)
         at = self.qkv.data
-        kl.require(kl.kv_append(kernel, DEVICE, k, v, self.q, at, at + q_bytes, at + q_bytes + kv_bytes, self.every_row,
-                                position, None, self.table, self.cosine, self.sine, self.cache, self.append))
-        kl.require(kl.paged_attention(kernel, DEVICE, self.attended, self.q, k, v, self.table, self.lengths, self.cache,
-                                      self.attend))
+        if self.eight_bit:
+            ks, vs = self.k_scales.data + i * self.scale_layer, self.v_scales.data + i * self.scale_layer
+            kl.require(kl.kv_append_f8(kernel, DEVICE, k, v, ks, vs, self.q, at, at + q_bytes, at + q_bytes + kv_bytes,
+                                       self.every_row, position, None, self.table, self.cosine, self.sine, self.cache8,
+                                       self.append))
+            kl.require(kl.paged_attention_f8(kernel, DEVICE, self.attended, self.q, k, v, ks, vs, self.table,
+                                             self.lengths, self.cache8, self.attend))
+        else:
+            kl.require(kl.kv_append(kernel, DEVICE, k, v, self.q, at, at + q_bytes, at + q_bytes + kv_bytes,
+                                    self.every_row, position, None, self.table, self.cosine, self.sine, self.cache,
+                                    self.append))
+            kl.require(kl.paged_attention(kernel, DEVICE, self.attended, self.q, k, v, self.table, self.lengths,
+                                          self.cache, self.attend))
         kl.matmul(kernel, DEVICE, self.y, w["o"], self.attended, c.query_heads * c.width, c.hidden, c.rows, q4)
         self._add(self.x, self.x, self.y)
         self._norm(self.h, self.x)
@@ -157,8 +177,9 @@ class Decoder:
     def fork(self, parents, children):
         """children[i] goes on where parents[i] stands."""
         p, c = upload(np.array(parents, np.int32)), upload(np.array(children, np.int32))
-        kl.require(kl.kv_fork(self.kernel, DEVICE, self.k, self.v, self.table, self.lengths, self.references, p, c,
-                              len(parents), self.cache, self.pages))
+        fork = kl.kv_fork_f8 if self.eight_bit else kl.kv_fork
+        kl.require(fork(self.kernel, DEVICE, *self.pools, self.table, self.lengths, self.references, p, c, len(parents),
+                        self.page_cache, self.pages))
         kl.require(kl.kv_cache_status(DEVICE) == 0)
         histories = [list(self.history[i]) for i in parents]
         for child, h in zip(children, histories):
@@ -175,8 +196,9 @@ class Decoder:
     def compact(self):
         """Moves the used pages to the low end; how many there are."""
         used = upload(np.zeros(1, np.int32))
-        kl.require(kl.kv_compact(self.kernel, DEVICE, self.k, self.v, self.table, self.references, used, self.table,
-                                 self.lengths, self.references, self.cache, self.pages))
+        compact = kl.kv_compact_f8 if self.eight_bit else kl.kv_compact
+        kl.require(compact(self.kernel, DEVICE, *self.pools, self.table, self.references, used, self.table, self.lengths,
+                           self.references, self.page_cache, self.pages))
         kl.require(kl.kv_cache_status(DEVICE) == 0)
         return int(used.download(1, np.int32)[0])
 
@@ -215,8 +237,10 @@ def run(c, decoder, prompts, steps, observe=lambda tokens, logits: None):
 
 
 def main():
+    parser = argparse.ArgumentParser()
+    parser.add_argument("--block-tokens", type=int, default=0, help="tokens to a scale of an 8-bit cache (0: F16)")
     c = Config()
-    decoder = Decoder(c, Weights(c, 1))
+    decoder = Decoder(c, Weights(c, 1), parser.parse_args().block_tokens)
     rng = np.random.default_rng(2)
     prompts = [list(rng.integers(2, c.vocabulary, n)) for n in (20, 7, 33, 16)]
     for row, tokens in enumerate(run(c, decoder, prompts, 24)):

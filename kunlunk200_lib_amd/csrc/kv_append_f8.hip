@@ -328,7 +328,8 @@ __device__ __forceinline__ void store_window(const F8Args &a, uint32_t item, int
     int turn = 0;
     for (uint64_t left = of_group(in_wave < size && here.s >= 0 && !here.same(last)); left; left &= left - 1) {
         const int at = __builtin_ctzll(left);
-        const Entry x{__shfl(here.s, shift + at, kWave), __shfl(here.lag, shift + at, kWave), __shfl(here.block, shift + at, kWave)};
+        const Entry x{__shfl(here.s, shift + at, kWave), __shfl(here.lag, shift + at, kWave),
+                      __shfl(here.block, shift + at, kWave)};
         const uint64_t window_has = of_group(x.same(here));
         // (it follows a left-out entry: an earlier one begins its block)
         if (of_group(x.same(before)) || window_has & ((uint64_t(1) << at) - 1)) continue;
@@ -347,7 +348,8 @@ template <typename T, bool HALVES, bool VEC, int SMALL, int LARGE, int UNITS>
 __global__ __launch_bounds__(LARGE ? LARGE : kThreads) void append_f8(F8Args a) {
     constexpr int kGroup = LARGE ? LARGE : kThreads;
     __shared__ uint32_t tops[2][kMostWaves];
-    const uint32_t queries = __umulhi(blockIdx.x, a.q_step), number = blockIdx.x - queries;    // of the workgroups before this one
+    const uint32_t queries = __umulhi(blockIdx.x, a.q_step);    // of the workgroups before this one
+    const uint32_t number = blockIdx.x - queries;
     if (__umulhi(blockIdx.x + 1, a.q_step) != queries) {
         turn_queries<T, HALVES, VEC>(a, queries * kGroup + threadIdx.x);
     } else if (LARGE > 0 && number < a.large_groups) {

@@ -618,7 +618,8 @@ int fork(const PagesArgs &a, const int *parents, const int *children, int count,
                        found, rows, far_claims);
     // at most eight (layer, pool, head) blocks of the last page per workgroup
     const int blocks = a.layers * 2 * a.pool.heads, copiers = std::max(1, std::min(blocks, 4096 / count));
-    hipLaunchKernelGGL((fork_apply<V, SCALED>), dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes, rows);
+    hipLaunchKernelGGL((fork_apply<V, SCALED>), dim3(1 + copiers, count), dim3(kCopyThreads), 0, stream, a, children, notes,
+                       rows);
     return hipGetLastError();
 }
 
@@ -677,7 +678,8 @@ extern "C" size_t kk_kv_fork_workspace_bytes(const kunlun::KVPagesLayout &p, int
 extern "C" int kk_kv_fork(void *k, void *v, int *table, int *lengths, int *references, const int *parents, const int *children,
                int count, const kunlun::KVCacheLayout &c, const kunlun::KVPagesLayout &p, void *workspace, int *status,
                hipStream_t stream) {
-    return fork<uint4, false>(args_of(k, v, table, lengths, references, c, p, status), parents, children, count, workspace, stream);
+    return fork<uint4, false>(args_of(k, v, table, lengths, references, c, p, status), parents, children, count, workspace,
+                              stream);
 }
 extern "C" int kk_kv_fork_f8(void *k, void *v, float *k_scales, float *v_scales, int *table, int *lengths, int *references,
                   const int *parents, const int *children, int count, const kunlun::KVCacheF8Layout &f8,

@@ -13,8 +13,8 @@
 // Rows. A lane's part of a K row is one run of bytes (piece G * D32 + d of 8 values in place of d * 4 + G: the sum over a
 // row's values has no order), so that 16-byte loads fetch it; q is taken in the same order.
 //
-// What bounds it: reading codes (2 * width bytes per token and head, and 8 / block_tokens of scales). 32 sequences of 32768 tokens
-// x 8 heads 335 us, 6.4 TB/s, what a kernel that only reads reaches; below, a launch's chains of latencies (some 6 us), the
+// What bounds it: reading codes (2 * width bytes per token and head, and 8 / block_tokens of scales). 32 sequences of 32768
+// tokens x 8 heads 335 us, 6.4 TB/s, what a kernel that only reads reaches; below, a launch's chains of latencies (some 6 us), the
 // beginnings of rows and the join's launch (4.5) stand beside it: 1 x 32768 16.8 us and 4.4 (the codes alone 10.2), 64 ragged to
 // 2048 x 8 heads 39 (21). A second step's rows on their way changed nothing that paid: 335 -> 346, 39 -> 45 us.
 //
@@ -72,12 +72,12 @@ __device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const floa
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         float sc[8], p[8], top = -INFINITY, heaviest = 0.0f;
-        // a factor above 1 (queries of a thousand and more) joins the scale, so that no partial product is infinite or
-        // rounded to nothing where the score is not
+        // a factor above 1 (queries of a thousand and more) comes after the scale: no partial product is infinite where the
+        // score is not, nor rounded to nothing but where that is next to nothing of a score
         whole_scores(scores[nt], fminf(undo[nt], 1.0f), c, sc);
         const float more = fmaxf(undo[nt], 1.0f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sc[i] *= ks[i] * more;
+        for (int i = 0; i < 8; ++i) sc[i] = sc[i] * ks[i] * more;
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sc[i] = there(i) ? sc[i] : -INFINITY;
