@@ -110,27 +110,27 @@ __device__ __forceinline__ float both_parts(float high) {
     return fabsf(high) == INFINITY ? high : high + low;
 }
 
-// Eight values of a row of q (16-byte loads where a.q_wide allows).
-__device__ __forceinline__ void load_query(const AttendArgs &a, int64_t at, float (&v)[8]) {
+// Eight values of a row of q (16-byte loads where a.q_wide allows); F16 as they are in the first four registers, so that
+// nothing waits for them here.
+__device__ __forceinline__ void load_query(const AttendArgs &a, int64_t at, float4v (&v)[2]) {
     if (a.f16) {
         const _Float16 *q = static_cast<const _Float16 *>(a.q) + at;
         if (a.q_wide) {
-            const half8 x = *reinterpret_cast<const half8 *>(q);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(x[i]);
+            v[0] = *reinterpret_cast<const float4v *>(q);
         } else {
+            half8 x;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(q[i]);
+            for (int i = 0; i < 8; ++i) x[i] = q[i];
+            v[0] = __builtin_bit_cast(float4v, x);
         }
     } else {
         const float *q = static_cast<const float *>(a.q) + at;
         if (a.q_wide) {
-            const float4v x = *reinterpret_cast<const float4v *>(q), y = *reinterpret_cast<const float4v *>(q + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = x[i], v[i + 4] = y[i];
+            v[0] = *reinterpret_cast<const float4v *>(q);
+            v[1] = *reinterpret_cast<const float4v *>(q + 4);
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = q[i];
+            v[0] = float4v{q[0], q[1], q[2], q[3]};
+            v[1] = float4v{q[4], q[5], q[6], q[7]};
         }
     }
 }
@@ -146,10 +146,26 @@ __device__ __forceinline__ T load_row(const void *p) {
 __device__ __forceinline__ int exponent_of(float v) { return static_cast<int>((__float_as_uint(v) >> 23) & 0xff) - 127; }
 
 // q columns: column c is head c % 8 of each tile, its high (c < 8) or low part; the scores times `undo` are in base 2.
-// in(d): whether the lane's piece d of a row is within the width.
+// in(d): whether the lane's piece d of a row is within the width. `loaded`: as load_query left it.
 template <int D32, int NT, typename In>
-__device__ __forceinline__ void split_queries(float scale_log2, int heads, int c, In in, const float (&q)[NT][D32][8],
-                                              half8 (&qf)[NT][D32], float (&undo)[NT]) {
+__device__ __forceinline__ void split_queries(bool f16, float scale_log2, int heads, int c, In in,
+                                              const float4v (&loaded)[NT][D32][2], half8 (&qf)[NT][D32], float (&undo)[NT]) {
+    float q[NT][D32][8];
+    if (f16) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int d = 0; d < D32; ++d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[nt][d][i] = static_cast<float>(__builtin_bit_cast(half8, loaded[nt][d][0])[i]);
+    } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int d = 0; d < D32; ++d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[nt][d][i] = loaded[nt][d][i / 4][i % 4];
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const bool column = nt * 8 + (c & 7) < heads;

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
     // a part past the sequence's end, before it asks for anything
     if (chunk > 0 && a.window == 0 && chunk * a.chunk >= scalar_load(a.lengths + s)) return;
     // the queries' values are on their way while the sequence's length and pages are read
-    float q[NT][D32][8];
+    float4v q[NT][D32][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int h = nt * 8 + (c & 7);
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
 
     half8 qf[NT][D32];
     float undo[NT];
-    split_queries<D32, NT>(a.scale_log2, heads, c, [&](int d) { return FULL || d * 32 + G * 8 < width; }, q, qf, undo);
+    split_queries<D32, NT>(a.f16, a.scale_log2, heads, c, [&](int d) { return FULL || d * 32 + G * 8 < width; }, q, qf, undo);
 
     float4v acc[NT][VW];
     float m[NT], l[NT];
@@ -367,7 +367,8 @@ __global__ __launch_bounds__(WAVES * kWave) void attend(AttendArgs a) {
 // Four waves with a step on its way each keep up with the memory (two workgroups to a CU: 172 for 165 with 64 x 4096 head by
 // head; width 64: 91 for 95). A new row costs a chain of latencies - length, page, rows - of some 4 us: the next row is
 // looked up while this one's first rows are on their way, its first rows are asked for behind this one's last scores, and
-// beginning it counts as a step of a share (64 sequences ragged to 2048 x 8 heads: 63 us without all that, 58 with).
+// beginning it counts as a step of a share (64 sequences ragged to 2048 x 8 heads: 63 us without all that, 58 with; 55
+// with F16 queries not waited for piece by piece).
 template <int D32, int VW>
 __global__ __launch_bounds__(kThreads, 1) void attend_even(AttendArgs a) {
     constexpr int VP = VW < 8 ? VW : 8, VR = VW / 2, width = 32 * D32;
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(kThreads, 1) void attend_even(AttendArgs a) {
                 }
             }
     };
-    float q[1][D32][8];
+    float4v q[1][D32][2];
     auto load_queries = [&](const Run &r) {
         const int64_t at = r.s * a.q_stride + (int64_t)((r.four * kWaves + wave) * a.group + (c & 7) % heads) * width;
 #pragma unroll
@@ -476,7 +477,7 @@ __global__ __launch_bounds__(kThreads, 1) void attend_even(AttendArgs a) {
     float undo[1], m[1], l[1];
     float4v acc[1][VW];
     auto start = [&] {
-        split_queries<D32, 1>(a.scale_log2, heads, c, [](int) { return true; }, q, qf, undo);
+        split_queries<D32, 1>(a.f16, a.scale_log2, heads, c, [](int) { return true; }, q, qf, undo);
         m[0] = -INFINITY;
         l[0] = 0.0f;
 #pragma unroll

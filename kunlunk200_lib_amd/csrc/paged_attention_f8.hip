@@ -15,8 +15,8 @@
 //
 // What bounds it: reading codes (2 * width bytes per token and head, and 8 / block_tokens of scales). 32 sequences of 32768
 // tokens x 8 heads 335 us, 6.4 TB/s, what a kernel that only reads reaches; below, a launch's chains of latencies (some 6 us), the
-// beginnings of rows and the join's launch (4.5) stand beside it: 1 x 32768 16.8 us and 4.4 (the codes alone 10.2), 64 ragged to
-// 2048 x 8 heads 39 (21). A second step's rows on their way changed nothing that paid: 335 -> 346, 39 -> 45 us.
+// beginnings of rows and the join's launch (4.5) stand beside it: 1 x 32768 15.7 us and 4.3 (the codes alone 10.2), 64 ragged
+// to 2048 x 8 heads 39 (21). A second step's rows on their way changed nothing that paid: 335 -> 346, 39 -> 45 us.
 //
 // Weights. w_t vs_t has the scales' range, not that of [0, 1]: it is multiplied by a power of two (`lift`) that takes the
 // largest one so far to [2^13, 2^14) before it is split into F16 parts, and the sums move along when that one grows, as
@@ -25,6 +25,7 @@
 #include "launch.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend_f8(AttendF8Args a) {
     // a part past the sequence's end, before it asks for anything
     if (chunk > 0 && a.window == 0 && chunk * a.chunk >= scalar_load(a.lengths + s)) return;
     // the queries' values are on their way while the sequence's length and pages are read
-    float q[NT][D32][8];
+    float4v q[NT][D32][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int h = nt * 8 + (c & 7);
@@ -353,20 +354,9 @@ __global__ __launch_bounds__(WAVES * kWave) void attend_f8(AttendF8Args a) {
     };
 
     int t0 = begin + wave * kStep;
-    const bool any = t0 < end;
-    Halves here{}, next{};
-    if (any) {
-        if constexpr (UNI) here = find_halves(a, row, kvh, t0, lo, hi, lane);
-        load_k(t0, here);
-        load_scales(t0, here);
-        load_v(t0, here);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-
+    Halves here{};
     half8 qf[NT][D32];
     float undo[NT];
-    split_queries<D32, NT>(a.scale_log2, heads, c, in, q, qf, undo);
-
     float4v acc[NT][VW];
     float m[NT], l[NT], most[NT], lift[NT];
 #pragma unroll
@@ -378,10 +368,14 @@ __global__ __launch_bounds__(WAVES * kWave) void attend_f8(AttendF8Args a) {
         for (int j = 0; j < VW; ++j) acc[nt][j] = float4v{0, 0, 0, 0};
     }
 
-    if (any) for (;;) {
+    // A step, with the loads of the next one or without. All loads stand in straight lines: where ways with and without
+    // them meet, a wait for older loads has to wait for these too. (With that, and the first V rows asked for after the
+    // queries are in parts, 200 ragged to 700 x 8 heads 46.5 -> 43 us, 64 to 1024 25.9 -> 23.5, 8 to 4096 19.6 -> 17.7.)
+    auto step = [&](auto more) {
+        constexpr bool kMore = decltype(more)::value;
         const int t1 = t0 + WAVES * kStep;
-        const bool more = t1 < end;
-        if constexpr (UNI) if (more) next = find_halves(a, row, kvh, t1, lo, hi, lane);
+        Halves next{};
+        if constexpr (UNI && kMore) next = find_halves(a, row, kvh, t1, lo, hi, lane);
         // a step with tokens that are not the chunk's, or whose page is missing
         const bool masked = t0 < lo || t0 + kStep > end || (UNI ? !(here.ok[0] && here.ok[1]) : holes);
         auto there = [&](int i) {
@@ -409,7 +403,7 @@ __global__ __launch_bounds__(WAVES * kWave) void attend_f8(AttendF8Args a) {
         // the next step's K rows are on their way during the weights and the second product, its V rows
         // during the next scores
         __builtin_amdgcn_sched_barrier(0);
-        if (more) {
+        if constexpr (kMore) {
             load_k(t1, next);
             load_scales(t1, next);
         }
@@ -426,12 +420,25 @@ __global__ __launch_bounds__(WAVES * kWave) void attend_f8(AttendF8Args a) {
             }
         }
         add_codes<VW, NT>(vr, pf, acc);
-        if (!more) break;
+        if constexpr (kMore) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(t1, next);
+            __builtin_amdgcn_sched_barrier(0);
+            t0 = t1;
+            here = next;
+        }
+    };
+    if (t0 < end) {
+        if constexpr (UNI) here = find_halves(a, row, kvh, t0, lo, hi, lane);
+        load_k(t0, here);
+        load_scales(t0, here);
         __builtin_amdgcn_sched_barrier(0);
-        load_v(t1, next);
+        split_queries<D32, NT>(a.f16, a.scale_log2, heads, c, in, q, qf, undo);
         __builtin_amdgcn_sched_barrier(0);
-        t0 = t1;
-        here = next;
+        load_v(t0, here);
+        __builtin_amdgcn_sched_barrier(0);
+        while (t0 + WAVES * kStep < end) step(std::true_type());
+        step(std::false_type());
     }
     if constexpr (!UNI) __syncthreads();             // page_ids are read; the sums go over them
 
@@ -545,7 +552,7 @@ __global__ __launch_bounds__(kThreads) void attend_even_f8(AttendF8Args a) {
             load_value<VW, true, true>(static_cast<const uint8_t *>(a.v) + w.at[i / 4] + (i & 3) * a.pool.token_stride + v_lane,
                                        c, width, vr[i]);
     };
-    float q[1][D32][8];
+    float4v q[1][D32][2];
     auto load_queries = [&](const Run &r) {
         const int64_t at = r.s * a.q_stride + (int64_t)((r.four * kWaves + wave) * a.group + (c & 7) % heads) * width;
 #pragma unroll
@@ -563,7 +570,7 @@ __global__ __launch_bounds__(kThreads) void attend_even_f8(AttendF8Args a) {
     float undo[1], m[1], l[1], most[1], lift[1];
     float4v acc[1][VW];
     auto start = [&] {
-        split_queries<D32, 1>(a.scale_log2, heads, c, [](int) { return true; }, q, qf, undo);
+        split_queries<D32, 1>(a.f16, a.scale_log2, heads, c, [](int) { return true; }, q, qf, undo);
         m[0] = -INFINITY;
         l[0] = most[0] = 0.0f;
         lift[0] = 1.0f;
@@ -690,7 +697,7 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
     // The rules are the F16 cache's (rows whole on eight waves or four, parts of one size, equal shares), whose chains of
     // latencies they balance and which are the same here; measured for this cache (us): 1 x 32768 tokens x 8 heads in parts of
-    // 512 21.3, of 256 24.5; 64 x 1024 x 8 whole 25.3 ragged and 28.9 full, in shares 26.7 and 35.1; 200 x 700 x 8 whole 45.3,
+    // 512 21.3, of 256 24.5; 64 x 1024 x 8 whole 23.5 ragged and 27.3 full, in shares 26.7 and 35.1; 200 x 700 x 8 whole 43,
     // in shares 47.6, on eight waves 64.8.
     const int whole = kMaxChunk + kStep;             // a window starts up to kStep - 1 tokens early
     r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
