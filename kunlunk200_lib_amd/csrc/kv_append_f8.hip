@@ -53,6 +53,7 @@ struct F8Args {
     uint32_t q_step;                     // the queries' share of all workgroups, of 2^32
     int window;                          // append: entries that a group of lanes looks through
     uint32_t items;                      // append: windows x heads_per_token; read: tokens x parts of one
+    uint32_t first;                      // read: the launch's first item
 };
 
 // Where token i goes: its sequence and position, or why it goes nowhere.
@@ -396,10 +397,11 @@ int launch(const F8Args &a, hipStream_t stream) {
 // pieces side by side. Bound by the bytes: 35000 tokens of 8 heads to F32, 359 MB, 77 us (by 8 codes a thread, every thread
 // with its own look-ups, 107).
 constexpr int kAhead = 8;
+constexpr uint32_t kLaunchItems = 1u << 25;          // of one launch, 2^31 threads: it has to stay below 2^32
 template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void read_f8(F8Args a, T *k_out, T *v_out) {
     constexpr int N = 16 / sizeof(T);
-    const uint32_t item = blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t item = a.first + blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (item >= a.items) return;
     const int token = a.heads_per_token.div(item), part = item - token * a.heads_per_token.d, lane = threadIdx.x % kWave;
     const Place at = place_of(a, token);
@@ -532,12 +534,15 @@ extern "C" int kk_kv_read_f8(void *k_out, void *v_out, const void *k_pool, const
     a.units_per_head = kk::FastDiv(pieces);
     a.heads_per_token = kk::FastDiv(parts);
     a.items = static_cast<uint32_t>(p.tokens * parts);
-    const dim3 grid((a.items + kThreads / kWave - 1) / (kThreads / kWave));
     _Float16 *kh = static_cast<_Float16 *>(k_out), *vh = static_cast<_Float16 *>(v_out);
     float *kf = static_cast<float *>(k_out), *vf = static_cast<float *>(v_out);
-    if (f16 && vec) hipLaunchKernelGGL((read_f8<_Float16, true>), grid, dim3(kThreads), 0, stream, a, kh, vh);
-    else if (f16) hipLaunchKernelGGL((read_f8<_Float16, false>), grid, dim3(kThreads), 0, stream, a, kh, vh);
-    else if (vec) hipLaunchKernelGGL((read_f8<float, true>), grid, dim3(kThreads), 0, stream, a, kf, vf);
-    else hipLaunchKernelGGL((read_f8<float, false>), grid, dim3(kThreads), 0, stream, a, kf, vf);
-    return hipGetLastError();
+    for (a.first = 0; a.first < a.items; a.first += kLaunchItems) {
+        const dim3 grid((std::min(a.items - a.first, kLaunchItems) + kThreads / kWave - 1) / (kThreads / kWave));
+        if (f16 && vec) hipLaunchKernelGGL((read_f8<_Float16, true>), grid, dim3(kThreads), 0, stream, a, kh, vh);
+        else if (f16) hipLaunchKernelGGL((read_f8<_Float16, false>), grid, dim3(kThreads), 0, stream, a, kh, vh);
+        else if (vec) hipLaunchKernelGGL((read_f8<float, true>), grid, dim3(kThreads), 0, stream, a, kf, vf);
+        else hipLaunchKernelGGL((read_f8<float, false>), grid, dim3(kThreads), 0, stream, a, kf, vf);
+        if (const hipError_t rc = hipGetLastError()) return rc;
+    }
+    return hipSuccess;
 }
