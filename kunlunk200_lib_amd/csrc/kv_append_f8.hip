@@ -2,7 +2,7 @@
 // queries and keys turned by their position's angles on the way, and tokens read back out of it.
 //
 // Storing. A block's scale is the least power of two 2^e, e >= -64, that takes the largest value of its new tokens to at most
-// 448, the codes' largest, or the scale that its earlier tokens have, where that is larger; where it grows the
+// 448, the codes' largest, or the scale that its earlier tokens have, where that is as large in size; where it grows the
 // earlier codes move down with it. By powers of two that loses nothing above the subnormal codes (2^-6 of the scale and
 // below), so a block filled token by token holds what it would hold filled at once, up to those. A value is rounded
 // once: keys are turned in F64, where products of F32 factors are exact, and reach F32 rounded to odd, so that rounding
@@ -255,8 +255,9 @@ __device__ __forceinline__ void store_block(const F8Args &a, int token, int s, i
     float scale = least_scale(top);
     if (earlier > 0) {
         const float old = *scale_at;
-        if (!(old <= scale) && scale == scale) scale = old;               // (a scale that is not a number stays)
-        if (scale > old) {
+        const bool grows = fabsf(old) < scale;                            // sizes: another producer's scale may be negative
+        if (!grows && scale == scale) scale = old;                        // (one that is not a number stays)
+        if (grows) {
             const float down = old / scale;
             for (int number = lane; number < earlier * units; number += GROUP) {
                 const int j = a.units_per_head.div(number);

@@ -4,9 +4,10 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from kv_f8 import CacheF8, finish, upload
+from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, run_append, upload
 
 pytestmark = pytest.mark.gpu
+HALVES = kl.RotaryPairs.halves
 
 
 def test_read_of_the_longest_lists(gpu):
@@ -28,4 +29,46 @@ def test_read_of_the_longest_lists(gpu):
             for buffer, pool in ((k, "k"), (v, "v")):
                 want = cache.values(pool)[0, 0, 0, position[first:first + n]].astype(np.float16)
                 assert np.array_equal(buffer.download((n, 8), np.float16, offset=first * 16), want)
+    assert gpu.kv_cache_status(0) == 0
+
+
+def append_behind(cache, page, at, k, v):
+    """The model of one new token behind others of its block at place `at` of a page, with any finite scale there: kept where
+    it is at least as large in size as the new value needs, else the codes move to the least power of two."""
+    block = cache.layout.block_tokens
+    b, earlier = at // block, slice(at // block * block, at)
+    for codes, scales, x in ((cache.k, cache.ks, k), (cache.v, cache.vs, v)):
+        for h in range(cache.layout.cache.heads):
+            old, need = float(scales[0, page, h, b]), float(least_scale(np.abs(x[h]).max()))
+            scale = old if abs(old) >= need else need
+            if scale != old:
+                codes[0, page, h, earlier] = encode(VALUES[codes[0, page, h, earlier]] * old / scale)
+            scales[0, page, h, b] = scale
+            # (a quotient in 64 bits is on a tie between codes only where the exact one is)
+            codes[0, page, h, at] = encode(x[h].astype(np.float64) / scale)
+
+
+@pytest.mark.parametrize("block", [2, 16, 64])
+def test_append_behind_negative_scales(gpu, block):
+    """Scales of either sign, smaller and larger than the new token's and equal to it."""
+    rng = np.random.default_rng(6001)
+    heads, width, page_tokens, rows = 3, 64, 64, 24
+    cache = CacheF8(rng, rows, page_tokens, heads, width, block)
+    for scales in cache.scales:
+        scales[...] = rng.choice([-1, 1], scales.shape) * 2.0 ** rng.integers(-12, 0, scales.shape)
+    model, at = cache.copy(), np.where(np.arange(rows) % 2, block - 1, block * (page_tokens // block - 1) + 1)
+    # needs of 2^-12 to 2^-1
+    top = 448 * 2.0 ** rng.integers(-12, 0, (2, rows, heads, 1))
+    k, v = (rng.uniform(-1, 1, (2, rows, heads, width)) * top).astype(np.float32)
+    for x, t in ((k, top[0]), (v, top[1])):
+        x[:, :, 5] = t[:, :, 0]
+    for row in range(rows):
+        append_behind(model, row, at[row], k[row], v[row])
+    cache.upload()
+    table = np.arange(rows, dtype=np.int32)[:, None]
+    run_append(cache, table, np.arange(rows), at, None, k, v, (), (), HALVES, 0)
+    cache.download()
+    old = cache.scales[0][0, np.arange(rows), :, at // block]
+    assert (old < 0).any() and (old > 0).any()
+    assert cache.same_as(model)
     assert gpu.kv_cache_status(0) == 0
