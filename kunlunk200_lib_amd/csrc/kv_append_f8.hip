@@ -188,6 +188,14 @@ __device__ __forceinline__ void eight_values(uint2 codes, float scale, float (&x
     x[0] = a[0] * scale, x[1] = a[1] * scale, x[2] = b[0] * scale, x[3] = b[1] * scale;
     x[4] = c[0] * scale, x[5] = c[1] * scale, x[6] = d[0] * scale, x[7] = d[1] * scale;
 }
+// A product to F32, rounded to odd: a code times a scale has up to 28 bits, and rounded to the nearest F32 first, 6 in 10^5 of
+// them would reach F16 one step off. (The remainder is not exact for products below 2^-125, which are 0 in F16.)
+__device__ __forceinline__ float times_to_odd(float a, float b) {
+    const float y = a * b, rest = fmaf(a, b, -y);
+    if (rest == 0.0f || !(fabsf(y) < INFINITY)) return y;
+    const uint32_t bits = __float_as_uint(y);
+    return __uint_as_float((bits - ((bits ^ __float_as_uint(rest)) >> 31)) | 1u);
+}
 
 // The new tokens of a block, one head of keys or values, by GROUP lanes that hold UNITS units each: entries token + j for
 // the bits j of `members`, of which the first stands at sequence s and position pos.
@@ -439,7 +447,11 @@ __global__ __launch_bounds__(kThreads) void read_f8(F8Args a, T *k_out, T *v_out
         const int hk = a.units_per_head.div(x), piece = x - hk * pieces;
         const bool is_k = hk < a.pool.heads;
         float y[8];
-        eight_values(codes[n], scale[n], y);
+        eight_values(codes[n], N == 8 ? 1.0f : scale[n], y);
+        if constexpr (N == 8) {                                           // F16 rows round once
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = times_to_odd(y[i], scale[n]);
+        }
         T *to = (is_k ? k_out + token * a.k_stride + hk * a.pool.width
                       : v_out + token * a.v_stride + (hk - a.pool.heads) * a.pool.width) + piece * N;
         if constexpr (VEC) {

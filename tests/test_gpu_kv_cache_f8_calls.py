@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, run_append, upload
+from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, run_append, run_read, upload
 
 pytestmark = pytest.mark.gpu
 HALVES = kl.RotaryPairs.halves
@@ -72,3 +72,26 @@ def test_append_behind_negative_scales(gpu, block):
     assert (old < 0).any() and (old > 0).any()
     assert cache.same_as(model)
     assert gpu.kv_cache_status(0) == 0
+
+
+@pytest.mark.parametrize("width", [8, 128])
+def test_read_rounds_any_scale_once(gpu, width):
+    """F16 rows beside scales of 24 bits: products whose nearest F32 lies on a tie between two F16 numbers, which the exact ones
+    do not; of every size from F16's subnormals to past its range, of both signs."""
+    rng = np.random.default_rng(6002)
+    pages, page_tokens, heads = 64, 64, 128 // width * 4
+    cache = CacheF8(rng, pages, page_tokens, heads, width, 1)
+    for flat, scales in zip(cache.flat, cache.scales):
+        flat[...] = rng.integers(0, 127, flat.shape) + 128 * rng.integers(0, 2, flat.shape)
+        scales[...] = rng.choice([-1, 1], scales.shape) * rng.uniform(1, 2, scales.shape) * 2.0 ** rng.integers(-24, 9, scales.shape)
+    cache.upload()
+    n = pages * page_tokens
+    table, position = np.arange(pages, dtype=np.int32)[None, :], np.arange(n)
+    twice = 0
+    for got, pool in zip(run_read(cache, table, np.zeros(n, int), position, np.float16), "kv"):
+        exact = cache.values(pool)[0].transpose(0, 2, 1, 3).reshape(got.shape)
+        with np.errstate(over="ignore"):
+            want = exact.astype(np.float16)
+            twice += (exact.astype(np.float32).astype(np.float16) != want).sum()
+        assert np.array_equal(got, want)
+    assert twice > 20, "no product that F32 takes to a tie"
