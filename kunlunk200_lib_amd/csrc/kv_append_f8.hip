@@ -190,12 +190,18 @@ __device__ __forceinline__ void eight_values(uint2 codes, float scale, float (&x
     x[4] = c[0] * scale, x[5] = c[1] * scale, x[6] = d[0] * scale, x[7] = d[1] * scale;
 }
 // A product to F32, rounded to odd: a code times a scale has up to 28 bits, and rounded to the nearest F32 first, 6 in 10^5 of
-// them would reach F16 one step off. (The remainder is not exact for products below 2^-125, which are 0 in F16; a
-// product past F32's range becomes its largest number.)
+// them would reach F16 one step off. (The remainder is not exact for products below 2^-125, which are 0 in F16 and as codes;
+// a product past F32's range becomes its largest number.)
 __device__ __forceinline__ float times_to_odd(float a, float b) {
     const float y = a * b, rest = fmaf(a, b, -y);
     const uint32_t bits = __float_as_uint(y), odd = (bits - ((bits ^ __float_as_uint(rest)) >> 31)) | 1u;
     return fabsf(rest) > 0.0f ? __uint_as_float(odd) : y;
+}
+
+// Four codes times a factor, each rounded once.
+__device__ __forceinline__ uint32_t four_codes_times(uint32_t codes, float by) {
+    const float2v a = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
+    return four_codes(times_to_odd(a[0], by), times_to_odd(a[1], by), times_to_odd(b[0], by), times_to_odd(b[1], by));
 }
 
 // The new tokens of a block, one head of keys or values, by GROUP lanes that hold UNITS units each: entries token + j for
@@ -271,9 +277,10 @@ __device__ __forceinline__ void store_block(const F8Args &a, int token, int s, i
             for (int number = lane; number < earlier * units; number += GROUP) {
                 const int j = a.units_per_head.div(number);
                 uint2 *codes = reinterpret_cast<uint2 *>(block + j * a.pool.token_stride + (number - j * units) * 8);
-                float y[8];
-                eight_values(*codes, down, y);
-                *codes = make_uint2(four_codes(y[0], y[1], y[2], y[3]), four_codes(y[4], y[5], y[6], y[7]));
+                const uint2 old_codes = *codes;
+                const uint32_t low = four_codes_times(old_codes.x, down);
+                __builtin_amdgcn_sched_barrier(0);                        // (side by side they take 10 registers more)
+                *codes = make_uint2(low, four_codes_times(old_codes.y, down));
             }
         }
         if constexpr (GROUP > kWave) __syncthreads();                     // every wave has read the old scale

@@ -95,3 +95,34 @@ def test_read_rounds_any_scale_once(gpu, width):
             twice += (exact.astype(np.float32).astype(np.float16) != want).sum()
         assert np.array_equal(got, want)
     assert twice > 20, "no product that F32 takes to a tie"
+
+
+def test_append_rounds_earlier_codes_once(gpu):
+    """Codes that move from a scale of 24 bits to a new one: products whose nearest F32 is a tie between two codes."""
+    rng = np.random.default_rng(6003)
+    rows, heads, width = 128, 1, 128
+    cache = CacheF8(rng, rows, 16, heads, width, 16)
+    # scale = tie / code and the numbers beside it, so that code * scale is within 2^-24 of a tie in the new scale, 1
+    tie = (np.arange(8, 16) + 0.5) / 8
+    code = rng.integers(9, 120, (2, rows))
+    for scales, codes, c in zip(cache.scales, (cache.k, cache.v), code):
+        s = (rng.choice(tie, rows) * 2.0 ** rng.integers(-4, 2, rows) / VALUES[c]).astype(np.float32)
+        s = np.where(s < 0.99, s, s / 256)
+        scales[0, :, 0, 0] = [np.nextafter(x, np.float32(rng.choice([0, x, 1]))) for x in s]
+        codes[0, :, 0, :, ::2] = c[:, None, None]
+    model = cache.copy()
+    k, v = rng.uniform(-1, 1, (2, rows, heads, width)).astype(np.float32)
+    k[:, :, 0] = v[:, :, 0] = 448
+    at = np.full(rows, 9)
+    for row in range(rows):
+        append_behind(model, row, at[row], k[row], v[row])
+    twice = 0
+    for codes, scales in ((cache.k, cache.scales[0]), (cache.v, cache.scales[1])):
+        y = VALUES[codes[0, :, 0, :9]].astype(np.float32) * scales[0, :, 0, 0, None, None]
+        twice += (encode(y) != encode(VALUES[codes[0, :, 0, :9]] * scales[0, :, 0, 0, None, None].astype(np.float64))).sum()
+    assert twice > 20, "no product that F32 takes to a tie"
+    cache.upload()
+    run_append(cache, np.arange(rows, dtype=np.int32)[:, None], np.arange(rows), at, None, k, v, (), (), HALVES, 0)
+    cache.download()
+    assert cache.same_as(model)
+    assert gpu.kv_cache_status(0) == 0
