@@ -529,7 +529,8 @@ bool paged_attention_f8(Kernel &, int device, void * y, const void * q, const vo
 // two, 2^-64 or more, that takes the largest of its new tokens' values to at most 448, or what it was where the block
 // holds earlier tokens and their scale (of either sign) is no smaller in size; where it grows, the earlier tokens' codes are
 // rounded to the new one.
-// A new value is rounded once, to the nearest code of its F64 rotation (ties to the even code). A value that is not finite
+// A new value is rounded once, to the nearest code of its F64 rotation (ties to the even code; beside an earlier scale that
+// is no power of two, which only another producer leaves, of the rotation rounded to odd in F32). A value that is not finite
 // makes its block's scale, so all of the block, not a number, until the block is begun again. Tokens of one block must
 // stand in consecutive entries of consecutive positions (some of which may be left out); what the block held from the first
 // of them on is forgotten.

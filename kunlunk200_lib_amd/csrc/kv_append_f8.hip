@@ -6,7 +6,9 @@
 // earlier codes move down with it. By powers of two that loses nothing above the subnormal codes (2^-6 of the scale and
 // below), so a block filled token by token holds what it would hold filled at once, up to those. A value is rounded
 // once: keys are turned in F64, where products of F32 factors are exact, and reach F32 rounded to odd, so that rounding
-// that to a code's four bits rounds the F64 value (in F32 throughout one code in 2^19 is the neighbour of the nearest).
+// that to a code's four bits rounds the F64 value (in F32 throughout one code in 2^19 is the neighbour of the nearest). Beside
+// an earlier scale that is no power of two, which only another producer leaves, the quotient goes through F32 rounded to odd
+// too; of a turned key it is that of the F32 value, for which the F64 one would have to stay in registers.
 //
 // The first new token of a block finds which follow it. Its lanes, a wave or less for a few tokens as in decoding, a
 // workgroup of up to 1024 for more, hold all of the block's new values of one head in registers between the largest and the
@@ -198,6 +200,14 @@ __device__ __forceinline__ float times_to_odd(float a, float b) {
     return fabsf(rest) > 0.0f ? __uint_as_float(odd) : y;
 }
 
+// x / scale to F32, rounded to odd, from y = x times the scale's rounded reciprocal, which is up to 1.5 steps off: a step towards
+// the quotient, then the remainder, whose sign is exact, says on which side of it that is.
+__device__ __forceinline__ float quotient_to_odd(float x, float scale, float by) {
+    const float first = x * by, y = fmaf(fmaf(-first, scale, x), by, first), rest = fmaf(-y, scale, x);
+    const uint32_t bits = __float_as_uint(y), odd = (bits - ((bits ^ __float_as_uint(rest) ^ __float_as_uint(scale)) >> 31)) | 1u;
+    return fabsf(rest) > 0.0f ? __uint_as_float(odd) : y == first ? first : y;      // (first: 0 with its sign)
+}
+
 // Four codes times a factor, each rounded once.
 __device__ __forceinline__ uint32_t four_codes_times(uint32_t codes, float by) {
     const float2v a = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(codes, true);
@@ -287,6 +297,7 @@ __device__ __forceinline__ void store_block(const F8Args &a, int token, int s, i
     }
     if (lane == 0) *scale_at = scale;
     const float by = 1.0f / scale;
+    const bool uneven = __any(__float_as_uint(scale) << 9 && scale == scale);   // a kept scale that is no power of two
 #pragma unroll
     for (int n = 0; n < UNITS; ++n) {
         const int number = lane + n * GROUP;
@@ -295,8 +306,16 @@ __device__ __forceinline__ void store_block(const F8Args &a, int token, int s, i
         if (!(members >> j & 1)) continue;
         const Unit<T, HALVES, VEC> unit(number - j * units, rotary);
         uint8_t *to = block + (earlier + j) * a.pool.token_stride;
-        const uint32_t low = four_codes(x[n][0] * by, x[n][1] * by, x[n][2] * by, x[n][3] * by);
-        const uint32_t high = four_codes(x[n][4] * by, x[n][5] * by, x[n][6] * by, x[n][7] * by);
+        uint32_t low, high;
+        if (uneven) {
+            auto odd = [&](int i) { return quotient_to_odd(x[n][i], scale, by); };
+            low = four_codes(odd(0), odd(1), odd(2), odd(3));
+            __builtin_amdgcn_sched_barrier(0);
+            high = four_codes(odd(4), odd(5), odd(6), odd(7));
+        } else {
+            low = four_codes(x[n][0] * by, x[n][1] * by, x[n][2] * by, x[n][3] * by);
+            high = four_codes(x[n][4] * by, x[n][5] * by, x[n][6] * by, x[n][7] * by);
+        }
         if constexpr (VEC) {
             if (HALVES && unit.turned) {
                 *reinterpret_cast<uint32_t *>(to + unit.element(0)) = low;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, run_append, run_read, upload
+from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, run_append, run_read, turned, upload
 
 pytestmark = pytest.mark.gpu
 HALVES = kl.RotaryPairs.halves
@@ -124,5 +124,64 @@ def test_append_rounds_earlier_codes_once(gpu):
     cache.upload()
     run_append(cache, np.arange(rows, dtype=np.int32)[:, None], np.arange(rows), at, None, k, v, (), (), HALVES, 0)
     cache.download()
+    assert cache.same_as(model)
+    assert gpu.kv_cache_status(0) == 0
+
+
+def to_odd(x):
+    """F32 of 64-bit values, rounded to odd: towards zero, the last bit set where that is not exact."""
+    near = x.astype(np.float32)
+    bits = near.view(np.uint32) - (np.abs(near.astype(np.float64)) > np.abs(x))
+    return np.where(near == x, near, (bits.astype(np.uint32) | 1).view(np.float32))
+
+
+@pytest.mark.parametrize("block,width,rotary", [(2, 8, 0), (16, 64, 0), (16, 64, 32), (64, 256, 256)])
+def test_append_rounds_once_beside_any_scale(gpu, block, width, rotary):
+    """New values at ties between codes beside a kept scale of 24 bits, and the F32 numbers around; turned by angles so small
+    that only F64 sees them. More than one new token of a block, and blocks whose scale is a power of two among them."""
+    rng = np.random.default_rng(6004)
+    rows, heads, page_tokens, new = 40, 2, 64, min(3, block - 1)
+    cache = CacheF8(rng, rows, page_tokens, heads, width, block)
+    for scales in cache.scales:
+        scales[...] = rng.choice([-1, 1], scales.shape) * rng.uniform(0.001, 0.1, scales.shape)
+        scales[0, ::7] = 2.0 ** -8
+    model = cache.copy()
+    b = rng.integers(0, page_tokens // block, rows)
+    first = b * block + block - new
+    ties = (VALUES[:126] + VALUES[1:127]) / 2
+    x = []
+    for scales in cache.scales:
+        s = scales[0, np.arange(rows), :, b].astype(np.float64)[:, None, :, None]
+        value = (rng.choice(ties, (rows, new, heads, width)) * s).astype(np.float32)
+        x.append(np.where(rng.random(value.shape) < 0.5, np.nextafter(value, np.float32(0)), value))
+    k, v = x
+    k[3, 0, 0, 5], v[3, 0, 0, 5] = 0.0, -0.0
+    half = rotary // 2
+    position = first[:, None] + np.arange(new)
+    cos, sin = np.ones((page_tokens, half), np.float32), rng.choice([-1, 1], (page_tokens, half)).astype(np.float32) * np.float32(2 ** -20)
+    twice = 0
+    for row in range(rows):
+        at = position[row]
+        turn = np.stack([turned(y, cos[p], sin[p], HALVES) for y, p in zip(k[row], at)])
+        for codes, scales, exact in ((model.k, model.ks, turn), (model.v, model.vs, v[row].astype(np.float64))):
+            for h in range(heads):
+                old, need = float(scales[0, row, h, b[row]]), float(least_scale(np.abs(exact[:, h]).max()))
+                scale = old if abs(old) >= need else need
+                earlier = slice(b[row] * block, first[row])
+                if scale != old:
+                    codes[0, row, h, earlier] = encode(VALUES[codes[0, row, h, earlier]] * old / scale)
+                scales[0, row, h, b[row]] = scale
+                # beside a power of two the nearest code of the exact value is that of the odd F32 number
+                values = to_odd(exact[:, h])
+                codes[0, row, h, at] = encode(values.astype(np.float64) / scale)
+                rough = values * (np.float32(1) / np.float32(scale))
+                twice += (encode(rough.astype(np.float64)) != encode(values.astype(np.float64) / scale)).sum()
+    assert twice > 0, "no quotient that F32 takes to a tie"
+    cache.upload()
+    flat = lambda y: y.reshape(rows * new, heads, width)  # noqa: E731
+    run_append(cache, np.arange(rows, dtype=np.int32)[:, None], np.repeat(np.arange(rows), new), position.reshape(-1), None,
+               flat(k), flat(v), cos, sin, HALVES, rotary)
+    cache.download()
+    assert all(np.array_equal(p, q) for p, q in zip(cache.scales, model.scales))
     assert cache.same_as(model)
     assert gpu.kv_cache_status(0) == 0
