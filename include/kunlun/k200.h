@@ -413,8 +413,9 @@ const char * kv_cache_reason(const KVCacheLayout &);
 
 // What the kernels met on `device` since the last call, completing its work
 // first: 0, or a sum of 1 (a page id outside the pool; its tokens were left out),
-// 2 (a sequence, position or length out of range, or a second entry for one sequence; left out or cut) and 4 (no
-// free page: the sequence kept its length, a fork's child is empty). -1: no such device.
+// 2 (a sequence, position or length out of range, or a second entry for one sequence; left out or cut; or a block's tokens
+// apart in a list of kv_append_f8) and 4 (no free page: the sequence kept its length, a fork's child is empty). -1: no such
+// device.
 int kv_cache_status(int device);
 
 // One new token per sequence: y[s][h] = sum over tokens t of
@@ -533,7 +534,7 @@ bool paged_attention_f8(Kernel &, int device, void * y, const void * q, const vo
 // is no power of two, which only another producer leaves, of the rotation rounded to odd in F32). A value that is not finite
 // makes its block's scale, so all of the block, not a number, until the block is begun again. Tokens of one block must
 // stand in consecutive entries of consecutive positions (some of which may be left out); what the block held from the first
-// of them on is forgotten.
+// of them on is forgotten. A list that breaks this rule is reported, and the blocks concerned hold nothing of use.
 // Up to 2^31 threads: (query_heads * width / 8 + 512 * heads) * tokens.
 const char * kv_append_f8_reason(const KVCacheF8Layout &, const KVAppendLayout &);
 bool kv_append_f8(Kernel &, int device, void * k_pool, void * v_pool, float * k_scales, float * v_scales, void * q_out,

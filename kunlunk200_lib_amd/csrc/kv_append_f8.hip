@@ -33,6 +33,8 @@ constexpr int kThreads = 256;
 constexpr int kLeastExponent = -64;      // of a scale
 constexpr int kMostGroups = 2048;        // that look through one entry each
 constexpr int kMostWaves = 16;           // of a workgroup
+constexpr int kPlaces = 4096;            // of a checking workgroup's table, 16 KB: a CU's 160 hold as many workgroups as its registers
+constexpr int kCheckedAhead = 4;         // entries of a thread on their way
 
 typedef float float2v __attribute__((ext_vector_type(2)));
 
@@ -52,6 +54,7 @@ struct F8Args {
     int tokens, sequences, row_pages, query_heads, rotary, positions;
     int block_log2, blocks;              // tokens of a scale are 2^block_log2; scales of a page and head
     uint32_t q_units;                    // units of kQueryHeads query heads, of all tokens
+    uint32_t check_groups;               // workgroups that look for blocks whose tokens stand apart
     uint32_t large_groups;               // workgroups for many new tokens of a block
     uint32_t q_step;                     // the queries' share of all workgroups, of 2^32
     int window;                          // append: entries that a group of lanes looks through
@@ -377,19 +380,64 @@ __device__ __forceinline__ void store_window(const F8Args &a, uint32_t item, int
     }
 }
 
+// Tokens of one block that stand apart in the list (k200.h forbids it) would each begin the block, and chance decides whose scale
+// stays. Such a list is reported: workgroup `part` enters the first of every run of a block's tokens, where the hash of sequence
+// and block gives it this part, in a table of LDS, and finds there a run of the same block that this one does not go on from. Half
+// a table's places for a part's share of the list; were all taken, the search ends without an answer. Beside the others' work
+// (32 sequences x 32 heads 5.63 -> 5.77 us a call, a prompt of 8000 tokens no change, of 100000 803 -> 818).
+template <int THREADS>
+__device__ __forceinline__ void check_list(const F8Args &a, uint32_t part, int *places) {
+    for (int x = threadIdx.x; x < kPlaces; x += THREADS) places[x] = -1;
+    __syncthreads();
+    bool unused;
+    for (int i0 = threadIdx.x; i0 < a.tokens; i0 += kCheckedAhead * THREADS) {
+        Entry here[kCheckedAhead], last[kCheckedAhead];
+#pragma unroll
+        for (int n = 0; n < kCheckedAhead; ++n) {
+            here[n] = entry_of(a, i0 + n * THREADS, unused);
+            last[n] = entry_of(a, i0 + n * THREADS - 1, unused);
+        }
+#pragma unroll
+        for (int n = 0; n < kCheckedAhead; ++n) {
+            const Entry &x = here[n];
+            if (x.s < 0 || x.same(last[n])) continue;
+            // by the golden ratio: neighbouring sequences and blocks far apart
+            const uint64_t hash = (static_cast<uint64_t>(x.s) << 32 | static_cast<uint32_t>(x.block)) * 0x9e3779b97f4a7c15u;
+            if (__umulhi(static_cast<uint32_t>(hash >> 32), a.check_groups) != part) continue;
+            uint32_t at = static_cast<uint32_t>(hash >> 32) % kPlaces;
+            for (int tries = 0; tries < kPlaces; ++tries, at = (at + 1) % kPlaces) {
+                const int other = atomicCAS(places + at, -1, i0 + n * THREADS);
+                if (other < 0) break;
+                const Entry y = entry_of(a, other, unused);
+                if (x.s != y.s || x.block != y.block) continue;
+                if (x.lag != y.lag) kk::report(a.status, kk::kBadIndex);
+                break;
+            }
+        }
+    }
+}
+
 // The workgroups of the queries, which stream, lie evenly among those of keys and values, which wait for one another's
 // results, so that a CU holds both (2047 tokens of 32 + 8 heads of 128: 20.3 us, one kind after the other 26). Of the
-// latter first come those that take many new tokens of a block together, then those of SMALL lanes for a block's few new
-// tokens (all of them, where a whole block has no more units).
+// latter first come those that check the list, then those that take many new tokens of a block together, then those of SMALL
+// lanes for a block's few new tokens (all of them, where a whole block has no more units).
 template <typename T, bool HALVES, bool VEC, int SMALL, int LARGE, int UNITS>
 __global__ __launch_bounds__(LARGE ? LARGE : kThreads) void append_f8(F8Args a) {
     constexpr int kGroup = LARGE ? LARGE : kThreads;
     __shared__ uint32_t tops[2][kMostWaves];
+    extern __shared__ int places[];      // kPlaces where workgroups check the list
     const uint32_t queries = __umulhi(blockIdx.x, a.q_step);    // of the workgroups before this one
-    const uint32_t number = blockIdx.x - queries;
+    uint32_t number = blockIdx.x - queries;
     if (__umulhi(blockIdx.x + 1, a.q_step) != queries) {
         turn_queries<T, HALVES, VEC>(a, queries * kGroup + threadIdx.x);
-    } else if (LARGE > 0 && number < a.large_groups) {
+        return;
+    }
+    if (number < a.check_groups) {
+        check_list<kGroup>(a, number, places);
+        return;
+    }
+    number -= a.check_groups;
+    if (LARGE > 0 && number < a.large_groups) {
         if constexpr (LARGE > 0) store_window<T, HALVES, VEC, LARGE, UNITS>(a, number, 1 << a.block_log2, false, tops);
     } else {
         const uint32_t item = (number - a.large_groups) * (kGroup / SMALL) + threadIdx.x / SMALL;
@@ -409,11 +457,13 @@ int launch_groups(F8Args a, hipStream_t stream) {
     const uint32_t small_groups = (a.items * SMALL + threads - 1) / threads;
     const int windows = (a.tokens + (1 << a.block_log2) - 1) >> a.block_log2;
     a.large_groups = LARGE && (int64_t)a.tokens * units > kWave ? windows * pairs : 0;
+    // (without positions each entry is a sequence of its own)
+    a.check_groups = a.position && a.block_log2 > 0 && a.tokens > 1 ? (a.tokens + kPlaces / 2 - 1) / (kPlaces / 2) : 0;
     // 2^32 q_groups / groups rounded up: the queries' share of the first n is n q_step / 2^32, whole at the last
-    const uint64_t groups = (uint64_t)a.large_groups + small_groups + q_groups;
+    const uint64_t groups = (uint64_t)a.check_groups + a.large_groups + small_groups + q_groups;
     a.q_step = static_cast<uint32_t>((((uint64_t)q_groups << 32) + groups - 1) / groups);
-    hipLaunchKernelGGL((append_f8<T, HALVES, VEC, SMALL, LARGE, UNITS>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0,
-                       stream, a);
+    hipLaunchKernelGGL((append_f8<T, HALVES, VEC, SMALL, LARGE, UNITS>), dim3(static_cast<unsigned>(groups)), dim3(threads),
+                       a.check_groups ? kPlaces * sizeof(int) : 0, stream, a);
     return hipGetLastError();
 }
 

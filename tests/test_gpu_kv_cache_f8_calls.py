@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, run_append, run_read, turned, upload
+from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, model_append, run_append, run_read, turned, upload
 
 pytestmark = pytest.mark.gpu
 HALVES = kl.RotaryPairs.halves
@@ -185,3 +185,70 @@ def test_append_rounds_once_beside_any_scale(gpu, block, width, rotary):
     assert all(np.array_equal(p, q) for p, q in zip(cache.scales, model.scales))
     assert cache.same_as(model)
     assert gpu.kv_cache_status(0) == 0
+
+
+def lists_of_runs(rng, rows, most, block):
+    """(sequence, position) of whole and partial runs of blocks in any order, each block's tokens together; some left out."""
+    sequence, position = [], []
+    runs = [(s, b) for s in range(rows) for b in range(most // block)]
+    for r in rng.permutation(len(runs)):
+        s, b = runs[r]
+        lo, hi = sorted(rng.integers(0, block + 1, 2))
+        sequence += [s] * (hi - lo)
+        position += list(range(b * block + lo, b * block + hi))
+    out = rng.random(len(position)) < 0.1
+    return np.where(out & (rng.random(len(out)) < 0.5), -1, sequence), np.where(out, -1, position)
+
+
+@pytest.mark.parametrize("rows,most,block,width", [(7, 64, 16, 64), (60, 128, 4, 8), (3, 4096, 2, 24), (40, 128, 64, 256)])
+def test_append_blocks_in_any_order(gpu, rows, most, block, width):
+    """What the rule allows is not reported, in lists of one checking workgroup and of several."""
+    rng = np.random.default_rng(6005)
+    cache = CacheF8(rng, rows * most // 64, 64, 1, width, block)
+    table = rng.permutation(rows * most // 64).astype(np.int32).reshape(rows, -1)
+    sequence, position = lists_of_runs(rng, rows, most, block)
+    k, v = rng.standard_normal((2, len(sequence), 1, width)).astype(np.float32)
+    model = cache.copy()
+    stored, status = model_append(model, table, sequence, position, k, v, (), (), HALVES, 0)
+    assert status == 0 and stored.sum() > 100
+    cache.upload()
+    run_append(cache, table, sequence, position, None, k, v, (), (), HALVES, 0)
+    assert gpu.kv_cache_status(0) == 0
+    cache.download()
+    assert cache.same_as(model)
+
+
+@pytest.mark.parametrize("block,width,half", [(16, 128, False), (2, 64, True), (64, 256, False), (4, 8, True)])
+def test_append_reports_blocks_in_pieces(gpu, block, width, half):
+    """Tokens of one block apart in the list: sequences in turn, positions backwards, one token of a long list far off. The
+    blocks that stand together in the same call are stored as ever."""
+    rng = np.random.default_rng(6006)
+    rows, most, dtype = 90, 256, np.float16 if half else np.float32
+    cache = CacheF8(rng, rows * most // 64, 64, 1, width, block)
+    table = rng.permutation(rows * most // 64).astype(np.int32).reshape(rows, -1)
+    together = np.repeat(np.arange(2, rows), 40), np.tile(np.arange(128, 168), rows - 2)
+    n = len(together[0])
+    lists = {
+        "in turn": (np.tile([0, 1], 8), np.repeat(np.arange(8), 2)),
+        "all in turn": (np.tile(np.arange(rows), 3), np.repeat(np.arange(3), rows)),
+        "backwards": (np.zeros(9, int), np.arange(9, 0, -1)),
+        "a gap": (np.zeros(4, int), np.array([0, 1, block, 1])),
+        "far off": (np.concatenate([[0], together[0], [0]]), np.concatenate([[block - 1], together[1], [0]])),
+        "one place twice": (np.concatenate([[1], together[0], [1]]), np.concatenate([[5], together[1], [5]])),
+    }
+    for name, (sequence, position) in lists.items():
+        print(name, flush=True)
+        k, v = rng.standard_normal((2, len(sequence), 1, width)).astype(dtype)
+        model = cache.copy()
+        cache.upload()
+        run_append(cache, table, sequence, position, None, k, v, (), (), HALVES, 0)
+        assert gpu.kv_cache_status(0) == kl.KV_BAD_INDEX, name
+        assert gpu.kv_cache_status(0) == 0
+        if len(sequence) > n:
+            cache.download()
+            inside = slice(1, n + 1)
+            model_append(model, table, *together, k[inside], v[inside], (), (), HALVES, 0)
+            untouched = np.ones(rows * most // 64, bool)
+            untouched[table[:2]] = False
+            for a, b in zip((cache.k, cache.v, cache.ks, cache.vs), (model.k, model.v, model.ks, model.vs)):
+                assert np.array_equal(a[:, untouched], b[:, untouched])
