@@ -519,7 +519,9 @@ const char * kv_cache_f8_reason(const KVCacheF8Layout &);
 
 // paged_attention over such a cache, with its rules and numerics: products run on the codes, which F16 holds exactly; a
 // token's key scale multiplies its score, its value scale its weight, in F32, and the product of weight and value
-// scale is held to 2^-22 of itself or 2^-39 of the largest one. Any finite F32 scales will do. A scale or a code that is not
+// scale is held to 2^-22 of itself, 2^-38 of the largest one or 2^-149, whichever is most. Any finite F32 scales will do, within
+// F32's range: weights below 2^-126 of the largest are 0, and a row whose values, weighted and summed before they are divided by
+// the weights' sum, leave that range is infinite. A scale or a code that is not
 // a number makes the rows that read it not a number. What stands past a row's length or before its window may be anything.
 const char * paged_attention_f8_reason(const KVCacheF8Layout &, const PagedAttentionLayout &);
 bool paged_attention_f8(Kernel &, int device, void * y, const void * q, const void * k, const void * v,

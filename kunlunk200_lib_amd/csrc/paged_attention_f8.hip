@@ -20,7 +20,8 @@
 //
 // Weights. w_t vs_t has the scales' range, not that of [0, 1]: it is multiplied by a power of two (`lift`) that takes the
 // largest one so far to [2^13, 2^14) before it is split into F16 parts, and the sums move along when that one grows, as
-// they do with m. So a weight times its scale is held to 2^-22 of itself or 2^-39 of the largest, whichever is more.
+// they do with m. So a weight times its scale is held to 2^-22 of itself, 2^-38 of the largest or 2^-149, whichever is most: the
+// low part ends at half of F16's least number, 2^-25 beside a largest of 2^13, and the power at 2^126.
 #include "attention_common.h"
 #include "launch.h"
 
@@ -39,6 +40,7 @@ constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
 constexpr int kRowSteps = 2;             // what beginning a row counts in a share (64 ragged to 2048 x 8 heads 40.0 us, 1: 44.0)
 constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even_f8 goes through
 constexpr int kLift = 13;                // exponent of the largest weight times its scale, as F16 parts
+constexpr int kMostLift = 126;           // of the power that takes it there, whose reciprocal is a normal number too
 
 struct AttendF8Args : AttendArgs {
     const float *k_scales, *v_scales;
@@ -101,7 +103,7 @@ __device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const floa
             l[nt] *= alpha;
             m[nt] = top;
             most[nt] = fmaxf(most[nt] * alpha, heaviest);
-            const int from_e = exponent_of(lift[nt]), to_e = kLift - max(exponent_of(most[nt]), -100);
+            const int from_e = exponent_of(lift[nt]), to_e = min(kLift - exponent_of(most[nt]), kMostLift);
             const float change = ldexpf(alpha, to_e - from_e);
             lift[nt] = ldexpf(1.0f, to_e);
 #pragma unroll

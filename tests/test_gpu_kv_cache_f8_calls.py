@@ -4,7 +4,9 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from kv_f8 import VALUES, CacheF8, encode, finish, least_scale, model_append, run_append, run_read, turned, upload
+from kv_f8 import (VALUES, CacheF8, encode, finish, least_scale, model_append, run_append, run_attention, run_read, turned,
+                   upload)
+from test_gpu_kv_cache_f8 import KERNELS, make
 
 pytestmark = pytest.mark.gpu
 HALVES = kl.RotaryPairs.halves
@@ -252,3 +254,43 @@ def test_append_reports_blocks_in_pieces(gpu, block, width, half):
             untouched[table[:2]] = False
             for a, b in zip((cache.k, cache.v, cache.ks, cache.vs), (model.k, model.v, model.ks, model.vs)):
                 assert np.array_equal(a[:, untouched], b[:, untouched])
+
+
+# --- attention --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("exponent", [-124, -112, -100, -64, 0, 90])
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_attention_value_scales_of_any_size(gpu, case, exponent):
+    """Value scales of 24 bits about one power of two, beside keys of 0, which make every weight 1.
+
+    All but four tokens' codes are 0, so a sum has four terms that are not, each held to 2^-22 of itself, 2^-38 of the largest
+    (at most 448 / 2 of a term) or 2^-149; two parts of four terms each, their sum, the joins of up to 8 waves' and 2 parts' sums and
+    the division round fewer than 32 times, by 2^-24 each."""
+    rng, lengths, table, cache, q = make(case, 60)
+    c = cache.layout.cache
+    cache.ks[...] = 0
+    cache.vs[...] = rng.choice([-1, 1], cache.vs.shape) * rng.uniform(1, 2, cache.vs.shape) * 2.0 ** exponent
+    gold, tol = np.zeros(q.shape), np.zeros(q.shape)
+    values = cache.v.copy()
+    cache.v[...] = 0
+    shown = {}
+    for s, n in enumerate(lengths):
+        for t in rng.choice(n, min(n, 4), replace=False):
+            page, at = table[s, t // c.page_tokens], t % c.page_tokens
+            shown[page, at] = True
+            cache.v[0, page, :, at] = values[0, page, :, at]
+    for s, n in enumerate(lengths):                      # (rows may share pages: more than four terms then)
+        t = np.arange(n)
+        page, at = table[s, t // c.page_tokens], t % c.page_tokens
+        keep = np.array([(p, a) in shown for p, a in zip(page, at)])
+        v = cache.values("v")[0, page[keep], :, at[keep]]                        # [term][head][value]
+        scales = np.abs(cache.vs[0, page[keep], :, at[keep] // cache.layout.block_tokens].astype(np.float64))
+        group = q.shape[1] // c.heads
+        each = np.abs(v) * (2.0 ** -22 + 8 * len(v) * 2.0 ** -24)
+        lost = 448 * np.maximum(2.0 ** -38 * scales.max(0), 2.0 ** -149)[:, None] * len(v)
+        gold[s] = np.repeat(v.sum(0) / n, group, 0)
+        tol[s] = np.repeat((each.sum(0) + lost) / n, group, 0) + 2.0 ** -149
+    y, _ = run_attention(cache, table, lengths, q)
+    err = np.abs(y.astype(np.float64) - gold)
+    assert np.all(np.isfinite(y))
+    assert np.all(err <= tol), f"worst {np.max(err / tol):.3g} of the tolerance"
