@@ -4,9 +4,9 @@ import numpy as np
 import pytest
 
 import kunlunk200_lib_amd as kl
-from kv_f8 import (VALUES, CacheF8, encode, finish, least_scale, model_append, run_append, run_attention, run_read, turned,
-                   upload)
-from test_gpu_kv_cache_f8 import KERNELS, make
+from kv_f8 import (VALUES, CacheF8, check, encode, finish, gold_attention, least_scale, model_append, model_read, run_append,
+                   run_attention, run_read, table_of, turned, upload)
+from test_gpu_kv_cache_f8 import KERNELS, angles, check_queries, make
 
 pytestmark = pytest.mark.gpu
 HALVES = kl.RotaryPairs.halves
@@ -294,3 +294,81 @@ def test_attention_value_scales_of_any_size(gpu, case, exponent):
     err = np.abs(y.astype(np.float64) - gold)
     assert np.all(np.isfinite(y))
     assert np.all(err <= tol), f"worst {np.max(err / tol):.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("scale,size", [(30.0, 1e4), (-0.5, 1e4), (0.125, 1e6), (-3e-9, 1e14)])
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_attention_far_scores(gpu, case, scale, size):
+    """Scores of up to 10^7: where the best token is ahead by more than the scores' error and 130, the others' weights are below
+    e^-130 and y is its value row, to 2^-22 for its weight's parts and some roundings of 2^-24."""
+    _, lengths, table, cache, q = make(case, 61)
+    c, group = cache.layout.cache, q.shape[1] // cache.layout.cache.heads
+    q = (q * size).astype(np.float32)
+    y, _ = run_attention(cache, table, lengths, q, scale=scale)
+    keys, values, clear, factor = cache.values("k")[0], cache.values("v")[0], 0, abs(float(np.float32(scale)))
+    for s, n in enumerate(lengths):
+        t = np.arange(n)
+        page, at = table[s, t // c.page_tokens], t % c.page_tokens
+        for h in range(q.shape[1]):
+            k, qh = keys[page, h // group, at], q[s, h].astype(np.float64)
+            score = (k @ qh) * float(np.float32(scale))
+            error = np.abs(k * qh).sum(1).max() * factor * (2.0 ** -21 + len(qh) * 2.0 ** -24 + 2.0 ** -22)
+            best = np.argsort(score)[-2:] if n > 1 else np.array([0, 0])
+            if n > 1 and score[best[1]] - score[best[0]] <= 2 * error + 130:
+                continue
+            clear += 1
+            want = values[page[best[1]], h // group, at[best[1]]]
+            assert np.all(np.abs(y[s, h] - want) <= np.abs(want) * (2.0 ** -22 + 8 * 2.0 ** -24)), (s, h)
+    assert clear > 0.8 * q.shape[0] * q.shape[1]
+
+
+# sequences, heads, query heads, width, tokens of a page, of a block, longest, window: many rows that one wave takes each, of up
+# to eight steps, above width 128, with widths that are no multiple of 32, page ids in LDS and two column tiles
+NARROW = [(1100, 2, 2, 128, 16, 16, 250, 0), (1100, 2, 4, 120, 16, 4, 250, 100), (300, 2, 2, 256, 16, 2, 250, 0),
+          (300, 2, 18, 256, 32, 32, 129, 0), (600, 1, 1, 200, 16, 16, 250, 0), (600, 2, 6, 80, 20, 4, 128, 0),
+          (600, 2, 2, 168, 12, 4, 220, 60), (600, 1, 3, 24, 1, 1, 90, 0), (1100, 2, 2, 104, 24, 8, 256, 0)]
+
+
+@pytest.mark.parametrize("case", range(len(NARROW)))
+def test_attention_one_wave(gpu, case):
+    sequences, heads, query_heads, width, page_tokens, block, longest, window = NARROW[case]
+    rng = np.random.default_rng(6100 + case)
+    lengths = rng.integers(0, longest + 1, sequences)
+    lengths[0] = longest
+    pages = -(-longest // page_tokens) + 3
+    # the sequences share a few pages: what is read is what counts here
+    table = rng.integers(0, pages, (sequences, pages)).astype(np.int32)
+    cache = CacheF8(rng, pages, page_tokens, heads, width, block, ("heads", "tokens")[case % 2], case % 3)
+    q = rng.standard_normal((sequences, query_heads, width)).astype((np.float32, np.float16)[case % 2])
+    y, route = run_attention(cache, table, lengths, q, window)
+    assert route == "paged_attention_f8"
+    gold, tol = gold_attention(cache, table, lengths, q, window, width ** -0.5)
+    check(y, gold, tol)
+    assert gpu.kv_cache_status(0) == 0
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("heads,width,page_tokens,block", [(32, 128, 16, 16), (9, 120, 16, 4), (64, 256, 64, 64), (5, 104, 20, 1)])
+def test_wide_tokens(gpu, heads, width, page_tokens, block, half):
+    """Tokens that several waves read back, the last one less than whole."""
+    rng = np.random.default_rng(6200)
+    dtype, parts = (np.float16 if half else np.float32), [(3, 20), (0, 1), (page_tokens, 2)]
+    lengths = [a + b for a, b in parts]
+    cache = CacheF8(rng, 12, page_tokens, heads, width, block)
+    table = table_of(rng, lengths, page_tokens, 12, 3)
+    sequence = np.concatenate([np.full(n, s) for s, (_, n) in enumerate(parts)])
+    position = np.concatenate([np.arange(a, a + n) for a, n in parts])
+    q, k, v = (rng.standard_normal((len(sequence), h, width)).astype(dtype) for h in (heads + 3, heads, heads))
+    cos, sin = angles(max(lengths), width // 2)
+    model = cache.copy()
+    stored, status = model_append(model, table, sequence, position, k, v, cos, sin, HALVES, width)
+    cache.upload()
+    y = run_append(cache, table, sequence, position, q, k, v, cos, sin, HALVES, width)
+    cache.download()
+    assert cache.same_as(model)
+    check_queries(y, q, stored, position, cos, sin, HALVES, width)
+    of, at = np.concatenate([np.full(n, s) for s, n in enumerate(lengths)]), np.concatenate([np.arange(n) for n in lengths])
+    for kind, common in ((np.float32, False), (np.float16, True)):
+        for a, b in zip(run_read(cache, table, of, at, kind, common=common), model_read(model, table, of, at, kind)):
+            assert np.array_equal(a, b)
+    assert gpu.kv_cache_status(0) == 0
