@@ -537,7 +537,8 @@ bool paged_attention_f8(Kernel &, int device, void * y, const void * q, const vo
 // makes its block's scale, so all of the block, not a number, until the block is begun again. Tokens of one block must
 // stand in consecutive entries of consecutive positions (some of which may be left out); what the block held from the first
 // of them on is forgotten. A list that breaks this rule is reported, and the blocks concerned hold nothing of use.
-// Up to 2^31 threads: (query_heads * width / 8 + 512 * heads) * tokens.
+// (query_heads * width / 8 + 512 * heads) * tokens stays below 2^31 - 1024; longer lists go in several calls, parted where a
+// block begins.
 const char * kv_append_f8_reason(const KVCacheF8Layout &, const KVAppendLayout &);
 bool kv_append_f8(Kernel &, int device, void * k_pool, void * v_pool, float * k_scales, float * v_scales, void * q_out,
                   const void * q, const void * k, const void * v, const int * sequence, const int * position,

@@ -18,7 +18,6 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kStep = 32;                // tokens of a wave's step
-constexpr float kWeightScale = 16384.0f; // of the weights' F16 parts
 constexpr float kLeastPart = 0x1p-24f;    // the least F16 above 0
 
 struct AttendArgs {
@@ -211,22 +210,6 @@ __device__ __forceinline__ void whole_scores(const float4v (&scores)[2], float u
             const float high = c < 8 ? part : other;
             if (fabsf(high) == INFINITY) sc[i] = high;
         }
-    }
-}
-
-// The second product: value j of a lane's eight tokens, picked out of their rows, times the weights.
-template <int VW, int NT>
-__device__ __forceinline__ void add_values(const uint32_t (&vr)[8][VW / 2], const half8 (&pf)[NT], float4v (&acc)[NT][VW]) {
-#pragma unroll
-    for (int j = 0; j < VW; ++j) {
-        union { uint32_t u[4]; half8 h; } vf;
-        const int word = (j / 8) * 4 + (j % 8) / 2;
-        const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) vf.u[u] = __builtin_amdgcn_perm(vr[2 * u + 1][word], vr[2 * u][word], pick);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-            acc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, pf[nt], acc[nt][j], 0, 0, 0);
     }
 }
 

@@ -33,7 +33,7 @@ constexpr int kThreads = 256;
 constexpr int kLeastExponent = -64;      // of a scale
 constexpr int kMostGroups = 2048;        // that look through one entry each
 constexpr int kMostWaves = 16;           // of a workgroup
-constexpr int kPlaces = 4096;            // of a checking workgroup's table, 16 KB: a CU's 160 hold as many workgroups as its registers
+constexpr int kPlaces = 4096;            // of a checking workgroup's table, 16 KB: no fewer workgroups fit on a CU
 constexpr int kCheckedAhead = 4;         // entries of a thread on their way
 
 typedef float float2v __attribute__((ext_vector_type(2)));
@@ -382,9 +382,9 @@ __device__ __forceinline__ void store_window(const F8Args &a, uint32_t item, int
 
 // Tokens of one block that stand apart in the list (k200.h forbids it) would each begin the block, and chance decides whose scale
 // stays. Such a list is reported: workgroup `part` enters the first of every run of a block's tokens, where the hash of sequence
-// and block gives it this part, in a table of LDS, and finds there a run of the same block that this one does not go on from. Half
-// a table's places for a part's share of the list; were all taken, the search ends without an answer. Beside the others' work
-// (32 sequences x 32 heads 5.63 -> 5.77 us a call, a prompt of 8000 tokens no change, of 100000 803 -> 818).
+// and block gives it this part, in a table of LDS, and finds there a run of the same block that this one does not go on from.
+// Half a table's places are for a part's share of the list; were all taken, the search would end without an answer. Beside the
+// others' work: 32 sequences x 32 heads 5.63 -> 5.77 us a call, a prompt of 8000 tokens no change, of 100000 803 -> 818.
 template <int THREADS>
 __device__ __forceinline__ void check_list(const F8Args &a, uint32_t part, int *places) {
     for (int x = threadIdx.x; x < kPlaces; x += THREADS) places[x] = -1;

@@ -48,7 +48,8 @@ const char * kv_append_f8_reason(const KVCacheF8Layout & f, const KVAppendLayout
     if (*cache) return cache;
     const char * call = kv_append_reason(f.cache, p);
     if (*call) return call;
-    // 64 lanes for a token's head and up to 128 of a workgroup that takes a block's, in a launch of fewer than 2^31 threads
+    // a bound that no launch comes near (a token's head takes up to 64 lanes and its part of a block's workgroup up to 128), so
+    // that the launch's numbers stay within 32 bits whatever the widths and blocks
     if ((p.query_heads * (int64_t)(f.cache.width / 8) + 2 * (int64_t)f.cache.heads * 256) * p.tokens > INT32_MAX - 1024)
         return "shape";
     return "";

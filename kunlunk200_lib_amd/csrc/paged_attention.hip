@@ -53,6 +53,7 @@ constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
 constexpr int kRowSteps = 1;             // what beginning a row counts in a share
 constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even goes through
+constexpr float kWeightScale = 16384.0f; // of the weights' F16 parts
 constexpr float kLeastWeight = 0x1p100f;  // p times this is above kLeastPart for every normal p
 
 // A step's scores to weights, high and low parts as the second product's columns; the maxima and sums so far move
@@ -90,6 +91,22 @@ __device__ __forceinline__ void weigh(const float4v (&scores)[NT][2], const floa
             const _Float16 high = static_cast<_Float16>(part);
             pf[nt][i] = c < 8 ? high : static_cast<_Float16>(p - static_cast<float>(high));
         }
+    }
+}
+
+// The second product: value j of a lane's eight tokens, picked out of their rows, times the weights.
+template <int VW, int NT>
+__device__ __forceinline__ void add_values(const uint32_t (&vr)[8][VW / 2], const half8 (&pf)[NT], float4v (&acc)[NT][VW]) {
+#pragma unroll
+    for (int j = 0; j < VW; ++j) {
+        union { uint32_t u[4]; half8 h; } vf;
+        const int word = (j / 8) * 4 + (j % 8) / 2;
+        const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) vf.u[u] = __builtin_amdgcn_perm(vr[2 * u + 1][word], vr[2 * u][word], pick);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            acc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.h, pf[nt], acc[nt][j], 0, 0, 0);
     }
 }
 

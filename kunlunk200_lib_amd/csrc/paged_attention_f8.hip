@@ -37,7 +37,7 @@ constexpr int kMinChunk = kWaves * kStep;
 constexpr int kMaxChunk = 512, kMaxChunkMany = 1024;
 constexpr int kMostChunks = 65535;       // the grid's limit
 constexpr int64_t kMostIds = 8000;       // page ids of a chunk in LDS, 32 KB
-constexpr int kRowSteps = 2;             // what beginning a row counts in a share (64 ragged to 2048 x 8 heads 40.0 us, 1: 44.0)
+constexpr int kRowSteps = 2;             // what beginning a row counts in a share (64 ragged to 2048 x 8 38.7 us, 1: 41.1, 3: 38.6)
 constexpr int kMostEven = 1024;          // sequences whose lengths a workgroup of attend_even_f8 goes through
 constexpr int kLift = 13;                // exponent of the largest weight times its scale, as F16 parts
 constexpr int kMostLift = 126;           // of the power that takes it there, whose reciprocal is a normal number too
@@ -698,9 +698,17 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     const int longest = p.window > 0 ? std::min<int64_t>(p.longest, (int64_t)p.window + kStep - 1) : p.longest;
     const int64_t rows = (int64_t)p.sequences * c.heads * r.tiles;
     // The rules are the F16 cache's (rows whole on eight waves or four, parts of one size, equal shares), whose chains of
-    // latencies they balance and which are the same here; measured for this cache (us): 1 x 32768 tokens x 8 heads in parts of
-    // 512 21.3, of 256 24.5; 64 x 1024 x 8 whole 23.5 ragged and 27.3 full, in shares 26.7 and 35.1; 200 x 700 x 8 whole 43,
-    // in shares 47.6, on eight waves 64.8.
+    // latencies they balance. Both sides of each for this cache, of one build (us a call; heads of 128, ragged where not full):
+    // - eight waves to a whole row / parts: 8, 16 and 32 x 512 tokens x 8 heads 9.0 / 10.4, 9.3 / 11.9 and 9.6 / 13.6; 32 x 768
+    //   11.3 / 15.4, 32 x 1024 13.1 / 17.1; 8 x 1024 12.3 / 12.0, windows of 1000 in 7 x 5 heads of 80 16.9 / 13.7. Fewer rows
+    //   of 768 are parted, though 16 x 768 x 8 would take 11.3 whole and takes 13.6.
+    // - four waves to a whole row / equal shares: 64 x 1024 x 8 23.0 / 26.6, full 26.3 / 34.5; 200 x 700 x 8 41.0 / 47.0 (on
+    //   eight waves 55.8); token by token 49.2 / 47.3, 200 x 1000 67.4 / 59.2; 300 x 500 x 4 heads of 256 53.9 / 55.0.
+    // - parts of 256, 512 and 1024 tokens: 1 x 32768 x 8 22.1, 20.1 and 19.6; 64 x 2048 x 2 in 512, 1024 and whole 16.7, 19.0 and
+    //   23.8; 128 x 3000 x 5 in 512, 1024 and 1536 63.0, 60.3 and 59.7; 48 full rows of 544 x 8 whole 14.8, in 256 20.1.
+    // - parts / equal shares: 64 x 2048 x 8 48.9 / 38.7; 32 x 4096 x 32 106.0 / 102.2; 64 x 2048 x 4 of 256 52.3 / 43.5.
+    // - the non-temporal hint (`once`), without / with: 200 x 700 x 8 42.0 / 40.5; 96 x 900 x 8, whose 92 MB the 256 MiB
+    //   cache holds from call to call, 25.3 / 26.3.
     const int whole = kMaxChunk + kStep;             // a window starts up to kStep - 1 tokens early
     r.wide = r.nt == 1 && c.width <= 128 && rows <= cus && longest > kMinChunk &&
              longest <= (rows > cus / 2 ? 2 * whole : whole);
@@ -719,8 +727,8 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
     r.chunk = static_cast<int>((chunk + kMinChunk - 1) / kMinChunk * kMinChunk);
     r.chunks = (longest + r.chunk - 1) / r.chunk;
     // One wave to a workgroup for many rows of up to four steps, or eight where the rows are very many or four waves' registers
-    // leave a CU to one workgroup (us on four waves and on one, 250 tokens ragged: 512 sequences x 8 heads 52.3 / 45.6; 300 x 4
-    // heads of 256 37.6 / 30.6; but 300 x 8 of 64 20.8 / 22.9, and 80 x 8, full rows, 14.3 / 18.1)
+    // leave a CU to one workgroup (us on four waves and on one, 250 tokens ragged: 512 sequences x 8 heads 46.6 / 44.5, of 120
+    // tokens 36.3 / 25.8; 300 x 4 heads of 256 33.7 / 26.9; but 300 x 8 of 64 18.7 / 20.9, and 80 x 8, full rows, 14.0 / 15.3)
     const bool eight = c.width > 128 || (c.width > 64 && rows > 8 * cus);
     r.narrow = r.nt == 1 && rows > 2 * cus && longest <= (eight ? 8 : 4) * kStep;
     r.once = r.tiles == 1 && (int64_t)p.sequences * longest * c.heads * c.width * 2 > (64 << 20);
@@ -731,8 +739,8 @@ Plan plan_of(const kunlun::KVCacheLayout &c, const kunlun::PagedAttentionLayout 
         (c.width % 64 == 0 || c.width == 96) && p.sequences <= kMostEven &&
         (p.sequences > 1 || (int64_t)longest * c.heads * c.width * 2 > (256 << 20)) &&
         (int64_t)p.sequences * c.heads * (longest / kStep + 3) < INT32_MAX)
-        // two workgroups to a CU, whose registers allow it up to width 128 (64 sequences ragged to 2048 x 8 heads of 128 39.1 us,
-        // one 45.5; 32 x 32768 335 and 398; three, which spill, 375; 4 heads of 256 one 48.3, two 55.6)
+        // two workgroups to a CU, whose registers allow it up to width 128 (64 sequences ragged to 2048 x 8 heads of 128 38.7 us
+        // a call, one 48.3, three 48.6; 32 x 32768 347, 417 and 373; 4 heads of 256 one 43.5, two 49.4)
         r.shares = c.width <= 128 ? 2 * cus : cus;
     return r;
 }
