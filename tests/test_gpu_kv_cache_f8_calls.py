@@ -236,7 +236,7 @@ def test_append_reports_blocks_in_pieces(gpu, block, width, half):
         "backwards": (np.zeros(9, int), np.arange(9, 0, -1)),
         "a gap": (np.zeros(4, int), np.array([0, 1, block, 1])),
         "far off": (np.concatenate([[0], together[0], [0]]), np.concatenate([[block - 1], together[1], [0]])),
-        "one place twice": (np.concatenate([[1], together[0], [1]]), np.concatenate([[5], together[1], [5]])),
+        "far off, the first first": (np.concatenate([[1], together[0], [1]]), np.concatenate([[0], together[1], [block - 1]])),
     }
     for name, (sequence, position) in lists.items():
         print(name, flush=True)
